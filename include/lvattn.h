@@ -26,13 +26,14 @@
  *   [6] band + 1  0: plain causal rule.  b + 1: key k_row0+j visible to query q_row0+i iff i + shift - b <= j <= i + shift
  *                (a query sees itself and the b keys before it: pre_tockens / --sliding-window,
  *                dot_product_attention.py:403-406, 462; written by the *_band builders, read by launches with causal == 2)
- *   [7] reserved, must be 0
+ *   [7] prefix  lvattn_fwd_score / lvattn_bwd_score: swept keys [0, prefix) are visible to every row beside the causal rule
+ *               (<= 0: none; the tables of lv_build_score_blocks); 0 in every other table
  * The backward kernels use the transposed descriptor (one per key block):
  *   [0] k_row0  [1] k_rows (1 .. LV_BWD_BLOCK_N)  [2] q_row0  [3] q_len
  *   [4] shift   key k_row0+j visible to query q_row0+i iff j <= i + shift (q_row0 is the first
  *               32-aligned query row that sees any key of the block)
  *   [5] out_delta  dk / dv rows go to row k_row0 + out_delta + j
- *   [6] band + 1   as above
+ *   [6] band + 1, [7] prefix (counted from k_row0)   as above
  */
 #ifndef LVATTN_H
 #define LVATTN_H
@@ -187,6 +188,36 @@ int lvattn_combine_lse(const void* ws_out, const float* ws_lse, void* out, float
                        void* stream);
 int lvattn_combine_sum(const float* ws, void* out, const int32_t* comb_dev, int n_comb, int block_rows, int heads, int d,
                        int64_t o_row_stride, int64_t o_head_stride, void* stream);
+
+/* ---- scores with a rule of their own ----------------------------------------------
+ * Packed attention, forward and backward, whose scores are changed before the softmax:
+ *   t_ij = cap * tanh(scale * q_i.k_j / cap) - slope[head] * |i - j|
+ * softcap = 0: no cap; slopes = NULL: no bias (fp32 [hq] in device memory; at most 64 query heads per KV head).  A key is
+ * visible to the rows of its segment at and after it (causal != 0) or to all of them, to every row of the segment when it
+ * lies below the segment's prefix length, and with band >= 0 only to the `band` rows after it.  The reference caps scores
+ * in its eager path (lcvlm_modellink/core/transformer/dot_product_attention.py:222-225) and hands alibi to the fused op as a
+ * full [s, s] bias (:113, :411-424); here both are computed where the score is.
+ *   lv_build_score_blocks  host, pure CPU: the work-item table, forward / dQ (backward == 0) or dK/dV form.  prefix_host [n_seg] or
+ *       NULL, band < 0 = none (a band goes with causal and without a prefix).  piece == 0: whole sweeps, results at their own
+ *       rows.  piece > 0 (multiple of 64 forward, 32 backward): sweeps cut every `piece` elements, results in workspace rows,
+ *       combine entries in comb_host as for lv_build_fwd_blocks_split.  desc_host == NULL only counts.  Returns the count.
+ *   lv_plan_score_split    host: the piece length for a launch of these sweeps, 0 = leave them whole.
+ *   lvattn_fwd_score / lvattn_bwd_score  as lvattn_fwd / lvattn_bwd on such tables; delta from lvattn_bwd_delta. */
+int lv_build_score_blocks(const int32_t* cu_seqlens_host, int n_seg, int causal, int band, const int32_t* prefix_host, int backward, int piece,
+                          int32_t* desc_host, int max_blocks, int32_t* comb_host, int max_comb, int* n_comb, int* ws_rows);
+int lv_plan_score_split(const int32_t* cu_seqlens_host, int n_seg, int causal, int band, const int32_t* prefix_host, int backward, int hq, int hkv,
+                        int n_cu);
+int lvattn_fwd_score(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* desc_dev, int n_blocks,
+                     int q_rows_total, int k_rows_total, int hq, int hkv, int d, int64_t q_row_stride, int64_t q_head_stride,
+                     int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, int64_t o_row_stride,
+                     int64_t o_head_stride, int64_t lse_stride, float softmax_scale, float softcap, const float* slopes, void* stream);
+int lvattn_bwd_score(const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dq, void* dk,
+                     void* dv, const int32_t* qdesc_dev, int n_qblocks, const int32_t* kdesc_dev, int n_kblocks, int q_rows_total,
+                     int k_rows_total, int hq, int hkv, int d, int64_t q_row_stride, int64_t q_head_stride, int64_t k_row_stride,
+                     int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, int64_t do_row_stride, int64_t do_head_stride,
+                     int64_t dq_row_stride, int64_t dq_head_stride, int64_t dk_row_stride, int64_t dk_head_stride, int64_t dv_row_stride,
+                     int64_t dv_head_stride, int64_t lse_stride, float softmax_scale, float softcap, const float* slopes, int accum_f32,
+                     void* stream);
 
 /* ---- incremental attention over a KV cache -------------------------------------
  * Replaces torch_npu.npu_incre_flash_attention as called with --use-kv-cache

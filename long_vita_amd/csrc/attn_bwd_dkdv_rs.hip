@@ -68,7 +68,7 @@ __device__ __forceinline__ void rs_dma4(const float* g, uint32_t lds_dst) {
                  : "=&s"(keep) : "v"(g), "s"(lds_dst) : "memory");
 }
 
-template <int D, bool CAUSAL, bool ACCUM_F32, int NSL>
+template <int D, bool CAUSAL, bool ACCUM_F32, int NSL, int MOD = 0>
 __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
     constexpr int NW = 8;
     constexpr int BQ = 32;             // query rows per unit (one 32-row slice of one head)
@@ -222,6 +222,12 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[mt][i] = 0.f;
     const float c = p.scale_log2e;
+    float slope_v = 0.f;   // lane g: -log2(e) times the slope of head g of the group (at most 64)
+    if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
+        if (lane < p.group) slope_v = -1.4426950408889634f * p.score.slopes[kvh * p.group + lane];
+        asm volatile("" : "+v"(slope_v));
+    }
+    const int pre = MOD != 0 ? dsc.prefix : 0;   // keys of the block below this are visible to every row
 
     // Both roles run the SAME loop, with role-dependent operand addresses, the K-waves one barrier
     // behind the V-waves.  An iteration handles NSL units u:
@@ -326,30 +332,52 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
                 const int i0 = c_sl * BQ;  // first query row of the unit, relative to q_row0
                 const bool dead_unit = (NSL > 1) && (c_n >= nunits);
                 ++c_n;
+                float nslope2 = 0.f;
+                if constexpr ((MOD & LV_SCORE_BIAS) != 0) nslope2 = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(slope_v), c_hg));
                 if (++c_hg == p.group) { c_hg = 0; --c_sl; }
                 if (!is_k) {
-                    const bool need_mask = dead_unit || (kbase_w + 31 > i0 + shift) || (i0 + BQ > q_len) || (kbase_w + 32 > k_rows) ||
+                    const bool need_mask = dead_unit || (kbase_w + 31 > (MOD != 0 ? max(i0 + shift, pre - 1) : i0 + shift)) || (i0 + BQ > q_len) || (kbase_w + 32 > k_rows) ||
                                            (kbase_w < i0 + BQ - 1 + band_low);
                     float pv[16];
+                    if constexpr (MOD != 0) {
+                        static_assert(MOD == 0 || !LV_RS_CFOLD, "the folded constants belong to the plain score");
+                        const float fk = (float)(i0 + shift - kj + 4 * h);   // distance of the lane's first row of the unit to its key
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            float g;
+                            const float t = lv_score<MOD>(x[u][i], c, p.score, nslope2, fk + (float)((i & 3) + 8 * (i >> 2)), &g);
+                            pv[i] = fast_exp2(t + cst[u][i >> 2][i & 3]);
+                            if constexpr ((MOD & LV_SCORE_CAP) != 0) x[u][i] = g;
+                        }
+                    } else {
 #pragma unroll
 #if LV_RS_CFOLD
                     for (int i = 0; i < 16; ++i) pv[i] = fast_exp2(x[u][i]);
 #else
                     for (int i = 0; i < 16; ++i) pv[i] = fast_exp2(__builtin_fmaf(x[u][i], c, cst[u][i >> 2][i & 3]));
 #endif
+                    }
                     if (need_mask) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             int ii = i0 + (i & 3) + 8 * (i >> 2) + 4 * h;
-                            bool dead = (kj > ii + shift) | (kj < ii + band_low) | (ii >= q_len) | (kj >= k_rows) | dead_unit;
+                            bool dead = (kj > (MOD != 0 ? max(ii + shift, pre - 1) : ii + shift)) | (kj < ii + band_low) | (ii >= q_len) | (kj >= k_rows) | dead_unit;
                             pv[i] = dead ? 0.f : pv[i];
                             asm volatile("" : "+v"(pv[i]));  // keeps this a branch
                         }
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) y[u][i >> 3][i & 7] = (__bf16)pv[i];
+                    if constexpr ((MOD & LV_SCORE_CAP) != 0) {   // the partner forms dS = P (1 - tanh^2) (dP - delta): it gets the first two factors
+                        bf16x8 z[2];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) z[i >> 3][i & 7] = (__bf16)(pv[i] * x[u][i]);
+                        *(LDS_PTR(bf16x8, p_ptr + u * PBUF)) = z[0];
+                        *(LDS_PTR(bf16x8, p_ptr + u * PBUF + 1024)) = z[1];
+                    } else {
                     *(LDS_PTR(bf16x8, p_ptr + u * PBUF)) = y[u][0];
                     *(LDS_PTR(bf16x8, p_ptr + u * PBUF + 1024)) = y[u][1];
+                    }
                 } else {
                     bf16x8 pf[2];
                     pf[0] = *(LDS_PTR(bf16x8, p_ptr + u * PBUF));
@@ -500,6 +528,25 @@ static void launch_rs(const BwdParams& p, int causal, int accum, hipStream_t str
         if (accum) hipLaunchKernelGGL((lv_bwd_dkdv_rs_kernel<D, false, true, NSL>), grid, block, lds, stream, p);
         else hipLaunchKernelGGL((lv_bwd_dkdv_rs_kernel<D, false, false, NSL>), grid, block, lds, stream, p);
     }
+}
+
+template <int D, int MOD>
+static void launch_rs_score(const BwdParams& p, int accum, hipStream_t stream) {
+    const dim3 grid((unsigned)((((int64_t)p.n_blocks * p.hkv + 7) / 8) * 8)), block(512);
+    const size_t lds = (size_t)4 * 2 * (2 * 32 * D * 2 + 256) + (size_t)2 * 4 * 2048;   // two units per iteration, staged two iterations ahead
+    if (accum) hipLaunchKernelGGL((lv_bwd_dkdv_rs_kernel<D, true, true, 2, MOD>), grid, block, lds, stream, p);
+    else hipLaunchKernelGGL((lv_bwd_dkdv_rs_kernel<D, true, false, 2, MOD>), grid, block, lds, stream, p);
+}
+
+int lv_launch_bwd_dkdv_rs_score(const BwdParams& p, int d, int accum, int mod, hipStream_t stream) {
+    if (p.n_blocks <= 0) return 0;
+    switch (mod & (LV_SCORE_CAP | LV_SCORE_BIAS)) {
+        case 0: d == 128 ? launch_rs_score<128, 4>(p, accum, stream) : launch_rs_score<64, 4>(p, accum, stream); break;
+        case LV_SCORE_CAP: d == 128 ? launch_rs_score<128, 5>(p, accum, stream) : launch_rs_score<64, 5>(p, accum, stream); break;
+        case LV_SCORE_BIAS: d == 128 ? launch_rs_score<128, 6>(p, accum, stream) : launch_rs_score<64, 6>(p, accum, stream); break;
+        default: d == 128 ? launch_rs_score<128, 7>(p, accum, stream) : launch_rs_score<64, 7>(p, accum, stream);
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
 int lv_launch_bwd_dkdv_rs(const BwdParams& p, int d, int causal, int accum, hipStream_t stream) {

@@ -35,7 +35,7 @@ __device__ __forceinline__ void dq_dma16(__amdgpu_buffer_rsrc_t rs, int voff, ui
                  : "=&s"(keep) : "v"(voff), "s"(rs), "s"(lds_dst) : "memory");
 }
 
-template <int D, bool CAUSAL, bool ACCUM_F32>
+template <int D, bool CAUSAL, bool ACCUM_F32, int MOD = 0>
 __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
     constexpr int BN = 32;            // keys per tile
     constexpr int KS = D / 16;
@@ -95,10 +95,12 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
     float delta = p.delta[(int64_t)head * p.lse_stride + q_row];
 
     int limit = qi + shift;
+    if constexpr (MOD != 0) limit = max(limit, dsc.prefix - 1);
     if (limit > k_len - 1 || qi >= q_rows) limit = k_len - 1;
     const int band_low = CAUSAL ? lv_band_low(dsc) : -(1 << 29);   // the band's lower end, when the descriptor has one
     const int low = qi + band_low;
     int wave_kmax = 32 * w + 32 + shift;
+    if constexpr (MOD != 0) wave_kmax = max(wave_kmax, dsc.prefix);
     wave_kmax = wave_kmax < 0 ? 0 : (wave_kmax > k_len ? k_len : wave_kmax);
     const int nkt = (k_len + BN - 1) / BN;
     const int my_nkt = (32 * w < q_rows) ? (wave_kmax + BN - 1) / BN : 0;
@@ -163,6 +165,11 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) { asm volatile("" : "+v"(qf[ks])); asm volatile("" : "+v"(dof[ks])); }
     asm volatile("" : "+v"(lse2), "+v"(delta));
+    float nslope2 = 0.f;
+    if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
+        nslope2 = -1.4426950408889634f * p.score.slopes[head];
+        asm volatile("" : "+v"(nslope2));
+    }
 
     // fragments of one MFMA group: SPG K rows, SPG V rows (slot sb_new), QPG K columns (slot sb_old)
     bf16x8 kfr[2][SPG], vfr[2][SPG], tfr[2][QPG];
@@ -205,12 +212,22 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
             // ================= VALU(t): dS_t =================
             if (t < my_nkt) {
                 const int kb0 = t * BN;
-                const bool need_mask = (kb0 + BN - 1 > 32 * w + shift) || (kb0 + BN > k_len) || (kb0 < 32 * w + 31 + band_low);
+                const bool need_mask = (kb0 + BN - 1 > (MOD != 0 ? max(32 * w + shift, dsc.prefix - 1) : 32 * w + shift)) || (kb0 + BN > k_len) || (kb0 < 32 * w + 31 + band_low);
                 // all the multiply-adds, then all the exponentials, then their consumers: back to back a
                 // dependent pair would stall on the first one's latency sixteen times over
                 float pv[16];
+                if constexpr (MOD != 0) {
+                    const float fq = (float)(qi + shift - kb0 - 4 * h);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) pv[i] = __builtin_fmaf(s[i], c, -lse2);
+                    for (int i = 0; i < 16; ++i) {
+                        float g;
+                        pv[i] = lv_score<MOD>(s[i], c, p.score, nslope2, fq - (float)((i & 3) + 8 * (i >> 2)), &g) - lse2;
+                        if constexpr ((MOD & LV_SCORE_CAP) != 0) s[i] = g;   // the score's own derivative, for dS below
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) pv[i] = __builtin_fmaf(s[i], c, -lse2);
+                }
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) pv[i] = fast_exp2(pv[i]);
@@ -224,7 +241,11 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
                     }
                 }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) dsf[i >> 3][i & 7] = (__bf16)(pv[i] * (dp[i] - delta));
+                for (int i = 0; i < 16; ++i) {
+                    float ds = pv[i] * (dp[i] - delta);
+                    if constexpr ((MOD & LV_SCORE_CAP) != 0) ds *= s[i];
+                    dsf[i >> 3][i & 7] = (__bf16)ds;
+                }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) { dsf[0][i] = (__bf16)0.f; dsf[1][i] = (__bf16)0.f; }
@@ -326,6 +347,25 @@ static void launch_dq_pp(const BwdParams& p, int causal, int accum, hipStream_t 
         if (accum) hipLaunchKernelGGL((lv_bwd_dq_pp_kernel<D, false, true>), grid, block, lds, stream, p);
         else hipLaunchKernelGGL((lv_bwd_dq_pp_kernel<D, false, false>), grid, block, lds, stream, p);
     }
+}
+
+template <int D, int MOD>
+static void launch_dq_pp_score(const BwdParams& p, int accum, hipStream_t stream) {
+    const dim3 grid((unsigned)((int64_t)p.n_qblocks * p.hq)), block(512);
+    const size_t lds = (size_t)5 * 2 * 32 * D * 2;
+    if (accum) hipLaunchKernelGGL((lv_bwd_dq_pp_kernel<D, true, true, MOD>), grid, block, lds, stream, p);
+    else hipLaunchKernelGGL((lv_bwd_dq_pp_kernel<D, true, false, MOD>), grid, block, lds, stream, p);
+}
+
+int lv_launch_bwd_dq_pp_score(const BwdParams& p, int d, int accum, int mod, hipStream_t stream) {
+    if (p.n_qblocks <= 0) return 0;
+    switch (mod & (LV_SCORE_CAP | LV_SCORE_BIAS)) {
+        case 0: d == 128 ? launch_dq_pp_score<128, 4>(p, accum, stream) : launch_dq_pp_score<64, 4>(p, accum, stream); break;
+        case LV_SCORE_CAP: d == 128 ? launch_dq_pp_score<128, 5>(p, accum, stream) : launch_dq_pp_score<64, 5>(p, accum, stream); break;
+        case LV_SCORE_BIAS: d == 128 ? launch_dq_pp_score<128, 6>(p, accum, stream) : launch_dq_pp_score<64, 6>(p, accum, stream); break;
+        default: d == 128 ? launch_dq_pp_score<128, 7>(p, accum, stream) : launch_dq_pp_score<64, 7>(p, accum, stream);
+    }
+    return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
 int lv_launch_bwd_dq_pp(const BwdParams& p, int d, int causal, int accum, hipStream_t stream) {

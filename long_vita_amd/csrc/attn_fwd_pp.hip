@@ -48,7 +48,7 @@ __device__ __forceinline__ void pp_dma16(__amdgpu_buffer_rsrc_t rs, int voff, ui
                  : "=&s"(keep) : "v"(voff), "s"(rs), "s"(lds_dst) : "memory");
 }
 
-template <int D, bool CAUSAL, bool ROPE = false>
+template <int D, bool CAUSAL, bool ROPE = false, int MOD = 0>
 __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
     constexpr int BN = 64;            // keys per tile
     constexpr int KS = D / 16;        // k-steps of the QK^T product
@@ -148,10 +148,12 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
     }
 
     int limit = qi + shift;  // visible keys (relative to k_row0) for this lane's row: j <= limit
+    if constexpr (MOD != 0) limit = max(limit, dsc.prefix - 1);
     if (limit > k_len - 1 || qi >= q_rows) limit = k_len - 1;
     const int band_low = CAUSAL ? lv_band_low(dsc) : -(1 << 29);   // ... and j >= qi + band_low when the descriptor has a band
     const int low = qi + band_low;
     int wave_kmax = 32 * w + 32 + shift;
+    if constexpr (MOD != 0) wave_kmax = max(wave_kmax, dsc.prefix);
     wave_kmax = wave_kmax < 0 ? 0 : (wave_kmax > k_len ? k_len : wave_kmax);
     const int nkt = (k_len + BN - 1) / BN;
     const int my_nkt = (32 * w < q_rows) ? (wave_kmax + BN - 1) / BN : 0;
@@ -209,7 +211,12 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) oacc[mt][i] = 0.f;
     float m_run = -1e30f, l_run = 0.f;
-    const float c = p.scale_log2e;
+    const float c = MOD != 0 ? 1.f : p.scale_log2e;   // (MOD: the scores become t, in log2 units, before the softmax sees them)
+    float nslope2 = 0.f;
+    if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
+        nslope2 = -1.4426950408889634f * p.score.slopes[head];
+        asm volatile("" : "+v"(nslope2));
+    }
     f32x16 s[2];
     bf16x8 pf[2][2];
 
@@ -242,7 +249,15 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
             // ================= VALU(t): softmax of S_t -> P_t =================
             if (t < my_nkt) {
                 const int kb0 = t * BN;
-                const bool need_mask = (kb0 + BN - 1 > 32 * w + shift) || (kb0 + BN > k_len) || (kb0 < 32 * w + 31 + band_low);
+                const bool need_mask = (kb0 + BN - 1 > (MOD != 0 ? max(32 * w + shift, dsc.prefix - 1) : 32 * w + shift)) || (kb0 + BN > k_len) || (kb0 < 32 * w + 31 + band_low);
+                if constexpr (MOD != 0) {
+                    const float fq = (float)(qi + shift - kb0 - 4 * h);   // distance of the row to the lane's first key of the tile
+#pragma unroll
+                    for (int st = 0; st < 2; ++st)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            s[st][i] = lv_score<MOD>(s[st][i], p.scale_log2e, p.score, nslope2, fq - (float)(32 * st + (i & 3) + 8 * (i >> 2)));
+                }
                 // Optimistic pass: once every row of the wave has a finite running maximum, P is formed
                 // against it WITHOUT looking for the tile's maximum first (a third of the softmax's
                 // instructions).  Scores far below the running maximum just give tiny P; a score far above
@@ -400,7 +415,8 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
                 *reinterpret_cast<bf16x4*>(optr + 32 * mt + 8 * g4 + 4 * h) = ov;
             }
         if (h == 0) {
-            float lse = (l_tot > 0.f) ? (m_run * p.scale + __logf(l_tot)) : -INFINITY;
+            const float unit = MOD != 0 ? 0.6931471805599453f : p.scale;
+            float lse = (l_tot > 0.f) ? (m_run * unit + __logf(l_tot)) : -INFINITY;
             p.lse[(int64_t)head * p.lse_stride + q_row0 + dsc.out_delta + qi] = lse;
         }
     }
@@ -426,6 +442,27 @@ static void launch_pp(const FwdParams& p0, int causal, hipStream_t stream) {
     }
     if (causal) hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true>), grid, block, lds, stream, p);
     else hipLaunchKernelGGL((lv_fwd_pp_kernel<D, false>), grid, block, lds, stream, p);
+}
+
+template <int D>
+static void launch_pp_score(const FwdParams& p0, int mod, hipStream_t stream) {
+    FwdParams p = p0;
+    p.head_per_xcd = lv_head_per_xcd(p) ? 1 : 0;
+    const dim3 grid(p.head_per_xcd ? (unsigned)(((p.hkv + 7) / 8) * 8 * p.n_blocks * p.group)
+                                   : (unsigned)((((int64_t)p.n_blocks * p.hkv + 7) / 8) * 8 * p.group)), block(512);
+    const size_t lds = (size_t)LV_PP_NS * 2 * 64 * D * 2;
+    switch (mod & (LV_SCORE_CAP | LV_SCORE_BIAS)) {
+        case 0: hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true, false, LV_SCORE_RULE>), grid, block, lds, stream, p); break;
+        case LV_SCORE_CAP: hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true, false, LV_SCORE_RULE | LV_SCORE_CAP>), grid, block, lds, stream, p); break;
+        case LV_SCORE_BIAS: hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true, false, LV_SCORE_RULE | LV_SCORE_BIAS>), grid, block, lds, stream, p); break;
+        default: hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true, false, LV_SCORE_RULE | LV_SCORE_CAP | LV_SCORE_BIAS>), grid, block, lds, stream, p);
+    }
+}
+
+int lv_launch_fwd_pp_score(const FwdParams& p, int d, int mod, hipStream_t stream) {
+    if (d == 128) launch_pp_score<128>(p, mod, stream);
+    else launch_pp_score<64>(p, mod, stream);
+    return hipGetLastError() == hipSuccess ? 0 : -2;
 }
 
 int lv_launch_fwd_pp(const FwdParams& p, int d, int causal, hipStream_t stream) {

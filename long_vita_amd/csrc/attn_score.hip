@@ -1,0 +1,216 @@
+// Attention whose scores follow a rule of their own: a tanh cap, a bias that grows with distance, a prefix that every row of
+// its segment sees.  Forward and backward, packed segments.
+//
+//   s_ij = scale q_i.k_j;  u_ij = cap tanh(s_ij / cap) (or s_ij);  t_ij = u_ij - slope_h |i - j|
+//   visible: same segment and (j <= i or j < prefix) and (no band or j >= i - band)
+//   O_i = sum_j softmax_j(t_ij) v_j,  lse_i = log sum_j exp t_ij
+//   dT = P (dP - delta);  dS = dT (1 - tanh^2);  dQ = scale dS K;  dK = scale dS^T Q;  dV = P^T dO
+//
+// The products are those of plain attention, so the kernels are the ping-pong forward, the ping-pong dQ and the role-split
+// dK/dV kernels instantiated with the rule applied to every raw product in their vector phase (lv_score in internal.h).  What
+// the rule needs is not the matrix pipe: a cap adds an exponential and a reciprocal to the one exponential of the softmax.
+// This file holds the host side: work-item tables that know the prefix and the band (whole sweeps or sweeps cut into
+// pieces), the choice of the piece length, and the entry points.
+#include "internal.h"
+#include "../../include/lvattn.h"
+
+#include <algorithm>
+#include <cstring>
+#include <exception>
+#include <vector>
+
+namespace {
+
+constexpr int kFwdRows = 256;
+constexpr int kBwdKeys = LV_BWD_BLOCK_N_INTERNAL;
+
+// a: the rows a work item owns, b: the range it sweeps; shift / prefix relative to the first swept (forward) or owned
+// (backward) key: key j visible to row i iff j <= i + shift or j < prefix
+struct Sweep { int a0, an, b0, bn, shift, prefix, band_p1; };
+
+void sweeps_of(const int32_t* cu, int n_seg, int causal, int band, const int32_t* prefix, bool backward, std::vector<Sweep>& out) {
+    for (int s = 0; s < n_seg; ++s) {
+        const int base = cu[s], len = cu[s + 1] - cu[s];
+        // without the causal rule every key is a prefix key
+        const int pre = !causal ? len : (prefix ? std::min(prefix[s], len) : 0);
+        const int band_p1 = band >= 0 ? band + 1 : 0;
+        if (!backward) {
+            for (int m = 0; m < len; m += kFwdRows) {
+                const int rows = std::min(kFwdRows, len - m);
+                const int first = band >= 0 ? std::max(0, m - band) & ~63 : 0;   // sweeps start on a 64-key tile
+                const int end = std::max(m + rows, pre);
+                out.push_back({base + m, rows, base + first, end - first, m - first, pre - first, band_p1});
+            }
+        } else {
+            for (int n = 0; n < len; n += kBwdKeys) {
+                const int keys = std::min(kBwdKeys, len - n);
+                const int first = n < pre ? 0 : n & ~31;                          // unit slices start on 32 rows
+                const int end = band >= 0 ? (int)std::min<int64_t>(len, (int64_t)n + keys + band) : len;
+                out.push_back({base + n, keys, base + first, end - first, first - n, pre - n, band_p1});
+            }
+        }
+    }
+}
+
+int check_segments(const int32_t* cu, int n_seg, int causal, int band, const int32_t* prefix) {
+    if (!cu || n_seg < 0) return lv_fail(LV_EINVAL, "cu_seqlens is null or n_seg < 0");
+    for (int i = 0; i < n_seg; ++i)
+        if (cu[0] < 0 || cu[i + 1] < cu[i]) return lv_fail(LV_EINVAL, "cu_seqlens must start at 0 or above and not decrease (entry %d)", i);
+    if (band >= 0 && (!causal || prefix)) return lv_fail(LV_EINVAL, "a band goes with the causal rule and without a prefix");
+    if (prefix && !causal) return lv_fail(LV_EINVAL, "a prefix goes with the causal rule");
+    for (int i = 0; prefix && i < n_seg; ++i)
+        if (prefix[i] < 0) return lv_fail(LV_EINVAL, "prefix_lens[%d] = %d < 0", i, prefix[i]);
+    return 0;
+}
+
+int build(const std::vector<Sweep>& base, int piece, bool backward, int32_t* desc, int max_blocks, int32_t* comb, int max_comb, int* n_comb,
+          int* ws_rows) {
+    struct Out { int32_t v[LV_DESC_INTS]; int64_t work; };
+    const int block = backward ? kBwdKeys : kFwdRows;
+    std::vector<Out> items;
+    int64_t ws = 0;
+    int nc = 0;
+    for (const Sweep& b : base) {
+        const int np = (piece > 0 && b.bn > piece) ? (b.bn + piece - 1) / piece : 1;
+        if (comb) {
+            if (nc >= max_comb) return lv_fail(LV_ESIZE, "room for %d combine entries", max_comb);
+            const int32_t c[4] = {b.a0, b.an, (int32_t)ws, np};
+            memcpy(comb + 4 * (size_t)nc, c, sizeof(c));
+        }
+        ++nc;
+        for (int p = 0; p < np; ++p) {
+            const int cut = piece > 0 ? p * piece : 0;
+            const int len = piece > 0 ? std::min(piece, b.bn - cut) : b.bn;
+            Out o{};
+            // a forward piece starts `cut` keys later (keys counted from there), a backward piece `cut` rows later
+            const int shift = backward ? b.shift + cut : b.shift - cut;
+            const int prefix = backward ? b.prefix : b.prefix - cut;
+            const int32_t v[LV_DESC_INTS] = {b.a0, b.an, b.b0 + cut, len, shift, piece > 0 ? (int32_t)(ws - b.a0) : 0, b.band_p1, prefix};
+            memcpy(o.v, v, sizeof(v));
+            o.work = (int64_t)b.an * len;
+            items.push_back(o);
+            ws += block;
+            if (ws > 0x7fffffffLL) return lv_fail(LV_ESIZE, "too many workspace rows");
+        }
+    }
+    if (n_comb) *n_comb = nc;
+    if (ws_rows) *ws_rows = (int)ws;
+    if (desc) {
+        if ((int64_t)items.size() > max_blocks) return lv_fail(LV_ESIZE, "need %lld block descriptors, room for %d", (long long)items.size(), max_blocks);
+        std::stable_sort(items.begin(), items.end(), [](const Out& a, const Out& b) { return a.work > b.work; });
+        for (size_t i = 0; i < items.size(); ++i) memcpy(desc + i * LV_DESC_INTS, items[i].v, sizeof(items[i].v));
+    }
+    return (int)items.size();
+}
+
+int check_rule(int d, int hq, int hkv, float softmax_scale, float softcap, const float* slopes) {
+    if (!(softcap >= 0.f) || softcap > 1e30f) return lv_fail(LV_EINVAL, "softcap %g must be a finite number above 0 (0: no cap)", (double)softcap);
+    if (!(softmax_scale > -1e30f && softmax_scale < 1e30f)) return lv_fail(LV_EINVAL, "softmax_scale is not finite");
+    if (slopes && hq / hkv > 64) return lv_fail(LV_EINVAL, "slopes: %d query heads per KV head (at most 64)", hq / hkv);
+    return 0;
+}
+
+}  // namespace
+
+ScoreRule lv_score_rule(float scale, float softcap, const float* slopes) {
+    ScoreRule r;
+    r.cap_in = softcap > 0.f ? (float)(2.0 * 1.4426950408889634 * (double)scale / (double)softcap) : 0.f;
+    r.cap_out = softcap * 1.4426950408889634f;
+    r.slopes = slopes;
+    return r;
+}
+int lv_score_mod(float softcap, const float* slopes) {
+    return LV_SCORE_RULE | (softcap > 0.f ? LV_SCORE_CAP : 0) | (slopes ? LV_SCORE_BIAS : 0);
+}
+
+extern "C" int lv_build_score_blocks(const int32_t* cu, int n_seg, int causal, int band, const int32_t* prefix_host, int backward, int piece,
+                                     int32_t* desc, int max_blocks, int32_t* comb, int max_comb, int* n_comb, int* ws_rows) {
+    try {
+        if (int e = check_segments(cu, n_seg, causal, band, prefix_host)) return e;
+        if (piece < 0 || piece % (backward ? 32 : 64)) return lv_fail(LV_EINVAL, "piece length %d", piece);
+        std::vector<Sweep> base;
+        sweeps_of(cu, n_seg, causal, band, prefix_host, backward != 0, base);
+        return build(base, piece, backward != 0, desc, max_blocks, comb, max_comb, n_comb, ws_rows);
+    } catch (const std::exception& e) {
+        return lv_fail(LV_ESIZE, "lv_build_score_blocks: %s", e.what());
+    }
+}
+
+extern "C" int lv_plan_score_split(const int32_t* cu, int n_seg, int causal, int band, const int32_t* prefix_host, int backward, int hq, int hkv,
+                                   int n_cu) {
+    try {
+        if (int e = check_segments(cu, n_seg, causal, band, prefix_host)) return e;
+        if (hq <= 0 || hkv <= 0 || hq % hkv || n_cu <= 0) return lv_fail(LV_EINVAL, "heads %d / %d, %d compute units", hq, hkv, n_cu);
+        std::vector<Sweep> base;
+        sweeps_of(cu, n_seg, causal, band, prefix_host, backward != 0, base);
+        std::vector<int> len;
+        for (const Sweep& b : base) len.push_back(b.bn);
+        // fixed cost of a work item in swept elements, as for plain attention (lv_plan_fwd_split / lv_plan_bwd_split)
+        const int group = hq / hkv;
+        return backward ? lv_plan_sweeps(len.data(), (int)len.size(), hkv, n_cu, (128 + group - 1) / group, 256)
+                        : lv_plan_sweeps(len.data(), (int)len.size(), hq, n_cu, 512, 256);
+    } catch (const std::exception& e) {
+        return lv_fail(LV_ESIZE, "lv_plan_score_split: %s", e.what());
+    }
+}
+
+extern "C" int lvattn_fwd_score(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* desc_dev, int n_blocks,
+                                int q_rows_total, int k_rows_total, int hq, int hkv, int d, int64_t q_rs, int64_t q_hs, int64_t k_rs, int64_t k_hs,
+                                int64_t v_rs, int64_t v_hs, int64_t o_rs, int64_t o_hs, int64_t lse_stride, float softmax_scale, float softcap,
+                                const float* slopes, void* stream) {
+    if (int e = lv_check_qkv(q, k, v, hq, hkv, d, q_rs, q_hs, k_rs, k_hs, v_rs, v_hs)) return e;
+    if (int e = check_rule(d, hq, hkv, softmax_scale, softcap, slopes)) return e;
+    if (!out || !lse || !desc_dev) return lv_fail(LV_EINVAL, "null out/lse/desc pointer");
+    if (((uintptr_t)out & 7) || (o_rs & 3) || (o_hs & 3)) return lv_fail(LV_EINVAL, "out must be 8-byte aligned with strides %% 4 == 0");
+    if (n_blocks < 0 || q_rows_total <= 0 || k_rows_total <= 0) return lv_fail(LV_EINVAL, "bad sizes");
+    if (n_blocks == 0) return LV_OK;
+    if ((int64_t)n_blocks * hq > 0x7fffffffLL) return lv_fail(LV_EINVAL, "grid too large");
+    FwdParams p{};
+    p.q = (const __bf16*)q; p.k = (const __bf16*)k; p.v = (const __bf16*)v; p.o = (__bf16*)out; p.lse = lse;
+    p.desc = (const AttnDesc*)desc_dev;
+    p.n_blocks = n_blocks; p.hq = hq; p.hkv = hkv; p.group = hq / hkv;
+    p.q_rows_total = q_rows_total; p.k_rows_total = k_rows_total;
+    p.q_rs = q_rs; p.q_hs = q_hs; p.k_rs = k_rs; p.k_hs = k_hs; p.v_rs = v_rs; p.v_hs = v_hs;
+    p.o_rs = o_rs; p.o_hs = o_hs; p.lse_stride = lse_stride;
+    p.scale = softmax_scale; p.scale_log2e = softmax_scale * 1.4426950408889634f;
+    p.score = lv_score_rule(softmax_scale, softcap, slopes);
+    if (lv_launch_fwd_pp_score(p, d, lv_score_mod(softcap, slopes), (hipStream_t)stream))
+        return lv_fail(LV_ELAUNCH, "forward launch failed: %s", hipGetErrorString(hipGetLastError()));
+    return LV_OK;
+}
+
+extern "C" int lvattn_bwd_score(const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dq, void* dk,
+                                void* dv, const int32_t* qdesc_dev, int n_qblocks, const int32_t* kdesc_dev, int n_kblocks, int q_rows_total,
+                                int k_rows_total, int hq, int hkv, int d, int64_t q_rs, int64_t q_hs, int64_t k_rs, int64_t k_hs, int64_t v_rs,
+                                int64_t v_hs, int64_t do_rs, int64_t do_hs, int64_t dq_rs, int64_t dq_hs, int64_t dk_rs, int64_t dk_hs,
+                                int64_t dv_rs, int64_t dv_hs, int64_t lse_stride, float softmax_scale, float softcap, const float* slopes,
+                                int accum_f32, void* stream) {
+    if (int e = lv_check_qkv(q, k, v, hq, hkv, d, q_rs, q_hs, k_rs, k_hs, v_rs, v_hs)) return e;
+    if (int e = check_rule(d, hq, hkv, softmax_scale, softcap, slopes)) return e;
+    if (!dout || !lse || !delta || !dq || !dk || !dv) return lv_fail(LV_EINVAL, "null pointer");
+    if ((n_qblocks > 0 && !qdesc_dev) || (n_kblocks > 0 && !kdesc_dev)) return lv_fail(LV_EINVAL, "null descriptor pointer");
+    if (((uintptr_t)dout & 15) || ((do_rs | do_hs) & 7)) return lv_fail(LV_EINVAL, "dout must be 16-byte aligned, strides %% 8 == 0");
+    if (do_rs < 0 || do_rs * 2 * 256 > 0x7fffffffLL) return lv_fail(LV_EINVAL, "dout row stride %lld elements out of range", (long long)do_rs);
+    if ((((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15) || ((dq_rs | dq_hs | dk_rs | dk_hs | dv_rs | dv_hs) & 3))
+        return lv_fail(LV_EINVAL, "dq/dk/dv must be 16-byte aligned with strides %% 4 == 0");
+    if (n_qblocks < 0 || n_kblocks < 0 || q_rows_total <= 0 || k_rows_total <= 0 || lse_stride < q_rows_total) return lv_fail(LV_EINVAL, "bad sizes");
+    if (accum_f32 < 0 || accum_f32 > 2) return lv_fail(LV_EINVAL, "accum_f32 = %d (0 bf16 results, 1 fp32 added to, 2 fp32 stored)", accum_f32);
+    if ((int64_t)n_qblocks * hq > 0x7fffffffLL || (int64_t)n_kblocks * hkv > 0x7fffffffLL) return lv_fail(LV_EINVAL, "grid too large");
+    BwdParams p{};
+    p.q = (const __bf16*)q; p.k = (const __bf16*)k; p.v = (const __bf16*)v; p.dout = (const __bf16*)dout;
+    p.lse = lse; p.delta = delta; p.dq = dq; p.dk = dk; p.dv = dv;
+    p.desc = (const AttnDesc*)kdesc_dev; p.qdesc = (const AttnDesc*)qdesc_dev;
+    p.n_blocks = n_kblocks; p.n_qblocks = n_qblocks; p.hq = hq; p.hkv = hkv; p.group = hq / hkv;
+    p.q_rows_total = q_rows_total; p.k_rows_total = k_rows_total;
+    p.q_rs = q_rs; p.q_hs = q_hs; p.k_rs = k_rs; p.k_hs = k_hs; p.v_rs = v_rs; p.v_hs = v_hs;
+    p.do_rs = do_rs; p.do_hs = do_hs; p.dq_rs = dq_rs; p.dq_hs = dq_hs;
+    p.dk_rs = dk_rs; p.dk_hs = dk_hs; p.dv_rs = dv_rs; p.dv_hs = dv_hs;
+    p.lse_stride = lse_stride; p.scale = softmax_scale; p.scale_log2e = softmax_scale * 1.4426950408889634f;
+    p.f32_store = (accum_f32 == 2);
+    p.score = lv_score_rule(softmax_scale, softcap, slopes);
+    const int mod = lv_score_mod(softcap, slopes);
+    // the two launches write different tensors and read the same ones: any order
+    if (lv_launch_bwd_dkdv_rs_score(p, d, accum_f32 != 0, mod, (hipStream_t)stream) || lv_launch_bwd_dq_pp_score(p, d, accum_f32 != 0, mod, (hipStream_t)stream))
+        return lv_fail(LV_ELAUNCH, "backward launch failed: %s", hipGetErrorString(hipGetLastError()));
+    return LV_OK;
+}

@@ -155,6 +155,12 @@ int build(std::vector<Item>& base, int piece, bool causal, bool backward, int32_
 
 }  // namespace
 
+int lv_plan_sweeps(const int* sweep, int n, int copies, int n_cu, int fixed, int min_piece) {
+    std::vector<Item> base((size_t)n);
+    for (int i = 0; i < n; ++i) base[i].bn = sweep[i];
+    return plan(base, copies, n_cu, fixed, min_piece);
+}
+
 extern "C" int lv_plan_fwd_split(const int32_t* cu, int n_seg, int causal, int heads, int n_cu) {
     if (check_cu_list(cu, n_seg) || heads <= 0 || n_cu <= 0) return LV_EINVAL;
     std::vector<Item> base;

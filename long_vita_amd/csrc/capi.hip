@@ -22,6 +22,14 @@ static int fail(int code, const char* fmt, ...) {
     return code;
 }
 
+int lv_fail(int code, const char* fmt, ...) {   // fail() for the other translation units
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(g_err, sizeof(g_err), fmt, ap);
+    va_end(ap);
+    return code;
+}
+
 extern "C" int lvattn_abi_version(void) { return 1; }
 
 // Forward kernel choice.  Default: the one-wave-per-SIMD kernel ("a4") for head dim 128 when a work item sweeps at least
@@ -220,7 +228,7 @@ extern "C" int lv_build_bwd_blocks_rect(int q0, int ql, int k0, int kl, int caus
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
-static int check_common(const void* q, const void* k, const void* v, int hq, int hkv, int d,
+int lv_check_qkv(const void* q, const void* k, const void* v, int hq, int hkv, int d,
                         int64_t q_rs, int64_t q_hs, int64_t k_rs, int64_t k_hs, int64_t v_rs, int64_t v_hs) {
     if (!q || !k || !v) return fail(LV_EINVAL, "null q/k/v pointer");
     if (d != 64 && d != 128) return fail(LV_EINVAL, "head dim %d not supported (64 or 128)", d);
@@ -249,7 +257,7 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* out, floa
                     int64_t q_rs, int64_t q_hs, int64_t k_rs, int64_t k_hs, int64_t v_rs, int64_t v_hs,
                     int64_t o_rs, int64_t o_hs, int64_t lse_stride, float scale, int causal, void* stream, const RopeArgs* rope,
                     bool dense = false, int mean_keys = -1) {
-    if (int e = check_common(q, k, v, hq, hkv, d, q_rs, q_hs, k_rs, k_hs, v_rs, v_hs)) return e;
+    if (int e = lv_check_qkv(q, k, v, hq, hkv, d, q_rs, q_hs, k_rs, k_hs, v_rs, v_hs)) return e;
     if (!out || !lse || (!desc_dev && !dense)) return fail(LV_EINVAL, "null out/lse/desc pointer");
     if (((uintptr_t)out & 7) || (o_rs & 3) || (o_hs & 3)) return fail(LV_EINVAL, "out must be 8-byte aligned with strides % 4 == 0");
     if (n_blocks < 0 || q_rows_total <= 0 || k_rows_total <= 0) return fail(LV_EINVAL, "bad sizes");
@@ -403,7 +411,7 @@ static int decode_impl(const char* who, const void* q, const void* k, const void
     // q is [batch, hq, d]: its batch stride is no tile row stride (the kernel forms q's offsets in 64 bits), so it only
     // has to be a multiple of 8 elements; the 256-row tile cap of the prefill kernels applies to the K / V row strides
     if (q_bs < 0 || (q_bs & 7)) return fail(LV_EINVAL, "%s: q batch stride %lld must be a non-negative multiple of 8 elements", who, (long long)q_bs);
-    if (int e = check_common(q, k, v, hq, hkv, d, 0, q_hs, k_rs, k_hs, v_rs, v_hs)) return e;
+    if (int e = lv_check_qkv(q, k, v, hq, hkv, d, 0, q_hs, k_rs, k_hs, v_rs, v_hs)) return e;
     if (!out || (!workspace && !library_scratch)) return fail(LV_EINVAL, "%s: null out/workspace pointer", who);
     if (batch <= 0 || k_len <= 0) return fail(LV_EINVAL, "%s: batch=%d k_len=%d", who, batch, k_len);
     if (hq / hkv > 32) return fail(LV_EINVAL, "%s: %d query heads per KV head (at most 32)", who, hq / hkv);
@@ -487,7 +495,7 @@ extern "C" int lvattn_bwd(const void* q, const void* k, const void* v, const voi
                           int64_t do_rs, int64_t do_hs, int64_t dq_rs, int64_t dq_hs,
                           int64_t dk_rs, int64_t dk_hs, int64_t dv_rs, int64_t dv_hs,
                           int64_t lse_stride, float scale, int causal, int accum_f32, void* stream) {
-    if (int e = check_common(q, k, v, hq, hkv, d, q_rs, q_hs, k_rs, k_hs, v_rs, v_hs)) return e;
+    if (int e = lv_check_qkv(q, k, v, hq, hkv, d, q_rs, q_hs, k_rs, k_hs, v_rs, v_hs)) return e;
     if (!dout || !lse || !delta || !dq || !dk || !dv) return fail(LV_EINVAL, "null pointer");
     if ((n_qblocks > 0 && !qdesc_dev) || (n_kblocks > 0 && !kdesc_dev)) return fail(LV_EINVAL, "null descriptor pointer");
     if (((uintptr_t)dout & 15) || ((do_rs | do_hs) & 7)) return fail(LV_EINVAL, "dout must be 16-byte aligned, strides % 8 == 0");

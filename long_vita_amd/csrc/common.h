@@ -86,7 +86,8 @@ struct AttnDesc {
     int band_p1;    // 0: plain causal rule.  b + 1: a band as well, key j visible to row i iff i + shift - b <= j <= i + shift
                     // (taken by the ping-pong forward, the ping-pong dQ and the role-split dK/dV kernels, which a launch
                     // with causal == 2 selects)
-    int pad2;
+    int prefix;     // MOD kernels: swept keys [0, prefix) (relative to the descriptor's first key) are visible to every row, beyond the
+                    // causal rule; <= 0: none.  0 in every other table
 };
 // lower end of a row's visible keys, as an offset to add to the row index: `i + lv_band_low(dsc)` is the first visible key
 // (far below zero without a band)

@@ -2,6 +2,37 @@
 #pragma once
 #include "common.h"
 
+// Rules that change a score before the softmax.  A kernel instantiated with MOD != 0 works on t = log2(e) * score, where
+//   score = cap * tanh(scale * q.k / cap)   (LV_SCORE_CAP; else scale * q.k)
+//           - slope[head] * |query position - key position|   (LV_SCORE_BIAS)
+// and always honours the descriptor's prefix (word 7).  tanh(y) = 1 - 2 / (2^(2 y log2 e) + 1): one exponential and one
+// reciprocal, exact limits on both sides (2^x = inf gives 1, 0 gives -1), absolute error of a few 2^-24.
+#define LV_SCORE_CAP 1
+#define LV_SCORE_BIAS 2
+#define LV_SCORE_RULE 4        // set in every MOD: prefix rows, no other rule needed
+struct ScoreRule {
+    float cap_in;              // 2 log2(e) scale / cap: the exponent of the tanh from the raw product q.k
+    float cap_out;             // cap log2(e)
+    const float* slopes;       // [hq], device
+};
+#ifdef __HIPCC__
+// raw product s -> t; `dist` = signed distance of the two positions; `grad` = d score / d (scale q.k) = 1 - tanh^2
+template <int MOD>
+__device__ __forceinline__ float lv_score(float s, float c, const ScoreRule& u, float nslope2, float dist, float* grad = nullptr) {
+    float t;
+    if constexpr (MOD & LV_SCORE_CAP) {
+        const float rc = __builtin_amdgcn_rcpf(fast_exp2(s * u.cap_in) + 1.f);
+        t = __builtin_fmaf(-2.f * u.cap_out, rc, u.cap_out);
+        if (grad) { const float f = 4.f * rc; *grad = __builtin_fmaf(-f, rc, f); }   // 1 - (1 - 2 rc)^2
+    } else {
+        t = s * c;
+        if (grad) *grad = 1.f;
+    }
+    if constexpr (MOD & LV_SCORE_BIAS) t = __builtin_fmaf(nslope2, __builtin_fabsf(dist), t);
+    return t;
+}
+#endif
+
 struct FwdParams {
     const __bf16* q;
     const __bf16* k;
@@ -23,6 +54,7 @@ struct FwdParams {
     int rope_tab_div;
     __bf16* q_rot;
     int64_t qr_rs, qr_hs;
+    ScoreRule score;    // read by the MOD != 0 kernels only
 };
 // Workgroup i of a launch runs on XCD i % 8, and every XCD has its own L2.  When ALL the work items of one KV head
 // (query blocks x the group's query heads) fit on an XCD's 32 CUs at once, they are given consecutive slots of one XCD:
@@ -50,6 +82,7 @@ __device__ __forceinline__ AttnDesc lv_fwd_desc(const FwdParams& p, int blk, int
 #endif
 int lv_launch_fwd(const FwdParams& p, int d, int causal, int waves, hipStream_t stream);
 int lv_launch_fwd_pp(const FwdParams& p, int d, int causal, hipStream_t stream);  // ping-pong form, 256-row items
+int lv_launch_fwd_pp_score(const FwdParams& p, int d, int mod, hipStream_t stream);  // the same with p.score applied
 int lv_launch_fwd_pp16(const FwdParams& p, int causal, hipStream_t stream);      // ping-pong form on 16x16x32 MFMAs, d = 128
 int lv_launch_fwd_a4(const FwdParams& p, int causal, hipStream_t stream);        // one wave per SIMD, 64 query rows per wave, d = 128
 
@@ -91,11 +124,22 @@ struct BwdParams {
     int64_t q_rs, q_hs, k_rs, k_hs, v_rs, v_hs, do_rs, do_hs, dq_rs, dq_hs, dk_rs, dk_hs, dv_rs, dv_hs, lse_stride;
     float scale, scale_log2e;
     int f32_store;   // fp32 results are stored, not added to what the buffers hold (accum_f32 == 2)
+    ScoreRule score; // read by the MOD != 0 kernels only
 };
 int lv_launch_bwd(const BwdParams& p, int d, int causal, int accum, hipStream_t stream);
 int lv_launch_bwd_dkdv_rs(const BwdParams& p, int d, int causal, int accum, hipStream_t stream);  // role-split dK/dV kernel
 int lv_launch_bwd_dkdv_g(const BwdParams& p, int causal, int accum, hipStream_t stream);          // one wave per SIMD, gap-scheduled dK/dV kernel, d = 128
 int lv_launch_bwd_dq_pp(const BwdParams& p, int d, int causal, int accum, hipStream_t stream);  // ping-pong dQ kernel
+int lv_launch_bwd_dq_pp_score(const BwdParams& p, int d, int accum, int mod, hipStream_t stream);    // with p.score applied
+int lv_launch_bwd_dkdv_rs_score(const BwdParams& p, int d, int accum, int mod, hipStream_t stream);
+ScoreRule lv_score_rule(float scale, float softcap, const float* slopes);
+int lv_score_mod(float softcap, const float* slopes);      // LV_SCORE_* bits of a rule
+// error text of the calling thread (lvattn_last_error); returns `code`
+int lv_fail(int code, const char* fmt, ...);
+int lv_check_qkv(const void* q, const void* k, const void* v, int hq, int hkv, int d, int64_t q_rs, int64_t q_hs, int64_t k_rs,
+                 int64_t k_hs, int64_t v_rs, int64_t v_hs);
+// piece length that a simulated schedule of `copies` copies of these sweeps likes best on n_cu compute units; 0 = leave them whole
+int lv_plan_sweeps(const int* sweep, int n, int copies, int n_cu, int fixed, int min_piece);
 void lv_select_bwd_kernels(int dq, int dkdv);   // 0 default, 1 the earlier kernel, (dkdv) 2 the gap-scheduled kernel, < 0 unchanged
 void lv_select_rs_units(int n);                  // 32-row units per iteration of the role-split dK/dV kernel: 1 or 2
 int lv_launch_bwd_delta(const void* o, const void* dout, float* delta, int rows, int hq, int d, int64_t o_rs, int64_t o_hs,

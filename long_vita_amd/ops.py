@@ -588,6 +588,196 @@ def varlen_attention(q, k, v, cu_seqlens: Sequence[int], scale: float | None = N
 
 
 # ---------------------------------------------------------------------------
+# autograd: packed attention whose scores follow a rule (tanh cap, distance bias, prefix)
+# ---------------------------------------------------------------------------
+class _ScoreRule:
+    """What a launch needs to know besides q, k, v: the segments, who sees whom, and how a score is changed.  ``slopes`` (fp32
+    [hq] on the device, or None) stays out of the table keys: tables do not depend on it."""
+
+    def __init__(self, cu, causal, band, prefix, softcap):
+        self.cu, self.causal, self.band, self.prefix, self.softcap = cu, causal, band, prefix, softcap
+        self.key = (cu, causal, band, prefix)
+
+    def _host(self):
+        cu = np.ascontiguousarray(np.asarray(self.cu, dtype=np.int32))
+        pre = None if self.prefix is None else np.ascontiguousarray(np.asarray(self.prefix, dtype=np.int32))
+        return cu, pre, (None if pre is None else pre.ctypes.data_as(_I32P)), -1 if self.band is None else self.band
+
+    def pieces(self, hq, hkv, device):
+        """(keys per forward / dQ piece, query rows per dK/dV piece); 0 = sweeps stay whole (lv_plan_score_split)."""
+        def build():
+            cu, _pre, pre_p, band = self._host()
+            fn = _lib.lib().lv_plan_score_split
+            return tuple(check(fn(cu.ctypes.data_as(_I32P), len(cu) - 1, int(self.causal), band, pre_p, bwd, hq, hkv, _n_cu(device)),
+                               "lv_plan_score_split") for bwd in (0, 1))
+        if _split_override["fwd"] is not None and _split_override["bwd"] is not None:
+            return int(_split_override["fwd"]), int(_split_override["bwd"])
+        planned = _blocks.get(("score_plan", self.key, hq, hkv, str(device)), build)
+        return tuple(int(p if o is None else o) for p, o in zip(planned, (_split_override["fwd"], _split_override["bwd"])))
+
+    def tables(self, backward, piece, device) -> SplitTables:
+        """Work items on the device; ``comb`` is None and ``ws_rows`` 0 when the sweeps stay whole (``piece`` 0)."""
+        def build():
+            cu, _pre, pre_p, band = self._host()
+            n_comb, ws_rows = C.c_int(0), C.c_int(0)
+
+            def call(desc, n_desc, comb, n_c):
+                return check(_lib.lib().lv_build_score_blocks(cu.ctypes.data_as(_I32P), len(cu) - 1, int(self.causal), band, pre_p, int(backward),
+                                                              int(piece), desc, n_desc, comb, n_c, C.byref(n_comb), C.byref(ws_rows)),
+                             "lv_build_score_blocks")
+            n = call(None, 0, None, 0)
+            desc = np.zeros((max(n, 1), LV_DESC_INTS), dtype=np.int32)
+            comb = np.zeros((max(n_comb.value, 1), 4), dtype=np.int32)
+            call(desc.ctypes.data_as(_I32P), desc.shape[0], comb.ctypes.data_as(_I32P), comb.shape[0])
+            return SplitTables(_to_device(desc[:n], device), torch.from_numpy(comb[:n_comb.value]).to(device) if piece else None,
+                               int(ws_rows.value) if piece else 0, LV_BWD_BLOCK_N if backward else 256, int(piece))
+        return _blocks.get(("score", self.key, bool(backward), int(piece), str(device)), build)
+
+
+def _score_fwd_launch(q, k, v, tables, rule, slopes, scale, out, lse):
+    rq, hq, d = q.shape
+    check(_lib.lib().lvattn_fwd_score(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(tables.desc), tables.desc.shape[0], rq, k.shape[0], hq, k.shape[1], d,
+        q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1), lse.stride(0),
+        float(scale), float(rule.softcap), _ptr(slopes), _stream()), "lvattn_fwd_score")
+
+
+def _score_bwd_launch(q, k, v, dout, lse, delta, tq, tk, rule, slopes, scale, dq, dk, dv, accum_f32):
+    rq, hq, d = q.shape
+    check(_lib.lib().lvattn_bwd_score(
+        _ptr(q), _ptr(k), _ptr(v), _ptr(dout), _ptr(lse), _ptr(delta), _ptr(dq), _ptr(dk), _ptr(dv),
+        _ptr(tq.desc), tq.desc.shape[0], _ptr(tk.desc), tk.desc.shape[0], rq, k.shape[0], hq, k.shape[1], d,
+        q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), dout.stride(0), dout.stride(1),
+        dq.stride(0), dq.stride(1), dk.stride(0), dk.stride(1), dv.stride(0), dv.stride(1), lse.stride(0),
+        float(scale), float(rule.softcap), _ptr(slopes), int(accum_f32), _stream()), "lvattn_bwd_score")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """The tensor itself when the kernels can address it (last dimension contiguous, 16-byte aligned rows, strides that fit a
+    tile's 32-bit offsets), a contiguous copy otherwise."""
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s >= 0 and s % 8 == 0 for s in t.stride()[:-1]) and t.stride(-3) < (1 << 22)
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+class _ScoreAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, slopes, rule, scale):
+        q, k, v = _rows(q), _rows(k), _rows(v)
+        total, hq, d = q.shape
+        dev = q.device
+        covered = rule.cu[0] == 0 and rule.cu[-1] == total
+        pieces = rule.pieces(hq, k.shape[1], dev)
+        out = (torch.empty if covered else torch.zeros)((total, hq, d), dtype=torch.bfloat16, device=dev)
+        lse = torch.empty((hq, total), dtype=torch.float32, device=dev)
+        if not covered:
+            lse.fill_(float("-inf"))
+        if rule.cu[-1] > rule.cu[0]:
+            t = rule.tables(False, pieces[0], dev)
+            if pieces[0]:
+                ws_out = torch.empty((t.ws_rows, hq, d), dtype=torch.bfloat16, device=dev)
+                ws_lse = torch.empty((hq, t.ws_rows), dtype=torch.float32, device=dev)
+                _score_fwd_launch(q, k, v, t, rule, slopes, scale, ws_out, ws_lse)
+                combine_lse_launch(ws_out, ws_lse, out, lse, t)
+            else:
+                _score_fwd_launch(q, k, v, t, rule, slopes, scale, out, lse)
+        ctx.save_for_backward(q, k, v, out, lse, slopes)
+        ctx.rule, ctx.scale, ctx.pieces, ctx.covered = rule, scale, pieces, covered
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _dlse):
+        q, k, v, out, lse, slopes = ctx.saved_tensors
+        _require_gpu(q, dout)
+        rule = ctx.rule
+        rq, hq, d = q.shape
+        hkv = k.shape[1]
+        dev = q.device
+        if rule.cu[-1] == rule.cu[0]:
+            return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None, None, None
+        dout = _rows(dout)
+        delta = torch.empty((hq, rq), dtype=torch.float32, device=dev)
+        check(_lib.lib().lvattn_bwd_delta(_ptr(out), _ptr(dout), _ptr(delta), rq, hq, d, out.stride(0), out.stride(1),
+                                          dout.stride(0), dout.stride(1), delta.stride(0), _stream()), "lvattn_bwd_delta")
+        make = torch.empty if ctx.covered else torch.zeros       # rows no segment covers get a zero gradient
+        dq = make((rq, hq, d), dtype=torch.bfloat16, device=dev)
+        dk, dv = (make((rq, hkv, d), dtype=torch.bfloat16, device=dev) for _ in range(2))
+        pf, pb = ctx.pieces
+        if pf or pb:      # one launch takes one kind of output buffer: when either sweep is cut, both go through workspaces
+            tq = rule.tables(False, pf or _ONE_PIECE, dev)
+            tk = rule.tables(True, pb or _ONE_PIECE, dev)
+            dq_ws = _workspace((tq.ws_rows, hq, d), dev)
+            dk_ws, dv_ws = (_workspace((tk.ws_rows, hkv, d), dev) for _ in range(2))
+            _score_bwd_launch(q, k, v, dout, lse, delta, tq, tk, rule, slopes, ctx.scale, dq_ws, dk_ws, dv_ws, 2)
+            combine_sum_launch(dq_ws, dq, tq)
+            combine_sum_launch(dk_ws, dk, tk)
+            combine_sum_launch(dv_ws, dv, tk)
+        else:
+            _score_bwd_launch(q, k, v, dout, lse, delta, rule.tables(False, 0, dev), rule.tables(True, 0, dev), rule, slopes, ctx.scale,
+                              dq, dk, dv, 0)
+        return dq, dk, dv, None, None, None
+
+
+def _check_rule_args(hq, hkv, softcap, slopes, device, who):
+    """softcap as a float (0 = none) and the slopes as contiguous fp32 on the device."""
+    cap = 0.0 if softcap is None else float(softcap)
+    if softcap is not None and not (0.0 < cap < 1e30):
+        raise LvAttnError(f"{who}: softcap must be a finite number above 0 (None for no cap), not {softcap!r}")
+    if slopes is not None:
+        if not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32 or slopes.shape != (hq,):
+            raise LvAttnError(f"{who}: alibi_slopes must be an fp32 tensor [{hq}] (one slope per query head)")
+        if slopes.requires_grad:
+            raise LvAttnError(f"{who}: alibi_slopes get no gradient; pass a tensor that does not require one")
+        if slopes.device != device:
+            raise LvAttnError(f"{who}: alibi_slopes live on {slopes.device}, the queries on {device}")
+        if hkv and hq // hkv > 64:
+            raise LvAttnError(f"{who}: at most 64 query heads per KV head with alibi_slopes")
+        slopes = slopes.contiguous()
+    return cap, slopes
+
+
+def score_attention(q, k, v, cu_seqlens: Sequence[int], scale: float | None = None, causal: bool = True, softcap: float | None = None,
+                    alibi_slopes: torch.Tensor | None = None, prefix_lens: Sequence[int] | None = None, band: int | None = None):
+    """``varlen_attention`` with a rule on the scores: q [T,Hq,D], k/v [T,Hkv,D] bf16 -> (out [T,Hq,D] bf16, lse [Hq,T] fp32);
+    differentiable in q, k, v.  Head dim 64 or 128.
+
+    t_ij = softcap * tanh(scale q_i.k_j / softcap) - alibi_slopes[h] * |i - j|, softmax over the keys of i's segment with
+    j <= i (all of them when ``causal`` is false).  ``prefix_lens`` (one per segment, causal only): the segment's first keys are
+    visible to all of its rows, as the tokens of an image that opens a sample are; a length past the segment means the whole
+    segment.  ``band`` (causal only, not with prefix_lens): a query sees itself and the ``band`` keys before it.
+    Rows outside every segment come back as zeros with lse -inf.  ``alibi_slopes`` (fp32 [Hq] on q's device) are constants."""
+    for t in (q, k, v):
+        if not isinstance(t, torch.Tensor):
+            raise LvAttnError("score_attention: q, k, v must be tensors")
+    _check_qkv(q, k, v)
+    if q.shape[0] != k.shape[0]:
+        raise LvAttnError(f"score_attention: {q.shape[0]} query rows and {k.shape[0]} key rows (packed self attention has as many of both)")
+    hq, hkv, d = q.shape[1], k.shape[1], q.shape[2]
+    if d not in (64, 128) or hq == 0 or hkv == 0 or hq % hkv:
+        raise LvAttnError(f"score_attention: {hq} / {hkv} heads of {d} (head dim 64 or 128, query heads a multiple of the KV heads)")
+    cu = tuple(int(x) for x in cu_seqlens)
+    if len(cu) < 1 or cu[0] < 0 or any(b < a for a, b in zip(cu[:-1], cu[1:])) or cu[-1] > q.shape[0]:
+        raise LvAttnError(f"score_attention: cu_seqlens must not decrease and must end within the {q.shape[0]} rows")
+    causal = bool(causal)
+    prefix = None if prefix_lens is None else tuple(int(x) for x in prefix_lens)
+    if prefix is not None:
+        if not causal or len(prefix) != len(cu) - 1 or min(prefix, default=0) < 0:
+            raise LvAttnError("score_attention: prefix_lens needs causal attention and one non-negative length per segment")
+        prefix = tuple(min(p, b - a) for p, a, b in zip(prefix, cu[:-1], cu[1:]))
+    if band is not None:
+        if not causal or prefix is not None or int(band) < 0:
+            raise LvAttnError("score_attention: a band needs causal attention, no prefix_lens and a length of 0 or more")
+        longest = max((b - a for a, b in zip(cu[:-1], cu[1:])), default=0)
+        band = int(band) if int(band) < longest - 1 else None       # a band no segment is longer than changes nothing
+    cap, slopes = _check_rule_args(hq, hkv, softcap, alibi_slopes, q.device, "score_attention")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise LvAttnError(f"score_attention: scale {scale} is not finite")
+    return _ScoreAttention.apply(q, k, v, slopes, _ScoreRule(cu, causal, band, prefix, cap), scale)
+
+
+# ---------------------------------------------------------------------------
 # data movement
 # ---------------------------------------------------------------------------
 class _PixelShuffleTokens(torch.autograd.Function):
