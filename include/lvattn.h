@@ -259,6 +259,32 @@ int lvattn_decode_noalloc(const void* q, const void* k, const void* v, void* out
                           int64_t o_batch_stride, int64_t o_head_stride,
                           float softmax_scale, int n_split, void* stream);
 
+/* ---- drafted tokens over a KV cache ---------------------------------------------
+ * No counterpart in the reference, whose kv-cache op (lcvlm_modellink/core/transformer/dot_product_attention.py:428-438) takes one
+ * new token per sequence, all caches equally long, plain scores.  q / out [batch, n, hq, d], k / v [batch, rows, hkv, d] bf16
+ * with element strides (last dimension contiguous), lse [batch, n, hq] fp32 contiguous or NULL.  cache_lens [batch] int32 and
+ * parents int32 live in device memory.  Sequence b holds cache_lens[b] keys that all its tokens see (a value outside
+ * [0, rows - n] is moved to the nearest end), the n drafted tokens' keys are the rows behind them.  parents[b][i] (batch stride
+ * 0: one tree for all) is the number of token i's parent: below i, -1 for a token that continues the cache, -2 for a slot
+ * that holds no token (its output is 0, its lse -inf, its K / V rows are not looked at); a parent at or past i counts as -1.
+ * parents == NULL: a chain (token i sees drafted tokens 0 .. i); n == 1 is the ordinary decode step.  The score rule is
+ * lvattn_fwd_score's, with token i at position cache_lens[b] + its depth and cached key j at position j.
+ * n <= 256, batch <= 512.  workspace: lvattn_tree_workspace_bytes(...) bytes, contents undefined afterwards, not shared by calls
+ * that may overlap.  Results do not depend on what lies behind row cache_lens[b] + n. */
+int64_t lvattn_tree_workspace_bytes(int batch, int n, int rows, int hq, int hkv, int d);
+int lvattn_tree(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* cache_lens, const int32_t* parents,
+                int64_t parents_batch_stride, void* workspace, int64_t workspace_bytes, int batch, int n, int rows, int hq, int hkv, int d,
+                int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride, int64_t k_batch_stride, int64_t k_row_stride,
+                int64_t k_head_stride, int64_t v_batch_stride, int64_t v_row_stride, int64_t v_head_stride, int64_t o_batch_stride,
+                int64_t o_token_stride, int64_t o_head_stride, float softmax_scale, float softcap, const float* slopes, void* stream);
+/* The accepted path of a tree becomes the cache's next rows, in place: row cache_lens[b] + path[b][i] -> row cache_lens[b] + i
+ * for i < n_accept[b] (path [batch, n] int32, ascending token numbers, as a path from the root down is), K and V and, when
+ * given, the accumulated weights [batch, hkv, rows] fp32 (batch / head strides).  Rows from cache_lens[b] + n_accept[b] on keep
+ * what they hold or held before their row moved. */
+int lv_tree_accept(void* k, void* v, float* weight, const int32_t* cache_lens, const int32_t* path, const int32_t* n_accept, int batch, int n,
+                   int rows, int hkv, int d, int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t v_batch_stride,
+                   int64_t v_row_stride, int64_t v_head_stride, int64_t w_batch_stride, int64_t w_head_stride, void* stream);
+
 /* ---- attention backward -----------------------------------------------------
  * Replaces the autograd of the calls above (npu_fusion_attention_grad, reached
  * through torch autograd from dot_product_attention.py:352-365 / :314-325) and the

@@ -272,6 +272,135 @@ def decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     return (out, lse) if return_lse else out
 
 
+TREE_MAX_TOKENS = 256       # drafted tokens per sequence of tree_attention
+TREE_MAX_BATCH = 512
+TREE_UNUSED = -2            # parents[] entry of a slot that holds no token
+
+
+def _cache_rows(t: torch.Tensor, name: str, who: str) -> torch.Tensor:
+    """A K or V cache [b, rows, hkv, d] as the cache kernels address it.  A cache is never copied behind the caller's back: one
+    the kernels cannot address is refused."""
+    if t.stride(3) != 1 or t.data_ptr() % 16 or any(s < 0 or s % 8 for s in t.stride()[:3]) or t.stride(1) >= 1 << 22:
+        raise LvAttnError(f"{who}: {name} needs a contiguous last dimension, 16-byte alignment, strides that are multiples of 8 elements and "
+                          f"a row stride below 4194304 (strides {tuple(t.stride())})")
+    return t
+
+
+def _check_cache(q, k, v, cache_lens, who):
+    """Shapes and types shared by the operators on a ragged KV cache; returns (b, n, rows, hq, hkv, d)."""
+    _require_gpu(q, k, v, cache_lens)
+    for t in (q, k) if v is None else (q, k, v):
+        if t.dtype != torch.bfloat16 or t.dim() != 4:
+            raise LvAttnError(f"{who}: expects bfloat16 q [b, n, hq, d] and caches [b, rows, hkv, d]")
+    b, n, hq, d = q.shape
+    rows, hkv = k.shape[1], k.shape[2]
+    if k.shape != (b, rows, hkv, d) or (v is not None and v.shape != k.shape):
+        raise LvAttnError(f"{who}: shape mismatch q{tuple(q.shape)} k{tuple(k.shape)}" + ("" if v is None else f" v{tuple(v.shape)}"))
+    if d not in (64, 128) or hq == 0 or hkv == 0 or hq % hkv:
+        raise LvAttnError(f"{who}: {hq} / {hkv} heads of {d} (head dim 64 or 128, query heads a multiple of the KV heads)")
+    if b == 0 or n == 0 or rows < n:
+        raise LvAttnError(f"{who}: {b} sequences, {n} tokens, caches of {rows} rows (at least one token, caches that hold the tokens)")
+    if cache_lens.dtype != torch.int32 or cache_lens.shape != (b,):
+        raise LvAttnError(f"{who}: cache_lens must be int32 [{b}]")
+    return b, n, rows, hq, hkv, d
+
+
+def _tree_parents(parents, b, n, device, who):
+    """(int32 tensor, batch stride) of a [n] or [b, n] tree table; (None, 0) for a chain."""
+    if parents is None:
+        return None, 0
+    if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int32 or tuple(parents.shape) not in ((n,), (b, n)):
+        raise LvAttnError(f"{who}: parents must be int32 [{n}] or [{b}, {n}]")
+    if parents.device != device:
+        raise LvAttnError(f"{who}: parents live on {parents.device}, the queries on {device}")
+    if parents.stride(-1) != 1 or parents.stride(0) < 0:
+        parents = parents.contiguous()
+    return parents, parents.stride(0) if parents.dim() == 2 else 0
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_lens: torch.Tensor, scale: float | None = None,
+                   parents: torch.Tensor | None = None, softcap: float | None = None, alibi_slopes: torch.Tensor | None = None,
+                   return_lse: bool = False, out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                   workspace: torch.Tensor | None = None):
+    """Drafted tokens of every sequence against its KV cache: q [b, n, hq, d], k / v [b, rows, hkv, d] bf16 -> out [b, n, hq, d]
+    (and lse [b, n, hq] fp32).  Sequence s sees its first ``cache_lens[s]`` rows (int32 [b] on the device, clamped to
+    [0, rows - n]); the drafted tokens' K / V are the n rows behind them.
+
+    ``parents`` (int32 [n] or [b, n] on the device): token i's parent in the draft tree, -1 where it continues the cache,
+    ``TREE_UNUSED`` (-2) for a slot that holds no token (output 0, lse -inf); a token sees itself and its ancestors.  Parents come
+    before their children (an entry that does not counts as -1).  None: a chain, and with n = 1 the ordinary decode step over
+    caches of different lengths.  ``softcap`` / ``alibi_slopes`` as in ``score_attention``, token i standing at position
+    ``cache_lens[s]`` + its depth and cached row j at position j (of an evicted cache that is no longer so).
+
+    At most 256 tokens per sequence and 512 sequences.  ``workspace`` (uint8, at least ``tree_workspace_bytes(...)``) lets a
+    program keep its own; calls that may overlap need one each.  No gradient."""
+    who = "tree_attention"
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
+        raise LvAttnError(f"{who} has no gradient: call it under torch.no_grad() or on tensors that do not require one")
+    b, n, rows, hq, hkv, d = _check_cache(q, k, v, cache_lens, who)
+    if n > TREE_MAX_TOKENS or b > TREE_MAX_BATCH:
+        raise LvAttnError(f"{who}: {b} sequences of {n} tokens (at most {TREE_MAX_BATCH} of {TREE_MAX_TOKENS})")
+    k, v = _cache_rows(k, "k", who), _cache_rows(v, "v", who)
+    if q.stride(3) != 1 or q.data_ptr() % 16 or any(s < 0 or s % 8 for s in q.stride()[:3]):
+        q = q.clone(memory_format=torch.contiguous_format)
+    cache_lens = cache_lens.contiguous()
+    parents, p_bs = _tree_parents(parents, b, n, q.device, who)
+    cap, slopes = _check_rule_args(hq, 0, softcap, alibi_slopes, q.device, who)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise LvAttnError(f"{who}: scale {scale} is not finite")
+    if out is None:
+        out = torch.empty((b, n, hq, d), dtype=torch.bfloat16, device=q.device)
+    elif out.shape != (b, n, hq, d) or out.dtype != torch.bfloat16 or out.device != q.device or out.stride(3) != 1:
+        raise LvAttnError(f"{who}: out must be bf16 [b, n, hq, d] on q's device with a contiguous last dimension")
+    if lse is None:
+        lse = torch.empty((b, n, hq), dtype=torch.float32, device=q.device) if return_lse else None
+    elif lse.shape != (b, n, hq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
+        raise LvAttnError(f"{who}: lse must be contiguous fp32 [b, n, hq] on q's device")
+    need = tree_workspace_bytes(b, n, rows, hq, hkv, d)
+    if workspace is None:
+        workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+    elif workspace.dtype != torch.uint8 or workspace.device != q.device or not workspace.is_contiguous() or workspace.numel() < need:
+        raise LvAttnError(f"{who}: workspace must be contiguous uint8 of at least {need} bytes on q's device")
+    check(_lib.lib().lvattn_tree(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(cache_lens), _ptr(parents), p_bs, _ptr(workspace),
+                                 workspace.numel(), b, n, rows, hq, hkv, d, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                                 *out.stride()[:3], scale, cap, _ptr(slopes), _stream()), "lvattn_tree")
+    return (out, lse) if return_lse else out
+
+
+def tree_workspace_bytes(b: int, n: int, rows: int, hq: int, hkv: int, d: int) -> int:
+    """Bytes of workspace ``tree_attention`` needs for these sizes."""
+    return int(_lib.lib().lvattn_tree_workspace_bytes(b, n, rows, hq, hkv, d))
+
+
+def tree_accept(k: torch.Tensor, v: torch.Tensor, cache_lens: torch.Tensor, path: torch.Tensor, n_accept: torch.Tensor,
+                weight: torch.Tensor | None = None) -> torch.Tensor:
+    """The accepted path of a draft tree becomes the caches' next rows, in place: row ``cache_lens[s] + path[s, i]`` moves to row
+    ``cache_lens[s] + i`` for i < ``n_accept[s]``, in k, v [b, rows, hkv, d] and ``weight`` [b, hkv, rows] when given.  ``path``
+    int32 [b, n] holds ascending token numbers (a parent stands before its child); entries past n_accept are not looked at.
+    Returns the new lengths, cache_lens + n_accept."""
+    who = "tree_accept"
+    _require_gpu(k, v, cache_lens, path, n_accept, weight)
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.dim() != 4 or k.shape != v.shape or k.shape[3] not in (64, 128):
+        raise LvAttnError(f"{who}: expects bfloat16 caches [b, rows, hkv, 64 or 128]")
+    b, rows, hkv, d = k.shape
+    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != b or not 1 <= path.shape[1] <= rows or not path.is_contiguous():
+        raise LvAttnError(f"{who}: path must be contiguous int32 [{b}, 1 to {rows}]")
+    for name, t in (("cache_lens", cache_lens), ("n_accept", n_accept)):
+        if t.dtype != torch.int32 or t.shape != (b,) or not t.is_contiguous():
+            raise LvAttnError(f"{who}: {name} must be contiguous int32 [{b}]")
+    if weight is not None and (weight.dtype != torch.float32 or weight.shape != (b, hkv, rows) or weight.stride(2) != 1):
+        raise LvAttnError(f"{who}: weight must be fp32 [{b}, {hkv}, {rows}] with contiguous rows")
+    _cache_rows(k, "k", who), _cache_rows(v, "v", who)
+    if any(s == 0 and m > 1 for t in (k, v) for s, m in zip(t.stride(), t.shape)):
+        raise LvAttnError(f"{who}: an expanded cache cannot be written in place")
+    if b and hkv:
+        w_s = (0, 0) if weight is None else weight.stride()[:2]
+        check(_lib.lib().lv_tree_accept(_ptr(k), _ptr(v), _ptr(weight), _ptr(cache_lens), _ptr(path), _ptr(n_accept), b, path.shape[1], rows, hkv, d,
+                                        *k.stride()[:3], *v.stride()[:3], *w_s, _stream()), "lv_tree_accept")
+    return cache_lens + n_accept
+
+
 def attn_bwd_launch(q, k, v, out, dout, lse, desc_q: torch.Tensor, desc_k: torch.Tensor, scale: float, causal: bool,
                     dq=None, dk=None, dv=None, delta=None, accum_f32: bool | int = False):
     """Backward of ``attn_fwd_launch``.  ``desc_q`` are the forward's query-block descriptors
