@@ -285,6 +285,37 @@ int lv_tree_accept(void* k, void* v, float* weight, const int32_t* cache_lens, c
                    int rows, int hkv, int d, int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t v_batch_stride,
                    int64_t v_row_stride, int64_t v_head_stride, int64_t w_batch_stride, int64_t w_head_stride, void* stream);
 
+/* ---- eviction by accumulated attention weight -----------------------------------
+ * No counterpart in the reference, whose cache only grows.
+ * lv_key_weights: w_out[b, kvh, j] = w_in[b, kvh, j] + sum over tokens i and the query heads h of kvh's group of
+ *   row_weight[b, i] * exp(t_ij - lse[b, i, h]): what the attention of lvattn_tree (same tokens, keys, tree and score rule; lse is
+ *   its output) gave to key j.  n tokens per sequence: one decode step, a tree (n <= 256 with parents), or a whole prompt
+ *   (parents == NULL, cache_lens 0).  row_weight [batch, n] fp32 or NULL (1); a token whose weight is not above 0 counts for nothing,
+ *   whatever its row holds.  w_in / w_out [batch, hkv, rows] fp32 with batch / head strides, w_out may be w_in; weights of rows
+ *   that are no keys are carried over.  Sums are compensated fp32 in a fixed order.  workspace may be NULL when
+ *   lv_key_weights_workspace_bytes is 0.
+ * lv_evict_index: index[b][kvh][0 .. min(len, keep)) = the rows to keep, ascending: all when cache_lens[b] <= keep, else rows
+ *   [0, sink), the last `recent`, and the heaviest of those between (ties: the lower row; NaN is heaviest), keep in all.  -1 behind
+ *   the last.  new_lens [batch] (or NULL) = min(len, keep).  Needs sink + recent <= keep <= rows.
+ * lv_evict_take: out row j of head kvh = in row index[b][kvh][j], for K, V and the weights; rows whose index is -1 are zeroed
+ *   (zero_fill) or left as they are.  The out buffers hold `keep` rows or more and must not overlap the in buffers; an index
+ *   must lie inside the in buffers. */
+int64_t lv_key_weights_workspace_bytes(int batch, int n, int rows, int hq, int hkv);
+int lv_key_weights(const void* q, const void* k, const float* lse, const float* row_weight, const float* w_in, float* w_out,
+                   const int32_t* cache_lens, const int32_t* parents, int64_t parents_batch_stride, void* workspace, int64_t workspace_bytes,
+                   int batch, int n, int rows, int hq, int hkv, int d, int64_t q_batch_stride, int64_t q_token_stride, int64_t q_head_stride,
+                   int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t w_in_batch_stride, int64_t w_in_head_stride,
+                   int64_t w_out_batch_stride, int64_t w_out_head_stride, float softmax_scale, float softcap, const float* slopes, void* stream);
+int64_t lv_evict_workspace_bytes(int batch, int rows, int hkv);
+int lv_evict_index(const float* weight, const int32_t* cache_lens, int32_t* index, int32_t* new_lens, void* workspace, int64_t workspace_bytes,
+                   int batch, int rows, int hkv, int keep, int sink, int recent, int64_t w_batch_stride, int64_t w_head_stride, void* stream);
+int lv_evict_take(const void* k_in, const void* v_in, const float* w_in, const int32_t* index, void* k_out, void* v_out, float* w_out, int batch,
+                  int hkv, int d, int keep, int zero_fill, int64_t k_in_batch_stride, int64_t k_in_row_stride, int64_t k_in_head_stride,
+                  int64_t v_in_batch_stride, int64_t v_in_row_stride, int64_t v_in_head_stride, int64_t w_in_batch_stride,
+                  int64_t w_in_head_stride, int64_t k_out_batch_stride, int64_t k_out_row_stride, int64_t k_out_head_stride,
+                  int64_t v_out_batch_stride, int64_t v_out_row_stride, int64_t v_out_head_stride, int64_t w_out_batch_stride,
+                  int64_t w_out_head_stride, void* stream);
+
 /* ---- attention backward -----------------------------------------------------
  * Replaces the autograd of the calls above (npu_fusion_attention_grad, reached
  * through torch autograd from dot_product_attention.py:352-365 / :314-325) and the

@@ -68,6 +68,11 @@ _SIGNATURES = {
                              _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _int, _vp]),
     "lvattn_tree_workspace_bytes": (_i64, [_int] * 6),
     "lvattn_tree": (_int, [_vp] * 7 + [_i64, _vp, _i64] + [_int] * 6 + [_i64] * 12 + [_f, _f, _vp, _vp]),
+    "lv_key_weights_workspace_bytes": (_i64, [_int] * 5),
+    "lv_key_weights": (_int, [_vp] * 8 + [_i64, _vp, _i64] + [_int] * 6 + [_i64] * 10 + [_f, _f, _vp, _vp]),
+    "lv_evict_workspace_bytes": (_i64, [_int] * 3),
+    "lv_evict_index": (_int, [_vp] * 5 + [_i64] + [_int] * 6 + [_i64, _i64, _vp]),
+    "lv_evict_take": (_int, [_vp] * 7 + [_int] * 5 + [_i64] * 16 + [_vp]),
     "lv_tree_accept": (_int, [_vp] * 6 + [_int] * 5 + [_i64] * 8 + [_vp]),
     "lvattn_decode_noalloc_max_bytes": (_i64, []),
     "lvattn_decode_noalloc": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _int,

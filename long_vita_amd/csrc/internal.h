@@ -136,6 +136,39 @@ struct AcceptParams {
     int64_t k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, w_bs, w_hs;
 };
 
+struct WeightParams {
+    const __bf16* q;
+    const __bf16* k;
+    const float* lse;            // [batch, n, hq]
+    const float* row_weight;     // [batch, n] or null: 1
+    const float* w_in;           // [batch, hkv, rows]
+    float* w_out;                // the same, may be w_in
+    const int32_t* cache_lens;
+    const int32_t* parents;
+    int64_t parents_bs;
+    float* part;                 // [pieces][batch * hkv][rows]
+    int batch, n, rows, hq, hkv, group, pieces;
+    int64_t q_bs, q_ns, q_hs, k_bs, k_rs, k_hs, wi_bs, wi_hs, wo_bs, wo_hs;
+    float scale_log2e;
+    ScoreRule score;
+};
+struct EvictParams {
+    const __bf16* k_in;
+    const __bf16* v_in;
+    const float* w_in;
+    __bf16* k_out;
+    __bf16* v_out;
+    float* w_out;
+    const int32_t* cache_lens;
+    int32_t* index;              // [batch * hkv][keep]
+    int32_t* new_lens;
+    uint32_t* hist;              // [3][batch * hkv][2048]
+    uint32_t* counts;            // [batch * hkv][chunks][2]
+    uint32_t* thr;               // [batch * hkv][2]
+    int batch, rows, hkv, keep, sink, recent, chunks, zero_fill;
+    int64_t ki_bs, ki_rs, ki_hs, vi_bs, vi_rs, vi_hs, wi_bs, wi_hs, ko_bs, ko_rs, ko_hs, vo_bs, vo_rs, vo_hs, wo_bs, wo_hs;
+};
+
 #define LV_BWD_BLOCK_N_INTERNAL 128
 
 struct BwdParams {

@@ -401,6 +401,123 @@ def tree_accept(k: torch.Tensor, v: torch.Tensor, cache_lens: torch.Tensor, path
     return cache_lens + n_accept
 
 
+def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: torch.Tensor, cache_lens: torch.Tensor, scale: float | None = None,
+                parents: torch.Tensor | None = None, softcap: float | None = None, alibi_slopes: torch.Tensor | None = None,
+                row_weight: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The attention weight every cached key received, added to a running sum: weight [b, hkv, rows] fp32 + sum over tokens and
+    query heads of the group of ``row_weight`` * exp(t - lse).  q [b, n, hq, d], k [b, rows, hkv, d], ``cache_lens``, ``parents`` and
+    the score rule as ``tree_attention`` took them, lse [b, n, hq] fp32 as it returned it.  n tokens: a decode step (1), a draft
+    tree (at most 256 with ``parents``) or a whole prompt (``cache_lens`` 0, no parents).
+
+    ``row_weight`` (fp32 [b, n]) weighs the tokens' contributions; a token whose weight is not above 0 (a drafted token that was
+    turned down) or whose lse is -inf counts for nothing, whatever its row of q holds.  Returns a new tensor, or ``out`` (fp32
+    [b, hkv, rows]; ``weight`` itself for an update in place).  Weights of rows that hold no key are carried over.  No gradient."""
+    who = "key_weights"
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
+        raise LvAttnError(f"{who} has no gradient: call it under torch.no_grad() or on tensors that do not require one")
+    b, n, rows, hq, hkv, d = _check_cache(q, k, None, cache_lens, who)
+    _require_gpu(lse, weight, row_weight, out)
+    k = _cache_rows(k, "k", who)
+    if parents is not None and n > TREE_MAX_TOKENS:
+        raise LvAttnError(f"{who}: a tree of {n} tokens (at most {TREE_MAX_TOKENS})")
+    if lse.dtype != torch.float32 or lse.shape != (b, n, hq):
+        raise LvAttnError(f"{who}: lse must be fp32 [{b}, {n}, {hq}]")
+    if row_weight is not None and (row_weight.dtype != torch.float32 or row_weight.shape != (b, n)):
+        raise LvAttnError(f"{who}: row_weight must be fp32 [{b}, {n}]")
+    for name, t in (("weight", weight), ("out", out)):
+        if t is not None and (t.dtype != torch.float32 or t.shape != (b, hkv, rows) or t.stride(2) != 1 or min(t.stride()) < 0):
+            raise LvAttnError(f"{who}: {name} must be fp32 [{b}, {hkv}, {rows}] with contiguous rows")
+    if out is None:
+        out = torch.empty((b, hkv, rows), dtype=torch.float32, device=q.device)
+    elif out.data_ptr() != weight.data_ptr() or out.stride() != weight.stride():
+        if _overlap(out, weight):
+            raise LvAttnError(f"{who}: out must be weight itself or not overlap it")
+    if any(x == 0 and m > 1 for x, m in zip(out.stride(), out.shape)):
+        raise LvAttnError(f"{who}: an expanded tensor cannot be written")
+    if q.stride(3) != 1 or q.data_ptr() % 16 or any(x < 0 or x % 8 for x in q.stride()[:3]):
+        q = q.clone(memory_format=torch.contiguous_format)
+    lse, cache_lens = lse.contiguous(), cache_lens.contiguous()
+    row_weight = None if row_weight is None else row_weight.contiguous()
+    parents, p_bs = _tree_parents(parents, b, n, q.device, who)
+    cap, slopes = _check_rule_args(hq, 0, softcap, alibi_slopes, q.device, who)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not math.isfinite(scale):
+        raise LvAttnError(f"{who}: scale {scale} is not finite")
+    need = int(_lib.lib().lv_key_weights_workspace_bytes(b, n, rows, hq, hkv))
+    ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
+    check(_lib.lib().lv_key_weights(_ptr(q), _ptr(k), _ptr(lse), _ptr(row_weight), _ptr(weight), _ptr(out), _ptr(cache_lens), _ptr(parents), p_bs,
+                                    _ptr(ws), need, b, n, rows, hq, hkv, d, *q.stride()[:3], *k.stride()[:3], *weight.stride()[:2],
+                                    *out.stride()[:2], scale, cap, _ptr(slopes), _stream()), "lv_key_weights")
+    return out
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two tensors meet."""
+    def span(t):
+        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def evict_cache(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, cache_lens: torch.Tensor, keep: int, sink: int = 0, recent: int = 0,
+                out: tuple | None = None):
+    """A KV cache cut down to ``keep`` rows per sequence and KV head: the first ``sink``, the last ``recent`` and the heaviest of
+    those between (``weight`` as ``key_weights`` adds it up; ties stay with the lower row), in their old order.  A sequence of
+    ``keep`` rows or fewer is kept whole.  k / v [b, rows, hkv, d] bf16, weight [b, hkv, rows] fp32, ``cache_lens`` int32 [b] on
+    the device (clamped to [0, rows]).  Every head keeps rows of its own, so row j of the new cache is no position any more:
+    rotate keys before they are cached, and use no distance bias on an evicted cache.
+
+    Returns (k, v, weight, lens, index): the new caches [b, keep, hkv, d] and weights [b, hkv, keep], zero behind a sequence's last
+    row, the new lengths min(len, keep) and index [b, hkv, keep] int32, the old row of every new one (-1 behind the last).
+    ``out`` = (k, v, weight) buffers with ``keep`` rows or more that must not overlap the old ones: their first rows are written,
+    all others are left as they are."""
+    who = "evict_cache"
+    _require_gpu(k, v, weight, cache_lens)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (k, v, weight)):
+        raise LvAttnError(f"{who} has no gradient: call it under torch.no_grad() or on tensors that do not require one")
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.dim() != 4 or k.shape != v.shape or k.shape[3] not in (64, 128) or 0 in k.shape:
+        raise LvAttnError(f"{who}: expects bfloat16 caches [b, rows, hkv, 64 or 128]")
+    b, rows, hkv, d = k.shape
+    keep, sink, recent = int(keep), int(sink), int(recent)
+    if not 1 <= keep <= rows or sink < 0 or recent < 0 or sink + recent > keep:
+        raise LvAttnError(f"{who}: keep {keep} must be 1 to {rows} rows and hold sink {sink} + recent {recent}")
+    if weight.dtype != torch.float32 or weight.shape != (b, hkv, rows) or weight.stride(2) != 1:
+        raise LvAttnError(f"{who}: weight must be fp32 [{b}, {hkv}, {rows}] with contiguous rows")
+    if cache_lens.dtype != torch.int32 or cache_lens.shape != (b,):
+        raise LvAttnError(f"{who}: cache_lens must be int32 [{b}]")
+    k, v = _cache_rows(k, "k", who), _cache_rows(v, "v", who)
+    dev = k.device
+    fresh = out is None
+    if fresh:
+        out = (torch.empty((b, keep, hkv, d), dtype=torch.bfloat16, device=dev), torch.empty((b, keep, hkv, d), dtype=torch.bfloat16, device=dev),
+               torch.empty((b, hkv, keep), dtype=torch.float32, device=dev))
+    k_out, v_out, w_out = out
+    if not fresh:
+        _require_gpu(k_out, v_out, w_out)
+        for name, t in (("k", k_out), ("v", v_out)):
+            if t.dtype != torch.bfloat16 or t.dim() != 4 or t.shape[0] != b or t.shape[1] < keep or t.shape[2:] != k.shape[2:]:
+                raise LvAttnError(f"{who}: out {name} must be bfloat16 [{b}, {keep} or more, {hkv}, {d}]")
+            _cache_rows(t, f"out {name}", who)
+        if w_out.dtype != torch.float32 or w_out.dim() != 3 or w_out.shape[:2] != (b, hkv) or w_out.shape[2] < keep or w_out.stride(2) != 1:
+            raise LvAttnError(f"{who}: out weight must be fp32 [{b}, {hkv}, {keep} or more] with contiguous rows")
+        if any(s == 0 and m > 1 for t in out for s, m in zip(t.stride(), t.shape)):
+            raise LvAttnError(f"{who}: an expanded tensor cannot be written")
+        if any(_overlap(o, i) for o in out for i in (k, v, weight)):
+            raise LvAttnError(f"{who}: the out buffers must not overlap the caches they are filled from")
+    index = torch.empty((b, hkv, keep), dtype=torch.int32, device=dev)
+    lens = torch.empty((b,), dtype=torch.int32, device=dev)
+    need = int(_lib.lib().lv_evict_workspace_bytes(b, rows, hkv))
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
+    check(_lib.lib().lv_evict_index(_ptr(weight), _ptr(cache_lens.contiguous()), _ptr(index), _ptr(lens), _ptr(ws), need, b, rows, hkv, keep, sink, recent,
+                                    *weight.stride()[:2], _stream()), "lv_evict_index")
+    check(_lib.lib().lv_evict_take(_ptr(k), _ptr(v), _ptr(weight), _ptr(index), _ptr(k_out), _ptr(v_out), _ptr(w_out), b, hkv, d, keep, int(fresh),
+                                   *k.stride()[:3], *v.stride()[:3], *weight.stride()[:2], *k_out.stride()[:3], *v_out.stride()[:3],
+                                   *w_out.stride()[:2], _stream()), "lv_evict_take")
+    return k_out, v_out, w_out, lens, index
+
+
 def attn_bwd_launch(q, k, v, out, dout, lse, desc_q: torch.Tensor, desc_k: torch.Tensor, scale: float, causal: bool,
                     dq=None, dk=None, dv=None, delta=None, accum_f32: bool | int = False):
     """Backward of ``attn_fwd_launch``.  ``desc_q`` are the forward's query-block descriptors
