@@ -5,16 +5,21 @@
 //   ancestor of i;  t as in attn_score.hip with token i at position len_b + depth_i;  O = softmax(t) V
 //
 // All query rows of one KV head -- n tokens x the group's heads -- share that head's keys, so they are the 32-wide column
-// blocks of S^T = K Q^T and O^T += V^T P^T (32x32x16 MFMAs) and each K / V byte is read once for all of them.  A workgroup is
-// 4 waves on a tile of 128 keys: WR of them side by side over up to 32 WR query rows, 4 / WR over the tile's keys (few rows:
-// the waves split the keys and are joined through LDS at the end; many rows: every wave sweeps the whole tile).
+// blocks of S^T = K Q^T and O^T += V^T P^T (32x32x16 MFMAs).  A workgroup is WR x WK waves: WR of them side by side over 32 WR
+// query rows (32, 64 or 128), WK over the keys, 32 of every 32 WK-key tile each.  The WR waves of a key slice share its rows of
+// K and V in LDS, brought by direct global -> LDS loads into a ring of tiles that keeps 64 - 96 KB per compute unit on their
+// way; a tile costs one barrier (none with WR = 1, where every wave streams for itself).  The key waves are joined once, at
+// the end.  Two waves per SIMD (WR > 1) put one's exponentials beside the other's matrix products.  Few rows are bound by the
+// cache's bytes, many (row blocks of 128, side by side on one XCD's L2) by the matrix and vector pipes.
 //
-// Few rows are bound by the cache's bytes, many by the matrix products.  The keys of ALL sequences form one list of tiles,
-// dealt evenly to G workgroups per KV head: a workgroup's share may begin inside one sequence and end inside another, so
-// ragged lengths leave no compute unit waiting.  Its result for a sequence goes to partial slot g + s (the pairs (g, s) along
-// the list only ever step forward, so the sum is unique) and a second kernel joins a sequence's slots in order.
+// The keys of ALL sequences form one list of tiles, dealt evenly to G workgroups per KV head: a workgroup's share may begin
+// inside one sequence and end inside another, so ragged lengths leave no compute unit waiting, and the requests run on into
+// the next sequence.  A share's result for a sequence goes to partial slot g + s (the pairs (g, s) along the list only ever
+// step forward, so the sum is unique) and a second kernel joins a sequence's slots in order.
 #include "internal.h"
 #include "../../include/lvattn.h"
+
+#include <type_traits>
 
 typedef __attribute__((address_space(3))) char lds_char;
 
@@ -30,49 +35,77 @@ __device__ __forceinline__ int tree_len(const TreeParams& p, int s) {
     const int len = p.cache_lens[s];
     return min(max(len, 0), p.rows - p.n);   // never outside the cache, whatever the caller's array says
 }
-__device__ __forceinline__ int tree_tiles(const TreeParams& p, int s) { return (tree_len(p, s) + p.n + LV_TREE_TILE - 1) / LV_TREE_TILE; }
 
-// cum[s] = tiles of sequences 0 .. s (one wave); returns after a barrier of the whole workgroup
-__device__ __forceinline__ void tree_scan(const TreeParams& p, int* cum) {
+// cum[s] = tiles of sequences 0 .. s, lens[s] (one wave); returns after a barrier of the whole workgroup
+template <int BN>
+__device__ __forceinline__ void tree_scan(const TreeParams& p, int* cum, int* lens) {
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x;
         int carry = 0;
         for (int s0 = 0; s0 < p.batch; s0 += 64) {
-            int x = s0 + lane < p.batch ? tree_tiles(p, s0 + lane) : 0;
+            const int len = s0 + lane < p.batch ? tree_len(p, s0 + lane) : 0;
+            int x = s0 + lane < p.batch ? (len + p.n + BN - 1) / BN : 0;
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
                 const int y = __shfl_up(x, off);
                 if (lane >= off) x += y;
             }
-            if (s0 + lane < p.batch) cum[s0 + lane] = carry + x;
+            if (s0 + lane < p.batch) {
+                cum[s0 + lane] = carry + x;
+                if (lens) lens[s0 + lane] = len;
+            }
             carry += __shfl(x, 63);
         }
     }
     __syncthreads();
 }
 
+// Direct global -> LDS load, 16 bytes per lane, lane i -> LDS byte lds_dst + 16 i (M0 carries lds_dst; nothing else in this
+// file uses M0, so it is not restored).  As asm so that the
+// compiler does not count it; completion is waited for by hand.
+__device__ __forceinline__ void tree_dma16(__amdgpu_buffer_rsrc_t rs, int voff, uint32_t lds_dst) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "s"(lds_dst) : "memory");
+}
+
+// [slots of K / V tiles][cum][lens][par][depth][anc][stat][obuf]
+#define LV_TREE_LDS_FIXED (LV_TREE_MAX_BATCH * 8 + LV_TREE_MAX_TOKENS * 8 + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4 + 2048 + 16384)
+#define LV_TREE_RING (128 * 1024)
+
+template <int WR>
+struct TreeShape {
+    static constexpr int WK = WR == 4 ? 2 : 4;
+    static constexpr int TILE = 32 * WK;      // keys per tile
+    static constexpr int THREADS = 64 * WR * WK;
+};
+
 template <int D, int WR, int MOD>
-__global__ __launch_bounds__(256, 2) void lv_tree_kernel(TreeParams p) {
-    constexpr int BN = LV_TREE_TILE;
-    constexpr int WK = 4 / WR;            // waves side by side over the keys
-    constexpr int KPW = BN / WK;          // keys of a tile per wave
+__global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(TreeParams p) {
+    constexpr int WK = TreeShape<WR>::WK;
+    constexpr int BN = TreeShape<WR>::TILE;
+    constexpr int NT = TreeShape<WR>::THREADS;
+    constexpr int NW = WR * WK;
+    constexpr int WN = 32;                // keys of a tile per wave
     constexpr int KS = D / 16;
     constexpr int MT = D / 32;
     constexpr int ROWB = D * 2;
-    constexpr int TILEB = BN * ROWB;
+    constexpr int SLICEB = WN * ROWB;     // K or V rows of one key slice
+    constexpr int SLOTB = WK * 2 * SLICEB;        // a tile: [key slice][K rows, V rows]
+    constexpr int NS = LV_TREE_RING / SLOTB > 4 ? 4 : LV_TREE_RING / SLOTB;   // ring slots: 2 or 4
     constexpr int CPR = D / 8;
-    constexpr int NT = 256;
-    constexpr int NLD = (BN * CPR) / NT;
+    constexpr int RPP = 64 / CPR;         // rows per 1-KiB request
+    constexpr int NP = SLICEB / 1024;     // requests per K or V slice: 8 (d = 128) or 4
+    constexpr int NPW = 2 * NP / WR;      // requests per wave and tile
     constexpr float RESCALE_LOG2 = 8.0f;
+    constexpr float OPTIMISTIC_MAX = 4096.0f;
 
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    lds_char* const ldsK = (lds_char*)smem;
-    lds_char* const ldsV = ldsK + TILEB;
-    int* const cum = reinterpret_cast<int*>(smem + 2 * TILEB);          // [LV_TREE_MAX_BATCH]
-    int* const par = cum + LV_TREE_MAX_BATCH;                           // [LV_TREE_MAX_TOKENS]
+    int* const cum = reinterpret_cast<int*>(smem + NS * SLOTB);         // [LV_TREE_MAX_BATCH]
+    int* const lens = cum + LV_TREE_MAX_BATCH;                          // [LV_TREE_MAX_BATCH]
+    int* const par = lens + LV_TREE_MAX_BATCH;                          // [LV_TREE_MAX_TOKENS]
     int* const depth = par + LV_TREE_MAX_TOKENS;                        // [LV_TREE_MAX_TOKENS]
-    uint32_t* const anc = reinterpret_cast<uint32_t*>(depth + LV_TREE_MAX_TOKENS);   // [tokens][words]: ancestors of a token
-    float* const stat = reinterpret_cast<float*>(anc + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32));   // [2][4][32]
+    uint32_t* const anc = reinterpret_cast<uint32_t*>(depth + LV_TREE_MAX_TOKENS);   // [tokens][words]: a token and its ancestors
+    float* const stat = reinterpret_cast<float*>(anc + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32));   // [2][8 waves][32]
+    float* const obuf = stat + 512;                                     // [8 waves][64 lanes][8]: 16 KB
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -89,64 +122,108 @@ __global__ __launch_bounds__(256, 2) void lv_tree_kernel(TreeParams p) {
     if (unit >= p.hkv * p.shares) return;
     const int kvh = unit % p.hkv, g = unit / p.hkv;
 
-    tree_scan(p, cum);
-    const int64_t total = cum[p.batch - 1];
+    tree_scan<BN>(p, cum, lens);
+    const int64_t total = __builtin_amdgcn_readfirstlane(cum[p.batch - 1]);
     const int64_t G = min((int64_t)p.shares, total);
     if (g >= G) return;
-    int64_t tile = g * total / G;
-    const int64_t tile_end = (g + 1) * total / G;
+    int tile = (int)(g * total / G);
+    const int tile_end = (int)((g + 1) * total / G);
     int s = 0;
-    while (cum[s] <= tile) ++s;
+    while (__builtin_amdgcn_readfirstlane(cum[s]) <= tile) ++s;
 
-    const int64_t k_tile = (int64_t)BN * p.k_rs, v_tile = (int64_t)BN * p.v_rs;
-    // thread -> 16-byte chunk tid % CPR of rows tid / CPR + RSTEP i (RSTEP is a period of the LDS swizzle)
-    constexpr int RSTEP = NT / CPR;
-    static_assert(RSTEP % 16 == 0, "the swizzle repeats every 16 rows");
-    const int st_lds = lds_off_tree<D>(tid / CPR, tid % CPR);
-    const int st_koff = (int)(tid / CPR * p.k_rs * 2) + tid % CPR * 16, st_voff = (int)(tid / CPR * p.v_rs * 2) + tid % CPR * 16;
-    const int k_step = (int)(RSTEP * p.k_rs * 2), v_step = (int)(RSTEP * p.v_rs * 2);
-    u32x4 kreg[NLD], vreg[NLD];
-    auto issue_loads = [&](int sq, int t) __attribute__((always_inline)) {
-        const int rows = min(tree_len(p, sq) + p.n - t * BN, BN);       // >= 1: the tile is one of the sequence's
-        // rows past the sequence's last key read as zero (buffer bounds check) and are masked below
-        auto krs = __builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(p.k + (int64_t)sq * p.k_bs + (int64_t)kvh * p.k_hs + t * k_tile), 0,
-                                                     (uint32_t)((rows - 1) * p.k_rs * 2 + ROWB), 0x00020000);
-        auto vrs = __builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(p.v + (int64_t)sq * p.v_bs + (int64_t)kvh * p.v_hs + t * v_tile), 0,
-                                                     (uint32_t)((rows - 1) * p.v_rs * 2 + ROWB), 0x00020000);
+    // ---- requests: this wave's part (NPW requests, K or V rows) of its key slice, tile after tile
+    int it_tile = tile, it_s = s, it_t, it_len, it_end;      // list position, sequence, tile and length of the sequence, its list end
+    auto seek = [&]() __attribute__((always_inline)) {
+        it_t = it_tile - (it_s ? __builtin_amdgcn_readfirstlane(cum[it_s - 1]) : 0);
+        it_len = __builtin_amdgcn_readfirstlane(lens[it_s]);
+        it_end = __builtin_amdgcn_readfirstlane(cum[it_s]);
+    };
+    seek();
+    lds_char* const ring = (lds_char*)smem + wk * 2 * SLICEB;           // this key slice in slot 0
+    const uint32_t ring_addr = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
+    // position -> chunk of the LDS image (the swizzle is an involution); it repeats every 16 rows
+    constexpr int NV = 16 / RPP;
+    int ch16[NV], k_voff[NV], v_voff[NV];
 #pragma unroll
-        for (int i = 0; i < NLD; ++i) {
-            kreg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(krs, st_koff + i * k_step, 0, 0));
-            vreg[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(vrs, st_voff + i * v_step, 0, 0));
+    for (int j = 0; j < NV; ++j) {
+        ch16[j] = lds_off_tree<D>(RPP * j + lane / CPR, lane % CPR) - (RPP * j + lane / CPR) * ROWB;
+        k_voff[j] = lane / CPR * (int)(p.k_rs * 2) + ch16[j];
+        v_voff[j] = lane / CPR * (int)(p.v_rs * 2) + ch16[j];
+    }
+    struct Req { __amdgpu_buffer_rsrc_t rs; int rs2, valid; };
+    auto prepare = [&](const __bf16* base, int64_t bs, int64_t rs, int64_t hs) __attribute__((always_inline)) {
+        const int first = it_t * BN + WN * wk;
+        const int valid = it_tile < tile_end ? min(it_len + p.n - first, WN) : 0;
+        // nothing to bring: zero records, every lane out of range
+        const uint32_t rec = valid > 0 ? (uint32_t)((valid - 1) * rs * 2 + ROWB) : 0u;
+        const __bf16* src = base + (valid > 0 ? (int64_t)it_s * bs + (int64_t)kvh * hs + (int64_t)first * rs : 0);
+        return Req{__builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(src), 0, rec, 0x00020000), (int)(rs * 2), valid};
+    };
+    // request j of a slice's K or V; a partial slice repeats its last key: never bytes that are no key's
+    auto bring = [&](const Req& q, const int (&voff)[NV], uint32_t dst, int j, bool whole) __attribute__((always_inline)) {
+        tree_dma16(q.rs, whole ? voff[j % NV] + RPP * j * q.rs2 : min(RPP * j + lane / CPR, q.valid - 1) * q.rs2 + ch16[j % NV], dst + j * 1024);
+    };
+    auto request_part = [&](const __bf16* base, int64_t bs, int64_t rs, int64_t hs, const int (&voff)[NV], uint32_t dst, auto j0, auto nj)
+                            __attribute__((always_inline)) {
+        const Req q = prepare(base, bs, rs, hs);
+        if (q.valid <= 0 || q.valid >= WN) {
+#pragma unroll
+            for (int j = 0; j < decltype(nj)::value; ++j) bring(q, voff, dst, decltype(j0)::value + j, true);
+        } else {
+#pragma unroll
+            for (int j = 0; j < decltype(nj)::value; ++j) bring(q, voff, dst, decltype(j0)::value + j, false);
         }
     };
-
-    lds_char* k_ptr[KS];   // K row read: row r of the 32-key sub-tile, chunk 2ks + h
+    auto request = [&](int sl) __attribute__((always_inline)) {
+        const uint32_t dst = ring_addr + sl * SLOTB;
+        typedef std::integral_constant<int, 0> Zero;
+        if constexpr (WR == 1) {
+            request_part(p.k, p.k_bs, p.k_rs, p.k_hs, k_voff, dst, Zero{}, std::integral_constant<int, NP>{});
+            request_part(p.v, p.v_bs, p.v_rs, p.v_hs, v_voff, dst + SLICEB, Zero{}, std::integral_constant<int, NP>{});
+        } else if constexpr (WR == 2) {
+            if (wr == 0) request_part(p.k, p.k_bs, p.k_rs, p.k_hs, k_voff, dst, Zero{}, std::integral_constant<int, NP>{});
+            else request_part(p.v, p.v_bs, p.v_rs, p.v_hs, v_voff, dst + SLICEB, Zero{}, std::integral_constant<int, NP>{});
+        } else {
+            if (wr == 0) request_part(p.k, p.k_bs, p.k_rs, p.k_hs, k_voff, dst, Zero{}, std::integral_constant<int, NP / 2>{});
+            else if (wr == 1) request_part(p.k, p.k_bs, p.k_rs, p.k_hs, k_voff, dst, std::integral_constant<int, NP / 2>{}, std::integral_constant<int, NP / 2>{});
+            else if (wr == 2) request_part(p.v, p.v_bs, p.v_rs, p.v_hs, v_voff, dst + SLICEB, Zero{}, std::integral_constant<int, NP / 2>{});
+            else request_part(p.v, p.v_bs, p.v_rs, p.v_hs, v_voff, dst + SLICEB, std::integral_constant<int, NP / 2>{}, std::integral_constant<int, NP / 2>{});
+        }
+        ++it_tile;
+        ++it_t;
+        if (it_tile == it_end && it_tile < tile_end) { ++it_s; seek(); }
+    };
+    // WR = 1 asks for tile t + NS when its own slot is free, WR > 1 for tile t + NS - 1 behind the barrier of tile t
+    constexpr int AHEAD = WR == 1 ? NS : NS - 1;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) k_ptr[ks] = ldsK + lds_off_tree<D>(KPW * wk + r, 2 * ks + h);
+    for (int i = 0; i < AHEAD; ++i) request(i);
+    int sl = 0;                                      // slot of the tile being consumed
+
+    int k_off[KS];     // K row read: row r, chunk 2ks + h
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k_off[ks] = lds_off_tree<D>(r, 2 * ks + h);
     const int i16 = lane & 15, q4 = i16 >> 2, p4 = i16 & 3, gl = (lane >> 4) & 1;
-    lds_char* v_ptr[MT][2];   // V transposed read
+    int v_off[MT][2];  // V transposed read
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int jh = 0; jh < 2; ++jh)
-            v_ptr[mt][jh] = ldsV + lds_off_tree<D>(8 * jh + 4 * h + q4, 4 * mt + 2 * gl + (p4 >> 1)) + 8 * (p4 & 1) + KPW * wk * ROWB;
+            v_off[mt][jh] = SLICEB + lds_off_tree<D>(8 * jh + 4 * h + q4, 4 * mt + 2 * gl + (p4 >> 1)) + 8 * (p4 & 1);
 
     // this lane's query row: row -> (token, head of the group)
-    const int row = 32 * (WR * rb + wr) + r;
     const int n_rows = p.n * p.group;
+    const int row = 32 * (WR * rb + wr) + r;
     const int rowc = min(row, n_rows - 1);
     const int token = rowc / p.group, head = kvh * p.group + rowc % p.group;
     float nslope2 = 0.f;
     if constexpr ((MOD & LV_SCORE_BIAS) != 0) nslope2 = -1.4426950408889634f * p.score.slopes[head];
     const float c = MOD != 0 ? 1.f : p.scale_log2e;
 
-    issue_loads(s, (int)(tile - (s ? cum[s - 1] : 0)));
-
     while (tile < tile_end) {
         // ---------------- one sequence of this share ----------------
-        const int len = tree_len(p, s), keys = len + p.n;
-        const int t0 = (int)(tile - (s ? cum[s - 1] : 0));
-        const int t1 = (int)(min(tile_end, (int64_t)cum[s]) - (s ? cum[s - 1] : 0));
+        const int len = __builtin_amdgcn_readfirstlane(lens[s]), keys = len + p.n;
+        const int list0 = s ? __builtin_amdgcn_readfirstlane(cum[s - 1]) : 0;
+        const int t0 = tile - list0, t1 = min(tile_end, __builtin_amdgcn_readfirstlane(cum[s])) - list0;
         const bool sees_tree = t1 * BN > len;
 
         bf16x8 qf[KS];
@@ -155,7 +232,7 @@ __global__ __launch_bounds__(256, 2) void lv_tree_kernel(TreeParams p) {
         for (int ks = 0; ks < KS; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(qptr + 16 * ks);
 
         int my_depth = token;             // without parents the tokens are a chain
-        bool unused = false;
+        bool live = row < n_rows;
         if (p.parents) {
             const int* pp = p.parents + (int64_t)s * p.parents_bs;
             __syncthreads();              // the previous sequence's arrays are no longer read
@@ -178,73 +255,87 @@ __global__ __launch_bounds__(256, 2) void lv_tree_kernel(TreeParams p) {
             }
             __syncthreads();
             my_depth = depth[token];
-            unused = par[token] == LV_TREE_UNUSED;
+            live = live && par[token] != LV_TREE_UNUSED;
         }
-        const bool live = row < n_rows && !unused;
 
         f32x16 oacc[MT];
+        float m_run = -1e30f, l_run = 0.f;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int i = 0; i < 16; ++i) oacc[mt][i] = 0.f;
-        float m_run = -1e30f, l_run = 0.f;
+        // every ordinary load (and store of the sequence before) retires here: from now on the counter holds requests only
+        asm volatile("" : "+v"(nslope2));
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            asm volatile("" : "+v"(qf[ks]));
+            if (!live) qf[ks] = bf16x8{};      // a row that holds no token: whatever is there stays out
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
         for (int t = t0; t < t1; ++t) {
-            const bool tree_tile = (t + 1) * BN > len;     // holds drafted keys, or keys past the end
-            if (tree_tile && p.parents) {
-                // rows of unused slots hold whatever was there: zero, so that not even a NaN gets through P = 0
+            const int kb0 = t * BN + WN * wk;
+            const bool some = kb0 < keys;            // this wave has keys of the tile
+            const bool masked = kb0 + WN > len;      // ... drafted ones, or rows past the end, among them
+            lds_char* const kb = ring + sl * SLOTB;
+            if constexpr (WR == 1) {
+                // K of this tile: requested before its V and the NS - 1 tiles behind it
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"((2 * NS - 1) * NP) : "memory");
+            } else {
+                // this wave's part of the tile has landed; behind the barrier everyone's has, and everyone is done with the
+                // tile before, whose slot takes the next request
+                asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * NPW) : "memory");
+                request(sl == 0 ? NS - 1 : sl - 1);
+            }
+            f32x16 x;
+            bf16x8 pf[2];     // P rounds to bf16, the matrix pipe's type; its sum is taken before the rounding
 #pragma unroll
-                for (int i = 0; i < NLD; ++i) {
-                    const int j = t * BN + (tid + NT * i) / CPR - len;
-                    if (j >= 0 && j < p.n && par[j] == LV_TREE_UNUSED) { kreg[i] = u32x4{0, 0, 0, 0}; vreg[i] = u32x4{0, 0, 0, 0}; }
+            for (int i = 0; i < 16; ++i) x[i] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const bf16x8 kf = *(LDS_PTR(bf16x8, kb + k_off[ks]));
+                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], x, 0, 0, 0);
+            }
+            if constexpr (MOD != 0) {                // t (log2 units) from the raw products
+                const int jl = kb0 + 4 * h;
+                const float fq = (float)(len + my_depth - jl);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    float dist = fq - (float)((i & 3) + 8 * (i >> 2));
+                    if constexpr ((MOD & LV_SCORE_BIAS) != 0)
+                        if (masked && p.parents) {       // a drafted key stands at its depth, not at its row
+                            const int j = jl + (i & 3) + 8 * (i >> 2) - len;
+                            if (j >= 0) dist = (float)(my_depth - depth[min(j, p.n - 1)]);
+                        }
+                    x[i] = lv_score<MOD>(x[i], p.scale_log2e, p.score, nslope2, dist);
                 }
             }
+            // Optimistic pass (see attn_fwd_pp.hip): with a finite running maximum P is formed against it without looking for
+            // the tile's own; a score far above it shows as a large sum and sends the tile through the exact pass.
+            bool exact = masked || __any(m_run < -1e29f);
+            if (!exact) {
+                const float mc = m_run * c;
+                float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < NLD; ++i) {      // (waits for tile t's loads)
-                *(LDS_PTR(u32x4, ldsK + st_lds + i * RSTEP * ROWB)) = kreg[i];
-                *(LDS_PTR(u32x4, ldsV + st_lds + i * RSTEP * ROWB)) = vreg[i];
+                for (int i = 0; i < 16; ++i) {
+                    const float pv = fast_exp2(__builtin_fmaf(x[i], c, -mc));
+                    sum += pv;
+                    pf[i >> 3][i & 7] = (__bf16)pv;
+                }
+                if (__any(!(sum <= OPTIMISTIC_MAX))) exact = true;      // (also catches inf / nan)
+                else l_run += sum;
             }
-            __syncthreads();
-            ++tile;
-            if (tile < tile_end) issue_loads(t + 1 < t1 ? s : s + 1, t + 1 < t1 ? t + 1 : 0);
-#pragma unroll 1
-            for (int sub = 0; sub < KPW / 32; ++sub) {
-                const int kb0 = t * BN + KPW * wk + 32 * sub;
-                if (kb0 >= keys) break;
-                const int soff = 32 * sub * ROWB;
-                f32x16 x;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) x[i] = 0.f;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const bf16x8 kf = *(LDS_PTR(bf16x8, k_ptr[ks] + soff));
-                    x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], x, 0, 0, 0);
-                }
-                const bool masked = kb0 + 32 > len;
-                if constexpr (MOD != 0) {
-                    const int jl = kb0 + 4 * h;
-                    const float fq = (float)(len + my_depth - jl);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float dist = fq - (float)((i & 3) + 8 * (i >> 2));
-                        if constexpr ((MOD & LV_SCORE_BIAS) != 0)
-                            if (masked && p.parents) {       // a drafted key stands at its depth, not at its row
-                                const int j = jl + (i & 3) + 8 * (i >> 2) - len;
-                                if (j >= 0) dist = (float)(my_depth - depth[min(j, p.n - 1)]);
-                            }
-                        x[i] = lv_score<MOD>(x[i], p.scale_log2e, p.score, nslope2, dist);
-                    }
-                }
+            if (exact) {
                 if (masked) {
                     // bit e of `vis`: key kb0 + e visible to this lane's token
                     uint32_t vis;
-                    const int j0 = kb0 - len;          // first key of the sub-tile, counted from the first drafted one
+                    const int j0 = kb0 - len;          // first key of the slice, counted from the first drafted one
                     if (p.parents) {
                         const uint32_t* aw = anc + token * words;
-                        const int lo = j0 >> 5;        // (arithmetic shift: -1 for a sub-tile that starts in the cache)
-                        const uint32_t a = lo < 0 ? 0xffffffffu : (lo < words ? aw[lo] : 0u);
-                        const uint32_t b = lo + 1 < words ? aw[lo + 1] : 0u;
-                        vis = (uint32_t)((((uint64_t)b << 32) | a) >> (j0 & 31));
+                        const int lo = j0 >> 5;        // (arithmetic shift: -1 for a slice that starts in the cache)
+                        const uint32_t a0 = lo < 0 ? 0xffffffffu : (lo < words ? aw[lo] : 0u);
+                        const uint32_t a1 = lo + 1 < words ? aw[lo + 1] : 0u;
+                        vis = (uint32_t)((((uint64_t)a1 << 32) | a0) >> (j0 & 31));
                     } else {
                         const int last = token - j0;   // keys up to the token's own
                         vis = last >= 31 ? 0xffffffffu : (last < 0 ? 0u : (2u << last) - 1u);
@@ -271,102 +362,108 @@ __global__ __launch_bounds__(256, 2) void lv_tree_kernel(TreeParams p) {
                         for (int i = 0; i < 16; ++i) oacc[mt][i] *= alpha;
                 }
                 const float mc = m_run * c;
-                float rs = 0.f;
-                bf16x8 pf[2];     // P rounds to bf16, the matrix pipe's type; its sum is taken before the rounding
+                float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     const float pv = fast_exp2(__builtin_fmaf(x[i], c, -mc));
-                    rs += pv;
+                    sum += pv;
                     pf[i >> 3][i & 7] = (__bf16)pv;
                 }
-                l_run += rs;
+                l_run += sum;
+            }
+            if constexpr (WR == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((2 * NS - 2) * NP) : "memory");   // V of this tile
+            if (some) {
+                if (masked && p.parents) {
+                    // rows of unused slots hold whatever was there: zero, so that not even a NaN gets through P = 0 (every
+                    // wave that shares the slice writes the same zeros before it reads)
+                    const int vrow = lane >> 1;
+                    const int j = min(kb0 + vrow, keys - 1) - len;
+                    if (j >= 0 && par[j] == LV_TREE_UNUSED)
 #pragma unroll
-                for (int s2 = 0; s2 < 2; ++s2) {
-                    const int voff = soff + 16 * s2 * ROWB;
+                        for (int i = 0; i < CPR / 2; ++i)
+                            *(LDS_PTR(u32x4, kb + SLICEB + vrow * ROWB + ((lane & 1) * (CPR / 2) + i) * 16)) = u32x4{0, 0, 0, 0};
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                }
+#pragma unroll
+                for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, v_ptr[mt][0] + voff));
-                        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, v_ptr[mt][1] + voff));
+                        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, kb + v_off[mt][0] + 16 * s2 * ROWB));
+                        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, kb + v_off[mt][1] + 16 * s2 * ROWB));
                         bf16x8 vf;
                         vf[0] = lo[0]; vf[1] = lo[1]; vf[2] = lo[2]; vf[3] = lo[3];
                         vf[4] = hi[0]; vf[5] = hi[1]; vf[6] = hi[2]; vf[7] = hi[3];
                         oacc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[s2], oacc[mt], 0, 0, 0);
                     }
-                }
             }
-            __syncthreads();        // every wave is done with the tile before it is overwritten
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave is done with the slot
+            if constexpr (WR == 1) request(sl);
+            sl = sl + 1 == NS ? 0 : sl + 1;
+            ++tile;
         }
 
-        // ---------------- this share's result for the sequence -> partial slot g + s ----------------
-        const int64_t part = ((int64_t)(kvh * p.n_rb + rb) * p.slots + g + s) * (32 * WR) + 32 * wr;   // first row of this wave's block
+        // ---------------- join the key waves; this share's result for the sequence -> partial slot g + s ----------------
+        const int64_t part = ((int64_t)(kvh * p.n_rb + rb) * p.slots + g + s) * (32 * WR) + 32 * wr;
         const float unit2 = MOD != 0 ? 0.6931471805599453f : p.scale;
         const float l_w = pair32_sum(l_run);
-        if constexpr (WK == 1) {
-            const float inv = (l_w > 0.f && live) ? 1.f / l_w : 0.f;
-            float* po = p.part_o + (part + r) * D + 4 * h;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4)
-                    *reinterpret_cast<f32x4*>(po + 32 * mt + 8 * g4) =
-                        f32x4{oacc[mt][4 * g4] * inv, oacc[mt][4 * g4 + 1] * inv, oacc[mt][4 * g4 + 2] * inv, oacc[mt][4 * g4 + 3] * inv};
-            if (h == 0) p.part_lse[part + r] = (l_w > 0.f && live) ? m_run * unit2 + __logf(l_w) : -INFINITY;
-        } else {
-            if (h == 0) {
-                stat[w * 32 + r] = m_run;
-                stat[128 + w * 32 + r] = l_w;
-            }
-            __syncthreads();
-            float m_tot = -1e30f;
-#pragma unroll
-            for (int i = 0; i < WK; ++i) m_tot = fmaxf(m_tot, stat[(i * WR + wr) * 32 + r]);
-            float l_tot = 0.f;
-#pragma unroll
-            for (int i = 0; i < WK; ++i) l_tot += stat[128 + (i * WR + wr) * 32 + r] * fast_exp2((stat[(i * WR + wr) * 32 + r] - m_tot) * c);
-            const float sc = fast_exp2((m_run - m_tot) * c);
-            float* const obuf = reinterpret_cast<float*>(smem);           // the (free) tile memory: [4 waves][MT][64 lanes][16]
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                float* dst = obuf + ((w * MT + mt) * 64 + lane) * 16;
-#pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4)
-                    *reinterpret_cast<f32x4*>(dst + 4 * g4) = f32x4{oacc[mt][4 * g4] * sc, oacc[mt][4 * g4 + 1] * sc,
-                                                                     oacc[mt][4 * g4 + 2] * sc, oacc[mt][4 * g4 + 3] * sc};
-            }
-            __syncthreads();
-            const float inv = (l_tot > 0.f && live) ? 1.f / l_tot : 0.f;
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                if (mt % WK != wk) continue;       // the key waves of a row block share out its d columns
-                f32x4 acc[4];
-#pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4) acc[g4] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < WK; ++i) {
-                    const float* src = obuf + (((i * WR + wr) * MT + mt) * 64 + lane) * 16;
-#pragma unroll
-                    for (int g4 = 0; g4 < 4; ++g4) acc[g4] += *reinterpret_cast<const f32x4*>(src + 4 * g4);
-                }
-                float* po = p.part_o + (part + r) * D + 32 * mt + 4 * h;
-#pragma unroll
-                for (int g4 = 0; g4 < 4; ++g4) *reinterpret_cast<f32x4*>(po + 8 * g4) = acc[g4] * inv;
-            }
-            if (wk == 0 && h == 0) p.part_lse[part + r] = (l_tot > 0.f && live) ? m_tot * unit2 + __logf(l_tot) : -INFINITY;
-            __syncthreads();        // the next tile goes where obuf is
+        if (h == 0) {
+            stat[w * 32 + r] = m_run;
+            stat[256 + w * 32 + r] = l_w;
         }
+        __syncthreads();
+        float m_tot = -1e30f, l_tot = 0.f;
+#pragma unroll
+        for (int i = 0; i < WK; ++i) m_tot = fmaxf(m_tot, stat[(i * WR + wr) * 32 + r]);
+#pragma unroll
+        for (int i = 0; i < WK; ++i) l_tot += stat[256 + (i * WR + wr) * 32 + r] * fast_exp2((stat[(i * WR + wr) * 32 + r] - m_tot) * c);
+        const float sc = fast_exp2((m_run - m_tot) * c);
+        const float inv = (l_tot > 0.f && live) ? 1.f / l_tot : 0.f;
+        if (wk == 0 && h == 0) p.part_lse[part + r] = (l_tot > 0.f && live) ? m_tot * unit2 + __logf(l_tot) : -INFINITY;
+        // eight accumulators of a lane at a time: [wave][4-float half][lane]; key wave wk then finishes 8 / WK of them
+        typedef __attribute__((ext_vector_type(8 / WK))) float fpart;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+#pragma unroll
+                for (int x4 = 0; x4 < 2; ++x4) {
+                    const int i = 8 * hf + 4 * x4;
+                    *reinterpret_cast<f32x4*>(obuf + ((w * 2 + x4) * 64 + lane) * 4) =
+                        f32x4{oacc[mt][i] * sc, oacc[mt][i + 1] * sc, oacc[mt][i + 2] * sc, oacc[mt][i + 3] * sc};
+                }
+                __syncthreads();
+                const int e0 = wk * (8 / WK);             // first of this wave's floats: half e0 / 4, place e0 % 4
+                fpart acc = {};
+#pragma unroll
+                for (int i = 0; i < WK; ++i) acc += *reinterpret_cast<const fpart*>(obuf + (((i * WR + wr) * 2 + e0 / 4) * 64 + lane) * 4 + e0 % 4);
+#pragma unroll
+                for (int e = 0; e < 8 / WK; ++e) acc[e] = inv > 0.f ? acc[e] * inv : 0.f;
+                *reinterpret_cast<fpart*>(p.part_o + (part + r) * D + 32 * mt + 8 * (2 * hf + e0 / 4) + 4 * h + e0 % 4) = acc;
+                __syncthreads();
+            }
         ++s;
     }
+    // no request may outlive the workgroup: its LDS could already belong to another one
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// out / lse of a row = the log-sum-exp merge of its sequence's slots, in order.  Eight rows per workgroup, 32 threads per row.
-template <int D>
-__global__ __launch_bounds__(256) void lv_tree_join_kernel(TreeParams p, int rows_pb) {
+// out / lse of a row = the log-sum-exp merge of its sequence's slots; every sum has a fixed order.  D / 4 threads take a slot's
+// columns; the 1024 / D groups of them share one row's slots (JR = 1: many shares per sequence) or take a row each (few).
+template <int D, int WR, bool ONE_ROW>
+__global__ __launch_bounds__(256) void lv_tree_join_kernel(TreeParams p) {
+    constexpr int rows_pb = 32 * WR;
+    constexpr int TPR = D / 4;                // threads per slot row
+    constexpr int GR = 256 / TPR;             // groups
     __shared__ int cum[LV_TREE_MAX_BATCH];
-    tree_scan(p, cum);
+    __shared__ float wgt[ONE_ROW ? LV_TREE_MAX_SHARES : 1];
+    __shared__ float red[8];
+    __shared__ f32x4 osum[GR][TPR];
+    const int tid = threadIdx.x, gr = tid / TPR, col = tid % TPR * 4;
+    tree_scan<TreeShape<WR>::TILE>(p, cum, nullptr);
     const int64_t total = cum[p.batch - 1];
     const int64_t G = min((int64_t)p.shares, total);
-    const int64_t idx = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;       // (sequence, KV head, row)
     const int n_rows = p.n * p.group;
+    const int64_t idx = ONE_ROW ? blockIdx.x : (int64_t)blockIdx.x * GR + gr;     // (sequence, KV head, row)
     if (idx >= (int64_t)p.batch * p.hkv * n_rows) return;
     const int row = (int)(idx % n_rows), kvh = (int)(idx / n_rows % p.hkv), s = (int)(idx / n_rows / p.hkv);
     const int64_t first = s ? cum[s - 1] : 0, last = cum[s] - 1;
@@ -374,63 +471,93 @@ __global__ __launch_bounds__(256) void lv_tree_join_kernel(TreeParams p, int row
     const int64_t g0 = ((first + 1) * G - 1) / total, g1 = ((last + 1) * G - 1) / total;
     const int rb = row / rows_pb;
     const int64_t part = ((int64_t)(kvh * p.n_rb + rb) * p.slots + g0 + s) * rows_pb + row % rows_pb;
-    const int np = (int)(g1 - g0 + 1);
+    const int np = (int)(g1 - g0 + 1);        // at most shares
     const float* lp = p.part_lse + part;
-    float m = -INFINITY;
-    for (int i = 0; i < np; ++i) m = fmaxf(m, lp[(int64_t)i * rows_pb]);
-    constexpr int C = D / 32;                 // columns per thread
-    const int col = (threadIdx.x & 31) * C;
-    float acc[C], tot = 0.f;
+    const float* po = p.part_o + part * D + col;
+    float m = -INFINITY, tot = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (ONE_ROW) {
+        for (int i = tid; i < np; i += 256) {
+            const float x = lp[(int64_t)i * rows_pb];
+            wgt[i] = x;
+            m = fmaxf(m, x);
+        }
 #pragma unroll
-    for (int e = 0; e < C; ++e) acc[e] = 0.f;
-    if (m > -INFINITY) {
-        const float* po = p.part_o + part * D + col;
+        for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off));
+        if ((tid & 63) == 0) red[tid >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        for (int i = tid; i < np; i += 256) {
+            const float x = m > -INFINITY ? __expf(wgt[i] - m) : 0.f;
+            wgt[i] = x;
+            tot += x;
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) tot += __shfl_xor(tot, off);
+        if ((tid & 63) == 0) red[4 + (tid >> 6)] = tot;
+        __syncthreads();
+        tot = red[4] + red[5] + red[6] + red[7];
 #pragma unroll 4
-        for (int i = 0; i < np; ++i) {
-            const float wgt = __expf(lp[(int64_t)i * rows_pb] - m);
-            tot += wgt;
+        for (int i = gr; i < np; i += GR) acc += wgt[i] * *reinterpret_cast<const f32x4*>(po + (int64_t)i * rows_pb * D);
+        osum[gr][tid % TPR] = acc;
+        __syncthreads();
+        if (gr > 0) return;
 #pragma unroll
-            for (int e = 0; e < C; ++e) acc[e] += wgt * po[(int64_t)i * rows_pb * D + e];
+        for (int i = 1; i < GR; ++i) acc += osum[i][tid];
+    } else {
+        for (int i = 0; i < np; ++i) m = fmaxf(m, lp[(int64_t)i * rows_pb]);
+        if (m > -INFINITY) {
+#pragma unroll 4
+            for (int i = 0; i < np; ++i) {
+                const float x = __expf(lp[(int64_t)i * rows_pb] - m);
+                tot += x;
+                acc += x * *reinterpret_cast<const f32x4*>(po + (int64_t)i * rows_pb * D);
+            }
         }
     }
     const float inv = tot > 0.f ? 1.f / tot : 0.f;
     const int token = row / p.group, head = kvh * p.group + row % p.group;
     __bf16* op = p.o + (int64_t)s * p.o_bs + (int64_t)token * p.o_ns + (int64_t)head * p.o_hs + col;
 #pragma unroll
-    for (int e = 0; e < C; ++e) op[e] = (__bf16)(acc[e] * inv);
-    if (p.lse && (threadIdx.x & 31) == 0) p.lse[((int64_t)s * p.n + token) * p.hq + head] = tot > 0.f ? m + __logf(tot) : -INFINITY;
+    for (int e = 0; e < 4; ++e) op[e] = (__bf16)(acc[e] * inv);
+    if (p.lse && col == 0) p.lse[((int64_t)s * p.n + token) * p.hq + head] = tot > 0.f ? m + __logf(tot) : -INFINITY;
 }
 
-// query rows per workgroup: 32, 64 or 128.  Up to 32 rows all four waves split the keys; from 65 on none do
-static int tree_rows_per_block(int n_rows) { return n_rows <= 32 ? 32 : (n_rows <= 64 ? 64 : 128); }
-
-struct TreePlan { int rows_pb, n_rb, shares, slots; int64_t part_rows; };
-// Shares per KV head: two workgroups fit a compute unit, so 512 workgroups fill the chip once; never more shares than tiles.
+struct TreePlan { int wr, n_rb, shares, slots; int64_t part_rows; };
+// Rows per workgroup: 32, 64 or 128.  Shares per KV head: a workgroup's ring fills a compute unit's LDS, so 256 workgroups fill
+// the chip, and one more would wait for a second round; never more shares than tiles.
 static TreePlan tree_plan(int batch, int n, int rows, int hq, int hkv) {
     TreePlan t;
     const int n_rows = n * (hq / hkv);
-    t.rows_pb = tree_rows_per_block(n_rows);
-    t.n_rb = (n_rows + t.rows_pb - 1) / t.rows_pb;
-    const int64_t tiles = (int64_t)batch * ((rows + LV_TREE_TILE - 1) / LV_TREE_TILE);
-    int64_t g = (512 + (int64_t)hkv * t.n_rb - 1) / ((int64_t)hkv * t.n_rb);
+    t.wr = n_rows <= 32 ? 1 : (n_rows <= 64 ? 2 : 4);
+    t.n_rb = (n_rows + 32 * t.wr - 1) / (32 * t.wr);
+    const int tile = t.wr == 4 ? TreeShape<4>::TILE : TreeShape<1>::TILE;
+    const int64_t tiles = (int64_t)batch * ((rows + tile - 1) / tile);
+    int64_t g = 256 / ((int64_t)hkv * t.n_rb);
     if (g > tiles) g = tiles;
-    t.shares = (int)g;
+    if (g < 1) g = 1;
+    t.shares = (int)g;                                  // <= 256 = LV_TREE_MAX_SHARES
     t.slots = (int)g + batch - 1;
-    t.part_rows = (int64_t)hkv * t.n_rb * t.slots * t.rows_pb;
+    t.part_rows = (int64_t)hkv * t.n_rb * t.slots * 32 * t.wr;
     return t;
 }
 
 template <int D, int WR>
-static void launch_tree(const TreeParams& p, int mod, dim3 grid, hipStream_t stream) {
-    const size_t lds = (size_t)2 * LV_TREE_TILE * D * 2 + LV_TREE_MAX_BATCH * 4 + LV_TREE_MAX_TOKENS * 8 +
-                       LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4 + 1024;
-    // (D = 64: the join buffer of the epilogue, 4 waves x 2 x 4 KB, is as large as the two tiles)
+static void launch_tree(const TreeParams& p, int mod, unsigned blocks, int64_t out_rows, hipStream_t stream) {
+    const dim3 grid(blocks), block(TreeShape<WR>::THREADS);
+    constexpr int slot = TreeShape<WR>::WK * 2 * 32 * D * 2;
+    constexpr size_t lds = (size_t)(LV_TREE_RING / slot > 4 ? 4 : LV_TREE_RING / slot) * slot + LV_TREE_LDS_FIXED;
+    static_assert(lds <= 160 * 1024, "one workgroup per compute unit");
     switch (mod) {
-        case 0: hipLaunchKernelGGL((lv_tree_kernel<D, WR, 0>), grid, dim3(256), lds, stream, p); break;
-        case LV_SCORE_CAP: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_CAP>), grid, dim3(256), lds, stream, p); break;
-        case LV_SCORE_BIAS: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_BIAS>), grid, dim3(256), lds, stream, p); break;
-        default: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_CAP | LV_SCORE_BIAS>), grid, dim3(256), lds, stream, p);
+        case 0: hipLaunchKernelGGL((lv_tree_kernel<D, WR, 0>), grid, block, lds, stream, p); break;
+        case LV_SCORE_CAP: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_CAP>), grid, block, lds, stream, p); break;
+        case LV_SCORE_BIAS: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_BIAS>), grid, block, lds, stream, p); break;
+        default: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_CAP | LV_SCORE_BIAS>), grid, block, lds, stream, p);
     }
+    if (hipPeekAtLastError() != hipSuccess) return;   // (reported by the caller)
+    // a group of threads walks its row's slots one after the other: worth it while there are few
+    if (p.shares > 32) hipLaunchKernelGGL((lv_tree_join_kernel<D, WR, true>), dim3((unsigned)out_rows), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((lv_tree_join_kernel<D, WR, false>), dim3((unsigned)((out_rows * (D / 4) + 255) / 256)), dim3(256), 0, stream, p);
 }
 
 extern "C" int64_t lvattn_tree_workspace_bytes(int batch, int n, int rows, int hq, int hkv, int d) {
@@ -452,12 +579,12 @@ extern "C" int lvattn_tree(const void* q, const void* k, const void* v, void* ou
     if (((k_bs | v_bs) & 7) || k_bs < 0 || v_bs < 0) return lv_fail(LV_EINVAL, "lvattn_tree: K / V batch strides must be non-negative multiples of 8 elements");
     if (((uintptr_t)workspace & 15) || parents_batch_stride < 0) return lv_fail(LV_EINVAL, "lvattn_tree: workspace must be 16-byte aligned, the parents' stride not negative");
     if (!(softcap >= 0.f) || softcap > 1e30f) return lv_fail(LV_EINVAL, "lvattn_tree: softcap %g must be a finite number above 0 (0: no cap)", (double)softcap);
-    if (!(softmax_scale > -1e30f && softmax_scale < 1e30f)) return lv_fail(LV_EINVAL, "lvattn_tree: softmax_scale is not finite");
+    if (!(softmax_scale > 0.f && softmax_scale < 1e30f)) return lv_fail(LV_EINVAL, "lvattn_tree: softmax_scale %g must be a finite number above 0", (double)softmax_scale);
     const TreePlan t = tree_plan(batch, n, rows, hq, hkv);
     const int64_t need = t.part_rows * (d + 1) * (int64_t)sizeof(float);
     if (workspace_bytes < need) return lv_fail(LV_ESIZE, "lvattn_tree: %lld bytes of workspace needed, room for %lld", (long long)need, (long long)workspace_bytes);
     const int64_t units = (int64_t)hkv * t.shares, blocks = (units + 7) / 8 * 8 * t.n_rb;
-    const int64_t join = ((int64_t)batch * hkv * n * (hq / hkv) + 7) / 8;
+    const int64_t join = (int64_t)batch * hkv * n * (hq / hkv);
     if (blocks > 0x7fffffffLL || join > 0x7fffffffLL) return lv_fail(LV_EINVAL, "lvattn_tree: grid too large");
     TreeParams p{};
     p.q = (const __bf16*)q; p.k = (const __bf16*)k; p.v = (const __bf16*)v; p.o = (__bf16*)out; p.lse = lse;
@@ -470,20 +597,17 @@ extern "C" int lvattn_tree(const void* q, const void* k, const void* v, void* ou
     p.scale = softmax_scale; p.scale_log2e = softmax_scale * 1.4426950408889634f;
     p.score = lv_score_rule(softmax_scale, softcap, slopes);
     const int mod = lv_score_mod(softcap, slopes) & (LV_SCORE_CAP | LV_SCORE_BIAS);
-    const dim3 grid((unsigned)blocks);
+    hipStream_t st = (hipStream_t)stream;
     if (d == 128) {
-        if (t.rows_pb == 32) launch_tree<128, 1>(p, mod, grid, (hipStream_t)stream);
-        else if (t.rows_pb == 64) launch_tree<128, 2>(p, mod, grid, (hipStream_t)stream);
-        else launch_tree<128, 4>(p, mod, grid, (hipStream_t)stream);
+        if (t.wr == 1) launch_tree<128, 1>(p, mod, (unsigned)blocks, join, st);
+        else if (t.wr == 2) launch_tree<128, 2>(p, mod, (unsigned)blocks, join, st);
+        else launch_tree<128, 4>(p, mod, (unsigned)blocks, join, st);
     } else {
-        if (t.rows_pb == 32) launch_tree<64, 1>(p, mod, grid, (hipStream_t)stream);
-        else if (t.rows_pb == 64) launch_tree<64, 2>(p, mod, grid, (hipStream_t)stream);
-        else launch_tree<64, 4>(p, mod, grid, (hipStream_t)stream);
+        if (t.wr == 1) launch_tree<64, 1>(p, mod, (unsigned)blocks, join, st);
+        else if (t.wr == 2) launch_tree<64, 2>(p, mod, (unsigned)blocks, join, st);
+        else launch_tree<64, 4>(p, mod, (unsigned)blocks, join, st);
     }
-    if (hipGetLastError() != hipSuccess) return lv_fail(LV_ELAUNCH, "lvattn_tree: launch failed");
-    if (d == 128) hipLaunchKernelGGL((lv_tree_join_kernel<128>), dim3((unsigned)join), dim3(256), 0, (hipStream_t)stream, p, t.rows_pb);
-    else hipLaunchKernelGGL((lv_tree_join_kernel<64>), dim3((unsigned)join), dim3(256), 0, (hipStream_t)stream, p, t.rows_pb);
-    return hipGetLastError() == hipSuccess ? LV_OK : lv_fail(LV_ELAUNCH, "lvattn_tree: launch failed");
+    return hipPeekAtLastError() == hipSuccess ? LV_OK : lv_fail(LV_ELAUNCH, "lvattn_tree: launch failed: %s", hipGetErrorString(hipGetLastError()));
 }
 
 // ---------------------------------------------------------------------------

@@ -106,9 +106,9 @@ struct DecodeParams {
 int lv_launch_decode(const DecodeParams& p, int d, hipStream_t stream);
 
 // Drafted tokens over a KV cache: q [batch, n, hq, d], k / v [batch, rows, hkv, d], out [batch, n, hq, d].
-#define LV_TREE_TILE 128
 #define LV_TREE_MAX_TOKENS 256
 #define LV_TREE_MAX_BATCH 512
+#define LV_TREE_MAX_SHARES 256
 struct TreeParams {
     const __bf16* q;
     const __bf16* k;
@@ -118,7 +118,7 @@ struct TreeParams {
     const int32_t* cache_lens;   // [batch]
     const int32_t* parents;      // [n] per sequence, or null: a chain
     int64_t parents_bs;
-    float* part_o;               // [hkv][n_rb][slots][rows per block][d]
+    float* part_o;               // [hkv][n_rb][slots][32 * WR][d]
     float* part_lse;             // the same without d
     int batch, n, rows, hq, hkv, group, n_rb, shares, slots;
     int64_t q_bs, q_ns, q_hs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, o_bs, o_ns, o_hs;

@@ -347,8 +347,8 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_lens
     parents, p_bs = _tree_parents(parents, b, n, q.device, who)
     cap, slopes = _check_rule_args(hq, 0, softcap, alibi_slopes, q.device, who)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise LvAttnError(f"{who}: scale {scale} is not finite")
+    if not 0.0 < scale < 1e30:
+        raise LvAttnError(f"{who}: scale {scale} must be a finite number above 0")
     if out is None:
         out = torch.empty((b, n, hq, d), dtype=torch.bfloat16, device=q.device)
     elif out.shape != (b, n, hq, d) or out.dtype != torch.bfloat16 or out.device != q.device or out.stride(3) != 1:

@@ -291,6 +291,7 @@ REFUSED = [
     ("cap", lambda q, k, v, L: ((q, k, v, L), dict(softcap=-1.0))),
     ("slopes", lambda q, k, v, L: ((q, k, v, L), dict(alibi_slopes=torch.zeros(2, device=q.device)))),
     ("scale", lambda q, k, v, L: ((q, k, v, L, float("nan")), {})),
+    ("scale_zero", lambda q, k, v, L: ((q, k, v, L, 0.0), {})),
     ("grad", lambda q, k, v, L: ((q.clone().requires_grad_(True), k, v, L), {})),
     ("out", lambda q, k, v, L: ((q, k, v, L), dict(out=torch.empty(1, device=q.device)))),
     ("lse", lambda q, k, v, L: ((q, k, v, L), dict(lse=torch.empty(1, device=q.device)))),
