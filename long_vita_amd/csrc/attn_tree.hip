@@ -6,7 +6,7 @@
 //
 // All query rows of one KV head -- n tokens x the group's heads -- share that head's keys, so they are the 32-wide column
 // blocks of S^T = K Q^T and O^T += V^T P^T (32x32x16 MFMAs).  A workgroup is WR x WK waves: WR of them side by side over 32 WR
-// query rows (32, 64 or 128), WK over the keys, 32 of every 32 WK-key tile each.  The WR waves of a key slice share its rows of
+// query rows (32, 64 or 128), WK over the keys, 32 or 64 of every 128-key tile each.  The WR waves of a key slice share its rows of
 // K and V in LDS, brought by direct global -> LDS loads into a ring of tiles that keeps 64 - 96 KB per compute unit on their
 // way; a tile costs one barrier (none with WR = 1, where every wave streams for itself).  The key waves are joined once, at
 // the end.  Two waves per SIMD (WR > 1) put one's exponentials beside the other's matrix products.  Few rows are bound by the
@@ -74,8 +74,13 @@ __device__ __forceinline__ void tree_dma16(__amdgpu_buffer_rsrc_t rs, int voff, 
 template <int WR>
 struct TreeShape {
     static constexpr int WK = WR == 4 ? 2 : 4;
-    static constexpr int TILE = 32 * WK;      // keys per tile
+    static constexpr int SUB = WR == 4 ? 2 : 1;   // 32-key slices per key wave and tile
+    static constexpr int TILE = 32 * WK * SUB;    // keys per tile: 128
+    static_assert(TILE == 128, "tree_plan counts tiles of 128 keys");
     static constexpr int THREADS = 64 * WR * WK;
+    template <int D> static constexpr int slot_bytes() { return TILE * 2 * D * 2; }       // a tile of K and V
+    template <int D> static constexpr int slots() { return WR == 4 ? 2 : (LV_TREE_RING / slot_bytes<D>() > 4 ? 4 : LV_TREE_RING / slot_bytes<D>()); }
+    template <int D> static constexpr int lds_bytes() { return slots<D>() * slot_bytes<D>() + LV_TREE_LDS_FIXED; }
 };
 
 template <int D, int WR, int MOD>
@@ -84,17 +89,20 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
     constexpr int BN = TreeShape<WR>::TILE;
     constexpr int NT = TreeShape<WR>::THREADS;
     constexpr int NW = WR * WK;
-    constexpr int WN = 32;                // keys of a tile per wave
+    constexpr int SUB = TreeShape<WR>::SUB;
+    constexpr int WN = 32;                // keys per slice
     constexpr int KS = D / 16;
     constexpr int MT = D / 32;
     constexpr int ROWB = D * 2;
     constexpr int SLICEB = WN * ROWB;     // K or V rows of one key slice
-    constexpr int SLOTB = WK * 2 * SLICEB;        // a tile: [key slice][K rows, V rows]
-    constexpr int NS = LV_TREE_RING / SLOTB > 4 ? 4 : LV_TREE_RING / SLOTB;   // ring slots: 2 or 4
+    constexpr int SLOTB = TreeShape<WR>::template slot_bytes<D>();            // a tile: [slice][K rows, V rows]
+    constexpr int NS = TreeShape<WR>::template slots<D>();                    // ring slots: 2 or 4
+    static_assert(SLOTB == WK * SUB * 2 * SLICEB && NS >= 2, "ring layout");
     constexpr int CPR = D / 8;
     constexpr int RPP = 64 / CPR;         // rows per 1-KiB request
     constexpr int NP = SLICEB / 1024;     // requests per K or V slice: 8 (d = 128) or 4
-    constexpr int NPW = 2 * NP / WR;      // requests per wave and tile
+    constexpr int NPW = 2 * SUB * NP / WR;        // requests per wave and tile
+    constexpr bool PP = WR == 4;          // ping-pong: key waves 0 and 1, the two waves of a SIMD, one phase apart
     constexpr float RESCALE_LOG2 = 8.0f;
     constexpr float OPTIMISTIC_MAX = 4096.0f;
 
@@ -139,64 +147,62 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
         it_end = __builtin_amdgcn_readfirstlane(cum[it_s]);
     };
     seek();
-    lds_char* const ring = (lds_char*)smem + wk * 2 * SLICEB;           // this key slice in slot 0
+    lds_char* const ring = (lds_char*)smem + wk * SUB * 2 * SLICEB;     // this wave's slices in slot 0
     const uint32_t ring_addr = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
-    // position -> chunk of the LDS image (the swizzle is an involution); it repeats every 16 rows
+    // one operand's rows as this wave asks for them: position -> chunk of the LDS image (the swizzle is an involution and
+    // repeats every 16 rows)
     constexpr int NV = 16 / RPP;
-    int ch16[NV], k_voff[NV], v_voff[NV];
+    struct Rows { const __bf16* base; int64_t bs, rs; int voff[NV]; };
+    auto rows_of = [&](const __bf16* base, int64_t bs, int64_t rs, int64_t hs) __attribute__((always_inline)) {
+        Rows x{base + (int64_t)kvh * hs, bs, rs, {}};
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        ch16[j] = lds_off_tree<D>(RPP * j + lane / CPR, lane % CPR) - (RPP * j + lane / CPR) * ROWB;
-        k_voff[j] = lane / CPR * (int)(p.k_rs * 2) + ch16[j];
-        v_voff[j] = lane / CPR * (int)(p.v_rs * 2) + ch16[j];
-    }
-    struct Req { __amdgpu_buffer_rsrc_t rs; int rs2, valid; };
-    auto prepare = [&](const __bf16* base, int64_t bs, int64_t rs, int64_t hs) __attribute__((always_inline)) {
-        const int first = it_t * BN + WN * wk;
+        for (int j = 0; j < NV; ++j)
+            x.voff[j] = lane / CPR * (int)(rs * 2) + lds_off_tree<D>(RPP * j + lane / CPR, lane % CPR) - (RPP * j + lane / CPR) * ROWB;
+        return x;
+    };
+    const bool v_part = WR > 1 && (wr & 1);          // WR > 1: even row waves bring K, odd ones V
+    const Rows own = rows_of(v_part ? p.v : p.k, v_part ? p.v_bs : p.k_bs, v_part ? p.v_rs : p.k_rs, v_part ? p.v_hs : p.k_hs);
+    const Rows own_v = WR == 1 ? rows_of(p.v, p.v_bs, p.v_rs, p.v_hs) : own;
+    auto request_slice = [&](const Rows& x, uint32_t dst, int u) __attribute__((always_inline)) {
+        int first = it_t * BN + WN * (wk * SUB + u);
+        // (ping-pong multiplies every slice: one behind the last key repeats it)
+        if constexpr (PP) first = min(first, it_len + p.n - 1);
         const int valid = it_tile < tile_end ? min(it_len + p.n - first, WN) : 0;
         // nothing to bring: zero records, every lane out of range
-        const uint32_t rec = valid > 0 ? (uint32_t)((valid - 1) * rs * 2 + ROWB) : 0u;
-        const __bf16* src = base + (valid > 0 ? (int64_t)it_s * bs + (int64_t)kvh * hs + (int64_t)first * rs : 0);
-        return Req{__builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(src), 0, rec, 0x00020000), (int)(rs * 2), valid};
-    };
-    // request j of a slice's K or V; a partial slice repeats its last key: never bytes that are no key's
-    auto bring = [&](const Req& q, const int (&voff)[NV], uint32_t dst, int j, bool whole) __attribute__((always_inline)) {
-        tree_dma16(q.rs, whole ? voff[j % NV] + RPP * j * q.rs2 : min(RPP * j + lane / CPR, q.valid - 1) * q.rs2 + ch16[j % NV], dst + j * 1024);
-    };
-    auto request_part = [&](const __bf16* base, int64_t bs, int64_t rs, int64_t hs, const int (&voff)[NV], uint32_t dst, auto j0, auto nj)
-                            __attribute__((always_inline)) {
-        const Req q = prepare(base, bs, rs, hs);
-        if (q.valid <= 0 || q.valid >= WN) {
+        const uint32_t rec = valid > 0 ? (uint32_t)((valid - 1) * x.rs * 2 + ROWB) : 0u;
+        const __bf16* src = x.base + (valid > 0 ? (int64_t)it_s * x.bs + (int64_t)first * x.rs : 0);
+        auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(src), 0, rec, 0x00020000);
+        const int rs2 = (int)(x.rs * 2);
+        if (valid <= 0 || valid >= WN) {
 #pragma unroll
-            for (int j = 0; j < decltype(nj)::value; ++j) bring(q, voff, dst, decltype(j0)::value + j, true);
-        } else {
+            for (int j = 0; j < NP; ++j) tree_dma16(rsrc, x.voff[j % NV] + RPP * j * rs2, dst + j * 1024);
+        } else {                                     // rows past the last key repeat it: never bytes that are no key's
+            const int lr = lane / CPR;
 #pragma unroll
-            for (int j = 0; j < decltype(nj)::value; ++j) bring(q, voff, dst, decltype(j0)::value + j, false);
+            for (int j = 0; j < NP; ++j) tree_dma16(rsrc, x.voff[j % NV] + (min(RPP * j + lr, valid - 1) - lr) * rs2, dst + j * 1024);
         }
     };
+    static_assert(WR == 1 ? SUB == 1 : 2 * SUB == WR, "WR > 1: every wave brings one slice's K or V rows");
     auto request = [&](int sl) __attribute__((always_inline)) {
-        const uint32_t dst = ring_addr + sl * SLOTB;
-        typedef std::integral_constant<int, 0> Zero;
-        if constexpr (WR == 1) {
-            request_part(p.k, p.k_bs, p.k_rs, p.k_hs, k_voff, dst, Zero{}, std::integral_constant<int, NP>{});
-            request_part(p.v, p.v_bs, p.v_rs, p.v_hs, v_voff, dst + SLICEB, Zero{}, std::integral_constant<int, NP>{});
-        } else if constexpr (WR == 2) {
-            if (wr == 0) request_part(p.k, p.k_bs, p.k_rs, p.k_hs, k_voff, dst, Zero{}, std::integral_constant<int, NP>{});
-            else request_part(p.v, p.v_bs, p.v_rs, p.v_hs, v_voff, dst + SLICEB, Zero{}, std::integral_constant<int, NP>{});
-        } else {
-            if (wr == 0) request_part(p.k, p.k_bs, p.k_rs, p.k_hs, k_voff, dst, Zero{}, std::integral_constant<int, NP / 2>{});
-            else if (wr == 1) request_part(p.k, p.k_bs, p.k_rs, p.k_hs, k_voff, dst, std::integral_constant<int, NP / 2>{}, std::integral_constant<int, NP / 2>{});
-            else if (wr == 2) request_part(p.v, p.v_bs, p.v_rs, p.v_hs, v_voff, dst + SLICEB, Zero{}, std::integral_constant<int, NP / 2>{});
-            else request_part(p.v, p.v_bs, p.v_rs, p.v_hs, v_voff, dst + SLICEB, std::integral_constant<int, NP / 2>{}, std::integral_constant<int, NP / 2>{});
-        }
+        const int u = wr >> 1;
+        const uint32_t dst = ring_addr + sl * SLOTB + (WR == 1 ? 0 : u * 2 * SLICEB);
+        request_slice(own, dst + (v_part ? SLICEB : 0), WR == 1 ? 0 : u);
+        if constexpr (WR == 1) request_slice(own_v, dst + SLICEB, 0);
         ++it_tile;
         ++it_t;
         if (it_tile == it_end && it_tile < tile_end) { ++it_s; seek(); }
     };
-    // WR = 1 asks for tile t + NS when its own slot is free, WR > 1 for tile t + NS - 1 behind the barrier of tile t
-    constexpr int AHEAD = WR == 1 ? NS : NS - 1;
+    // WR = 1 asks for tile t + NS when its own slot is free, WR = 2 for tile t + NS - 1 behind the barrier of tile t, the
+    // ping-pong for K of tile t + 2 and V of tile t + 1 in the vector phase of tile t
+    constexpr int AHEAD = WR == 1 || PP ? NS : NS - 1;
+    if constexpr (PP) {
+        static_assert(!PP || NS == 2, "two slots");
+        request(0);
+        if (!(wr & 1)) request(1);
+    } else {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) request(i);
+        for (int i = 0; i < AHEAD; ++i) request(i);
+    }
     int sl = 0;                                      // slot of the tile being consumed
 
     int k_off[KS];     // K row read: row r, chunk 2ks + h
@@ -273,10 +279,192 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
         }
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
+        // ---- the scores of this wave's slices of tile t (first key kb0) -> P
+        f32x16 x[SUB];
+        bf16x8 pf[SUB][2];     // P rounds to bf16, the matrix pipe's type; its sum is taken before the rounding
+        auto weigh = [&]() __attribute__((always_inline)) {      // P against the running maximum; its row sum (this lane's half)
+            const float mc = m_run * c;
+            float sum = 0.f;
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float pv = fast_exp2(__builtin_fmaf(x[u][i], c, -mc));
+                    sum += pv;
+                    pf[u][i >> 3][i & 7] = (__bf16)pv;
+                }
+            return sum;
+        };
+        auto softmax = [&](int kb0, bool masked) __attribute__((always_inline)) {
+            if constexpr (MOD != 0) {                // t (log2 units) from the raw products
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    const int jl = kb0 + WN * u + 4 * h;
+                    const float fq = (float)(len + my_depth - jl);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float dist = fq - (float)((i & 3) + 8 * (i >> 2));
+                        if constexpr ((MOD & LV_SCORE_BIAS) != 0)
+                            if (masked && p.parents) {       // a drafted key stands at its depth, not at its row
+                                const int j = jl + (i & 3) + 8 * (i >> 2) - len;
+                                if (j >= 0) dist = (float)(my_depth - depth[min(j, p.n - 1)]);
+                            }
+                        x[u][i] = lv_score<MOD>(x[u][i], p.scale_log2e, p.score, nslope2, dist);
+                    }
+                }
+            }
+            // Optimistic pass (see attn_fwd_pp.hip): with a finite running maximum P is formed against it without looking for
+            // the tile's own; a score far above it shows as a large sum and sends the tile through the exact pass.
+            bool exact = masked || __any(m_run < -1e29f);
+            if (!exact) {
+                const float sum = weigh();
+                if (__any(!(sum <= OPTIMISTIC_MAX))) exact = true;      // (also catches inf / nan)
+                else l_run += sum;
+            }
+            if (!exact) return;
+            if (masked) {
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    // bit e of `vis`: key kb0 + 32 u + e visible to this lane's token
+                    uint32_t vis;
+                    const int j0 = kb0 + WN * u - len;          // first key of the slice, counted from the first drafted one
+                    if (p.parents) {
+                        const uint32_t* aw = anc + token * words;
+                        const int lo = j0 >> 5;        // (arithmetic shift: below 0 for a slice that starts in the cache)
+                        const uint32_t a0 = lo < 0 ? 0xffffffffu : (lo < words ? aw[lo] : 0u);
+                        const uint32_t a1 = lo + 1 < 0 ? 0xffffffffu : (lo + 1 < words ? aw[lo + 1] : 0u);
+                        vis = (uint32_t)((((uint64_t)a1 << 32) | a0) >> (j0 & 31));
+                    } else {
+                        const int last = token - j0;   // keys up to the token's own
+                        vis = last >= 31 ? 0xffffffffu : (last < 0 ? 0u : (2u << last) - 1u);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int e = (i & 3) + 8 * (i >> 2) + 4 * h;
+                        x[u][i] = (vis >> e) & 1 ? x[u][i] : -INFINITY;
+                    }
+                }
+            }
+            float mx = x[0][0];
+#pragma unroll
+            for (int u = 0; u < SUB; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mx = fmaxf(mx, x[u][i]);
+            mx = pair32_max(mx);
+            const float m_new = fmaxf(m_run, mx);
+            const bool grow = (m_new - m_run) * c > RESCALE_LOG2;
+            if (__any(grow)) {
+                const float alpha = fast_exp2((m_run - m_new) * c);
+                m_run = m_new;
+                l_run *= alpha;
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) oacc[mt][i] *= alpha;
+            }
+            l_run += weigh();
+        };
+        // rows of unused slots hold whatever was there: zero, so that not even a NaN gets through P = 0 (every wave that shares
+        // the slice writes the same zeros before it reads)
+        auto blank_unused = [&](lds_char* vrows, int first) __attribute__((always_inline)) {
+            const int vrow = lane >> 1;
+            const int j = min(first + vrow, keys - 1) - len;
+            if (j >= 0 && par[j] == LV_TREE_UNUSED)
+#pragma unroll
+                for (int i = 0; i < CPR / 2; ++i)
+                    *(LDS_PTR(u32x4, vrows + vrow * ROWB + ((lane & 1) * (CPR / 2) + i) * 16)) = u32x4{0, 0, 0, 0};
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        };
+
+        if constexpr (PP) {
+            // Vector phase of tile t: softmax, requests.  Matrix phase: S of tile t + 1 and O^T += V_t^T P_t.  Key wave 1 runs one
+            // barrier behind key wave 0, so a SIMD has one of its two waves in each phase (see attn_fwd_pp.hip).
+            asm volatile("s_barrier" ::: "memory");          // (the counter is at zero: everyone's first K and V are there)
+#pragma unroll
+            for (int u = 0; u < SUB; ++u) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const bf16x8 kf = *(LDS_PTR(bf16x8, ring + sl * SLOTB + u * 2 * SLICEB + k_off[ks]));
+                    x[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], x[u], 0, 0, 0);
+                }
+            }
+            // every row wave has read its K of this tile before one of them asks for the tile that replaces it
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (wk == 1) asm volatile("s_barrier" ::: "memory");
+            for (int t = t0; t < t1; ++t) {
+                const int kb0 = t * BN + WN * SUB * wk;
+                const bool masked = kb0 + WN * SUB > len;
+                softmax(kb0, masked);
+                request((wr & 1) ? sl ^ 1 : sl);         // V of tile t + 1, K of tile t + 2
+                __builtin_amdgcn_sched_barrier(0);
+                // all but the newest requests have landed: K of tile t + 1, V of tile t
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(NPW) : "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                lds_char* const kb = ring + (sl ^ 1) * SLOTB;
+                lds_char* const vb = ring + sl * SLOTB;
+                if (masked && p.parents)
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u) blank_unused(vb + u * 2 * SLICEB + SLICEB, kb0 + WN * u);
+                __builtin_amdgcn_s_setprio(2);
+                // groups (u, s2) of MT products with V rows 16 s2 .. of slice u and KS / 2 steps of S[u]; the fragments of a group
+                // are read while the one before it runs
+                bf16x8 vfr[2][MT], kfr[2][KS / 2];
+                auto load_group = [&](int g, int set) __attribute__((always_inline)) {
+                    const int u = g >> 1, s2 = g & 1;
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt) {
+                        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, vb + v_off[mt][0] + u * 2 * SLICEB + 16 * s2 * ROWB));
+                        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, vb + v_off[mt][1] + u * 2 * SLICEB + 16 * s2 * ROWB));
+                        bf16x8& vf = vfr[set][mt];
+                        vf[0] = lo[0]; vf[1] = lo[1]; vf[2] = lo[2]; vf[3] = lo[3];
+                        vf[4] = hi[0]; vf[5] = hi[1]; vf[6] = hi[2]; vf[7] = hi[3];
+                    }
+#pragma unroll
+                    for (int kk = 0; kk < KS / 2; ++kk) kfr[set][kk] = *(LDS_PTR(bf16x8, kb + u * 2 * SLICEB + k_off[s2 * (KS / 2) + kk]));
+                };
+                constexpr int RPG = 2 * MT + KS / 2, MPG = MT + KS / 2;
+                static_assert(MT == KS / 2 && RPG * 2 == MPG * 3, "three reads per two products");
+                load_group(0, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, RPG, 0);
+#pragma unroll
+                for (int g4 = 0; g4 < 2 * SUB; ++g4) {
+                    const int u = g4 >> 1, s2 = g4 & 1, set = g4 & 1;
+                    if (g4 + 1 < 2 * SUB) load_group(g4 + 1, set ^ 1);
+                    if (s2 == 0) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {       // two accumulation targets in turn
+                        oacc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vfr[set][i], pf[u][s2], oacc[i], 0, 0, 0);
+                        x[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kfr[set][i], qf[s2 * (KS / 2) + i], x[u], 0, 0, 0);
+                    }
+                    if (g4 + 1 < 2 * SUB) {
+#pragma unroll
+                        for (int i = 0; i < MPG / 2; ++i) {
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                            __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+                        }
+                    } else {
+                        __builtin_amdgcn_sched_group_barrier(0x008, MPG, 0);
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(0);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                sl ^= 1;
+                ++tile;
+            }
+            if (wk == 0) asm volatile("s_barrier" ::: "memory");
+        } else {
         for (int t = t0; t < t1; ++t) {
-            const int kb0 = t * BN + WN * wk;
-            const bool some = kb0 < keys;            // this wave has keys of the tile
-            const bool masked = kb0 + WN > len;      // ... drafted ones, or rows past the end, among them
+            const int kb0 = t * BN + WN * SUB * wk;
+            const bool masked = kb0 + WN * SUB > len;      // drafted keys, or rows past the end, are among the wave's
             lds_char* const kb = ring + sl * SLOTB;
             if constexpr (WR == 1) {
                 // K of this tile: requested before its V and the NS - 1 tiles behind it
@@ -287,119 +475,41 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
                 asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * NPW) : "memory");
                 request(sl == 0 ? NS - 1 : sl - 1);
             }
-            f32x16 x;
-            bf16x8 pf[2];     // P rounds to bf16, the matrix pipe's type; its sum is taken before the rounding
 #pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = 0.f;
+            for (int u = 0; u < SUB; ++u)
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                const bf16x8 kf = *(LDS_PTR(bf16x8, kb + k_off[ks]));
-                x = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], x, 0, 0, 0);
-            }
-            if constexpr (MOD != 0) {                // t (log2 units) from the raw products
-                const int jl = kb0 + 4 * h;
-                const float fq = (float)(len + my_depth - jl);
+                for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    float dist = fq - (float)((i & 3) + 8 * (i >> 2));
-                    if constexpr ((MOD & LV_SCORE_BIAS) != 0)
-                        if (masked && p.parents) {       // a drafted key stands at its depth, not at its row
-                            const int j = jl + (i & 3) + 8 * (i >> 2) - len;
-                            if (j >= 0) dist = (float)(my_depth - depth[min(j, p.n - 1)]);
-                        }
-                    x[i] = lv_score<MOD>(x[i], p.scale_log2e, p.score, nslope2, dist);
+            for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+                for (int u = 0; u < SUB; ++u) {
+                    const bf16x8 kf = *(LDS_PTR(bf16x8, kb + u * 2 * SLICEB + k_off[ks]));
+                    x[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, qf[ks], x[u], 0, 0, 0);
                 }
-            }
-            // Optimistic pass (see attn_fwd_pp.hip): with a finite running maximum P is formed against it without looking for
-            // the tile's own; a score far above it shows as a large sum and sends the tile through the exact pass.
-            bool exact = masked || __any(m_run < -1e29f);
-            if (!exact) {
-                const float mc = m_run * c;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float pv = fast_exp2(__builtin_fmaf(x[i], c, -mc));
-                    sum += pv;
-                    pf[i >> 3][i & 7] = (__bf16)pv;
-                }
-                if (__any(!(sum <= OPTIMISTIC_MAX))) exact = true;      // (also catches inf / nan)
-                else l_run += sum;
-            }
-            if (exact) {
-                if (masked) {
-                    // bit e of `vis`: key kb0 + e visible to this lane's token
-                    uint32_t vis;
-                    const int j0 = kb0 - len;          // first key of the slice, counted from the first drafted one
-                    if (p.parents) {
-                        const uint32_t* aw = anc + token * words;
-                        const int lo = j0 >> 5;        // (arithmetic shift: -1 for a slice that starts in the cache)
-                        const uint32_t a0 = lo < 0 ? 0xffffffffu : (lo < words ? aw[lo] : 0u);
-                        const uint32_t a1 = lo + 1 < words ? aw[lo + 1] : 0u;
-                        vis = (uint32_t)((((uint64_t)a1 << 32) | a0) >> (j0 & 31));
-                    } else {
-                        const int last = token - j0;   // keys up to the token's own
-                        vis = last >= 31 ? 0xffffffffu : (last < 0 ? 0u : (2u << last) - 1u);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int e = (i & 3) + 8 * (i >> 2) + 4 * h;
-                        x[i] = (vis >> e) & 1 ? x[i] : -INFINITY;
-                    }
-                }
-                float mx = x[0];
-#pragma unroll
-                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
-                mx = pair32_max(mx);
-                const float m_new = fmaxf(m_run, mx);
-                const bool grow = (m_new - m_run) * c > RESCALE_LOG2;
-                if (__any(grow)) {
-                    const float alpha = fast_exp2((m_run - m_new) * c);
-                    m_run = m_new;
-                    l_run *= alpha;
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) oacc[mt][i] *= alpha;
-                }
-                const float mc = m_run * c;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float pv = fast_exp2(__builtin_fmaf(x[i], c, -mc));
-                    sum += pv;
-                    pf[i >> 3][i & 7] = (__bf16)pv;
-                }
-                l_run += sum;
-            }
+            softmax(kb0, masked);
             if constexpr (WR == 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((2 * NS - 2) * NP) : "memory");   // V of this tile
-            if (some) {
-                if (masked && p.parents) {
-                    // rows of unused slots hold whatever was there: zero, so that not even a NaN gets through P = 0 (every
-                    // wave that shares the slice writes the same zeros before it reads)
-                    const int vrow = lane >> 1;
-                    const int j = min(kb0 + vrow, keys - 1) - len;
-                    if (j >= 0 && par[j] == LV_TREE_UNUSED)
 #pragma unroll
-                        for (int i = 0; i < CPR / 2; ++i)
-                            *(LDS_PTR(u32x4, kb + SLICEB + vrow * ROWB + ((lane & 1) * (CPR / 2) + i) * 16)) = u32x4{0, 0, 0, 0};
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                }
+            for (int u = 0; u < SUB; ++u) {
+                if (kb0 + WN * u >= keys) continue;            // (nothing was brought for a slice without keys)
+                lds_char* const vb = kb + u * 2 * SLICEB;
+                if (masked && p.parents) blank_unused(vb + SLICEB, kb0 + WN * u);
 #pragma unroll
                 for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, kb + v_off[mt][0] + 16 * s2 * ROWB));
-                        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, kb + v_off[mt][1] + 16 * s2 * ROWB));
+                        const bf16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, vb + v_off[mt][0] + 16 * s2 * ROWB));
+                        const bf16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(LDS_PTR(bf16x4, vb + v_off[mt][1] + 16 * s2 * ROWB));
                         bf16x8 vf;
                         vf[0] = lo[0]; vf[1] = lo[1]; vf[2] = lo[2]; vf[3] = lo[3];
                         vf[4] = hi[0]; vf[5] = hi[1]; vf[6] = hi[2]; vf[7] = hi[3];
-                        oacc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[s2], oacc[mt], 0, 0, 0);
+                        oacc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, pf[u][s2], oacc[mt], 0, 0, 0);
                     }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave is done with the slot
             if constexpr (WR == 1) request(sl);
             sl = sl + 1 == NS ? 0 : sl + 1;
             ++tile;
+        }
         }
 
         // ---------------- join the key waves; this share's result for the sequence -> partial slot g + s ----------------
@@ -531,8 +641,7 @@ static TreePlan tree_plan(int batch, int n, int rows, int hq, int hkv) {
     const int n_rows = n * (hq / hkv);
     t.wr = n_rows <= 32 ? 1 : (n_rows <= 64 ? 2 : 4);
     t.n_rb = (n_rows + 32 * t.wr - 1) / (32 * t.wr);
-    const int tile = t.wr == 4 ? TreeShape<4>::TILE : TreeShape<1>::TILE;
-    const int64_t tiles = (int64_t)batch * ((rows + tile - 1) / tile);
+    const int64_t tiles = (int64_t)batch * ((rows + 127) / 128);
     int64_t g = 256 / ((int64_t)hkv * t.n_rb);
     if (g > tiles) g = tiles;
     if (g < 1) g = 1;
@@ -545,8 +654,7 @@ static TreePlan tree_plan(int batch, int n, int rows, int hq, int hkv) {
 template <int D, int WR>
 static void launch_tree(const TreeParams& p, int mod, unsigned blocks, int64_t out_rows, hipStream_t stream) {
     const dim3 grid(blocks), block(TreeShape<WR>::THREADS);
-    constexpr int slot = TreeShape<WR>::WK * 2 * 32 * D * 2;
-    constexpr size_t lds = (size_t)(LV_TREE_RING / slot > 4 ? 4 : LV_TREE_RING / slot) * slot + LV_TREE_LDS_FIXED;
+    constexpr size_t lds = TreeShape<WR>::template lds_bytes<D>();
     static_assert(lds <= 160 * 1024, "one workgroup per compute unit");
     switch (mod) {
         case 0: hipLaunchKernelGGL((lv_tree_kernel<D, WR, 0>), grid, block, lds, stream, p); break;
