@@ -13,8 +13,7 @@
 // cache's bytes, many (row blocks of 128, side by side on one XCD's L2) by the matrix and vector pipes.
 //
 // The keys of ALL sequences form one list of tiles, dealt evenly to G workgroups per KV head: a workgroup's share may begin
-// inside one sequence and end inside another, so ragged lengths leave no compute unit waiting, and the requests run on into
-// the next sequence.  A share's result for a sequence goes to partial slot g + s (the pairs (g, s) along the list only ever
+// inside one sequence and end inside another, so ragged lengths leave no compute unit waiting.  A share's result for a sequence goes to partial slot g + s (the pairs (g, s) along the list only ever
 // step forward, so the sum is unique) and a second kernel joins a sequence's slots in order.
 #include "internal.h"
 #include "../../include/lvattn.h"
@@ -60,6 +59,17 @@ __device__ __forceinline__ void tree_scan(const TreeParams& p, int* cum, int* le
     __syncthreads();
 }
 
+// The list dealt to the shares: `total` tiles, the first total % G shares one more than the rest.
+struct TreeDeal {
+    uint32_t G, each, extra;
+    __device__ TreeDeal(uint32_t shares, uint32_t total) : G(min(shares, total)), each(total / G), extra(total - each * G) {}
+    __device__ int first(uint32_t g) const { return (int)(g * each + min(g, extra)); }
+    __device__ int share_of(uint32_t tile) const {
+        const uint32_t head = extra * (each + 1);
+        return (int)(tile < head ? tile / (each + 1) : extra + (tile - head) / each);
+    }
+};
+
 // Direct global -> LDS load, 16 bytes per lane, lane i -> LDS byte lds_dst + 16 i (M0 carries lds_dst; nothing else in this
 // file uses M0, so it is not restored).  As asm so that the
 // compiler does not count it; completion is waited for by hand.
@@ -67,8 +77,8 @@ __device__ __forceinline__ void tree_dma16(__amdgpu_buffer_rsrc_t rs, int voff, 
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "s"(lds_dst) : "memory");
 }
 
-// [slots of K / V tiles][cum][lens][par][depth][anc][stat][obuf]
-#define LV_TREE_LDS_FIXED (LV_TREE_MAX_BATCH * 8 + LV_TREE_MAX_TOKENS * 8 + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4 + 2048 + 16384)
+// [slots of K / V tiles][cum][lens][par][depth][anc][stat]
+#define LV_TREE_LDS_FIXED (LV_TREE_MAX_BATCH * 8 + LV_TREE_MAX_TOKENS * 8 + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4 + 2048)
 #define LV_TREE_RING (128 * 1024)
 
 template <int WR>
@@ -113,7 +123,8 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
     int* const depth = par + LV_TREE_MAX_TOKENS;                        // [LV_TREE_MAX_TOKENS]
     uint32_t* const anc = reinterpret_cast<uint32_t*>(depth + LV_TREE_MAX_TOKENS);   // [tokens][words]: a token and its ancestors
     float* const stat = reinterpret_cast<float*>(anc + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32));   // [2][8 waves][32]
-    float* const obuf = stat + 512;                                     // [8 waves][64 lanes][8]: 16 KB
+    f32x4* const obuf = reinterpret_cast<f32x4*>(smem);                 // the join's buffer is the ring: [wave][MT][4][lane]
+    static_assert(NS * SLOTB >= NW * MT * 4096, "the join fits the ring");
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -131,22 +142,15 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
     const int kvh = unit % p.hkv, g = unit / p.hkv;
 
     tree_scan<BN>(p, cum, lens);
-    const int64_t total = __builtin_amdgcn_readfirstlane(cum[p.batch - 1]);
-    const int64_t G = min((int64_t)p.shares, total);
-    if (g >= G) return;
-    int tile = (int)(g * total / G);
-    const int tile_end = (int)((g + 1) * total / G);
+    const TreeDeal deal(p.shares, __builtin_amdgcn_readfirstlane(cum[p.batch - 1]));
+    if (g >= (int)deal.G) return;
+    int tile = __builtin_amdgcn_readfirstlane(deal.first(g));
+    const int tile_end = __builtin_amdgcn_readfirstlane(deal.first(g + 1));
     int s = 0;
     while (__builtin_amdgcn_readfirstlane(cum[s]) <= tile) ++s;
 
-    // ---- requests: this wave's part (NPW requests, K or V rows) of its key slice, tile after tile
-    int it_tile = tile, it_s = s, it_t, it_len, it_end;      // list position, sequence, tile and length of the sequence, its list end
-    auto seek = [&]() __attribute__((always_inline)) {
-        it_t = it_tile - (it_s ? __builtin_amdgcn_readfirstlane(cum[it_s - 1]) : 0);
-        it_len = __builtin_amdgcn_readfirstlane(lens[it_s]);
-        it_end = __builtin_amdgcn_readfirstlane(cum[it_s]);
-    };
-    seek();
+    // ---- requests: this wave's part (NPW requests, K or V rows) of its key slice, tile after tile of the sequence at hand
+    int rq_s = 0, rq_t = 0, rq_t1 = 0, rq_keys = 0;      // sequence, next tile to ask for, the share's last of it, keys
     lds_char* const ring = (lds_char*)smem + wk * SUB * 2 * SLICEB;     // this wave's slices in slot 0
     const uint32_t ring_addr = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)ring);
     // one operand's rows as this wave asks for them: position -> chunk of the LDS image (the swizzle is an involution and
@@ -164,13 +168,13 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
     const Rows own = rows_of(v_part ? p.v : p.k, v_part ? p.v_bs : p.k_bs, v_part ? p.v_rs : p.k_rs, v_part ? p.v_hs : p.k_hs);
     const Rows own_v = WR == 1 ? rows_of(p.v, p.v_bs, p.v_rs, p.v_hs) : own;
     auto request_slice = [&](const Rows& x, uint32_t dst, int u) __attribute__((always_inline)) {
-        int first = it_t * BN + WN * (wk * SUB + u);
+        int first = rq_t * BN + WN * (wk * SUB + u);
         // (ping-pong multiplies every slice: one behind the last key repeats it)
-        if constexpr (PP) first = min(first, it_len + p.n - 1);
-        const int valid = it_tile < tile_end ? min(it_len + p.n - first, WN) : 0;
+        if constexpr (PP) first = min(first, rq_keys - 1);
+        const int valid = rq_t < rq_t1 ? min(rq_keys - first, WN) : 0;
         // nothing to bring: zero records, every lane out of range
         const uint32_t rec = valid > 0 ? (uint32_t)((valid - 1) * x.rs * 2 + ROWB) : 0u;
-        const __bf16* src = x.base + (valid > 0 ? (int64_t)it_s * x.bs + (int64_t)first * x.rs : 0);
+        const __bf16* src = x.base + (valid > 0 ? (int64_t)rq_s * x.bs + (int64_t)first * x.rs : 0);
         auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(src), 0, rec, 0x00020000);
         const int rs2 = (int)(x.rs * 2);
         if (valid <= 0 || valid >= WN) {
@@ -188,22 +192,8 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
         const uint32_t dst = ring_addr + sl * SLOTB + (WR == 1 ? 0 : u * 2 * SLICEB);
         request_slice(own, dst + (v_part ? SLICEB : 0), WR == 1 ? 0 : u);
         if constexpr (WR == 1) request_slice(own_v, dst + SLICEB, 0);
-        ++it_tile;
-        ++it_t;
-        if (it_tile == it_end && it_tile < tile_end) { ++it_s; seek(); }
+        ++rq_t;
     };
-    // WR = 1 asks for tile t + NS when its own slot is free, WR = 2 for tile t + NS - 1 behind the barrier of tile t, the
-    // ping-pong for K of tile t + 2 and V of tile t + 1 in the vector phase of tile t
-    constexpr int AHEAD = WR == 1 || PP ? NS : NS - 1;
-    if constexpr (PP) {
-        static_assert(!PP || NS == 2, "two slots");
-        request(0);
-        if (!(wr & 1)) request(1);
-    } else {
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) request(i);
-    }
-    int sl = 0;                                      // slot of the tile being consumed
 
     int k_off[KS];     // K row read: row r, chunk 2ks + h
 #pragma unroll
@@ -231,6 +221,22 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
         const int list0 = s ? __builtin_amdgcn_readfirstlane(cum[s - 1]) : 0;
         const int t0 = tile - list0, t1 = min(tile_end, __builtin_amdgcn_readfirstlane(cum[s])) - list0;
         const bool sees_tree = t1 * BN > len;
+
+        // WR = 1 asks for tile t + NS when its own slot is free, WR = 2 for tile t + NS - 1 behind the barrier of tile t, the
+        // ping-pong for K of tile t + 2 and V of tile t + 1 in the vector phase of tile t
+        rq_s = s;
+        rq_t = t0;
+        rq_t1 = t1;
+        rq_keys = keys;
+        int sl = 0;                       // slot of the tile being consumed
+        if constexpr (PP) {
+            static_assert(!PP || NS == 2, "two slots");
+            request(0);
+            if (!v_part) request(1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < (WR == 1 ? NS : NS - 1); ++i) request(i);
+        }
 
         bf16x8 qf[KS];
         const __bf16* qptr = p.q + (int64_t)s * p.q_bs + (int64_t)token * p.q_ns + (int64_t)head * p.q_hs + 8 * h;
@@ -520,6 +526,9 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
             stat[w * 32 + r] = m_run;
             stat[256 + w * 32 + r] = l_w;
         }
+        // (what was asked for past the share's last tile of the sequence brings nothing, but has to be over before the ring is
+        // written by hand)
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         float m_tot = -1e30f, l_tot = 0.f;
 #pragma unroll
@@ -529,32 +538,25 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
         const float sc = fast_exp2((m_run - m_tot) * c);
         const float inv = (l_tot > 0.f && live) ? 1.f / l_tot : 0.f;
         if (wk == 0 && h == 0) p.part_lse[part + r] = (l_tot > 0.f && live) ? m_tot * unit2 + __logf(l_tot) : -INFINITY;
-        // eight accumulators of a lane at a time: [wave][4-float half][lane]; key wave wk then finishes 8 / WK of them
-        typedef __attribute__((ext_vector_type(8 / WK))) float fpart;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
+            for (int g4 = 0; g4 < 4; ++g4)
+                obuf[((w * MT + mt) * 4 + g4) * 64 + lane] = f32x4{oacc[mt][4 * g4] * sc, oacc[mt][4 * g4 + 1] * sc, oacc[mt][4 * g4 + 2] * sc, oacc[mt][4 * g4 + 3] * sc};
+        __syncthreads();
 #pragma unroll
-                for (int x4 = 0; x4 < 2; ++x4) {
-                    const int i = 8 * hf + 4 * x4;
-                    *reinterpret_cast<f32x4*>(obuf + ((w * 2 + x4) * 64 + lane) * 4) =
-                        f32x4{oacc[mt][i] * sc, oacc[mt][i + 1] * sc, oacc[mt][i + 2] * sc, oacc[mt][i + 3] * sc};
-                }
-                __syncthreads();
-                const int e0 = wk * (8 / WK);             // first of this wave's floats: half e0 / 4, place e0 % 4
-                fpart acc = {};
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int i = 0; i < WK; ++i) acc += *reinterpret_cast<const fpart*>(obuf + (((i * WR + wr) * 2 + e0 / 4) * 64 + lane) * 4 + e0 % 4);
+            for (int e = 0; e < 4 / WK; ++e) {        // key wave wk finishes 16 / WK of a lane's accumulators
+                const int g4 = wk * (4 / WK) + e;
+                f32x4 acc = obuf[((wr * MT + mt) * 4 + g4) * 64 + lane];
 #pragma unroll
-                for (int e = 0; e < 8 / WK; ++e) acc[e] = inv > 0.f ? acc[e] * inv : 0.f;
-                *reinterpret_cast<fpart*>(p.part_o + (part + r) * D + 32 * mt + 8 * (2 * hf + e0 / 4) + 4 * h + e0 % 4) = acc;
-                __syncthreads();
+                for (int i = 1; i < WK; ++i) acc += obuf[(((i * WR + wr) * MT + mt) * 4 + g4) * 64 + lane];
+                *reinterpret_cast<f32x4*>(p.part_o + (part + r) * D + 32 * mt + 8 * g4 + 4 * h) = inv > 0.f ? acc * inv : f32x4{0.f, 0.f, 0.f, 0.f};
             }
+        __syncthreads();                  // the next sequence's requests go where obuf is
         ++s;
     }
-    // no request may outlive the workgroup: its LDS could already belong to another one
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
 // out / lse of a row = the log-sum-exp merge of its sequence's slots; every sum has a fixed order.  D / 4 threads take a slot's
@@ -570,18 +572,15 @@ __global__ __launch_bounds__(256) void lv_tree_join_kernel(TreeParams p) {
     __shared__ f32x4 osum[GR][TPR];
     const int tid = threadIdx.x, gr = tid / TPR, col = tid % TPR * 4;
     tree_scan<TreeShape<WR>::TILE>(p, cum, nullptr);
-    const int64_t total = cum[p.batch - 1];
-    const int64_t G = min((int64_t)p.shares, total);
+    const TreeDeal deal(p.shares, cum[p.batch - 1]);
     const int n_rows = p.n * p.group;
     const int64_t idx = ONE_ROW ? blockIdx.x : (int64_t)blockIdx.x * GR + gr;     // (sequence, KV head, row)
     if (idx >= (int64_t)p.batch * p.hkv * n_rows) return;
-    const int row = (int)(idx % n_rows), kvh = (int)(idx / n_rows % p.hkv), s = (int)(idx / n_rows / p.hkv);
-    const int64_t first = s ? cum[s - 1] : 0, last = cum[s] - 1;
-    // share that holds tile t: the largest g with floor(g total / G) <= t
-    const int64_t g0 = ((first + 1) * G - 1) / total, g1 = ((last + 1) * G - 1) / total;
+    const int row = (int)((uint32_t)idx % n_rows), unit = (int)((uint32_t)idx / n_rows), kvh = unit % p.hkv, s = unit / p.hkv;
+    const int g0 = deal.share_of(s ? cum[s - 1] : 0), g1 = deal.share_of(cum[s] - 1);
     const int rb = row / rows_pb;
     const int64_t part = ((int64_t)(kvh * p.n_rb + rb) * p.slots + g0 + s) * rows_pb + row % rows_pb;
-    const int np = (int)(g1 - g0 + 1);        // at most shares
+    const int np = g1 - g0 + 1;               // at most shares
     const float* lp = p.part_lse + part;
     const float* po = p.part_o + part * D + col;
     float m = -INFINITY, tot = 0.f;
@@ -663,8 +662,9 @@ static void launch_tree(const TreeParams& p, int mod, unsigned blocks, int64_t o
         default: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_CAP | LV_SCORE_BIAS>), grid, block, lds, stream, p);
     }
     if (hipPeekAtLastError() != hipSuccess) return;   // (reported by the caller)
-    // a group of threads walks its row's slots one after the other: worth it while there are few
-    if (p.shares > 32) hipLaunchKernelGGL((lv_tree_join_kernel<D, WR, true>), dim3((unsigned)out_rows), dim3(256), 0, stream, p);
+    // a workgroup per row takes the slots side by side; with more rows than the chip holds at once (eight workgroups to a compute
+    // unit) a group of threads walks its row's slots instead, eight or sixteen rows to a workgroup
+    if (out_rows <= 2048) hipLaunchKernelGGL((lv_tree_join_kernel<D, WR, true>), dim3((unsigned)out_rows), dim3(256), 0, stream, p);
     else hipLaunchKernelGGL((lv_tree_join_kernel<D, WR, false>), dim3((unsigned)((out_rows * (D / 4) + 255) / 256)), dim3(256), 0, stream, p);
 }
 
@@ -693,7 +693,8 @@ extern "C" int lvattn_tree(const void* q, const void* k, const void* v, void* ou
     if (workspace_bytes < need) return lv_fail(LV_ESIZE, "lvattn_tree: %lld bytes of workspace needed, room for %lld", (long long)need, (long long)workspace_bytes);
     const int64_t units = (int64_t)hkv * t.shares, blocks = (units + 7) / 8 * 8 * t.n_rb;
     const int64_t join = (int64_t)batch * hkv * n * (hq / hkv);
-    if (blocks > 0x7fffffffLL || join > 0x7fffffffLL) return lv_fail(LV_EINVAL, "lvattn_tree: grid too large");
+    if (blocks > 0x7fffffffLL || join > 0x7fffffffLL || (int64_t)batch * (rows / 128 + 1) > 0x7fffffffLL)
+        return lv_fail(LV_EINVAL, "lvattn_tree: grid too large");
     TreeParams p{};
     p.q = (const __bf16*)q; p.k = (const __bf16*)k; p.v = (const __bf16*)v; p.o = (__bf16*)out; p.lse = lse;
     p.cache_lens = cache_lens; p.parents = parents; p.parents_bs = parents_batch_stride;
