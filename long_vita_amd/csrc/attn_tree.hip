@@ -15,67 +15,10 @@
 // The keys of ALL sequences form one list of tiles, dealt evenly to G workgroups per KV head: a workgroup's share may begin
 // inside one sequence and end inside another, so ragged lengths leave no compute unit waiting.  A share's result for a sequence goes to partial slot g + s (the pairs (g, s) along the list only ever
 // step forward, so the sum is unique) and a second kernel joins a sequence's slots in order.
-#include "internal.h"
+#include "cache_list.h"
 #include "../../include/lvattn.h"
 
 #include <type_traits>
-
-typedef __attribute__((address_space(3))) char lds_char;
-
-template <int D>
-__device__ __forceinline__ int lds_off_tree(int row, int chunk) {
-    if constexpr (D == 128) return lds_off128(row, chunk);
-    else return lds_off64(row, chunk);
-}
-
-#define LV_TREE_UNUSED (-2)   // parents[] entry of a slot that holds no token
-
-__device__ __forceinline__ int tree_len(const TreeParams& p, int s) {
-    const int len = p.cache_lens[s];
-    return min(max(len, 0), p.rows - p.n);   // never outside the cache, whatever the caller's array says
-}
-
-// cum[s] = tiles of sequences 0 .. s, lens[s] (one wave); returns after a barrier of the whole workgroup
-template <int BN>
-__device__ __forceinline__ void tree_scan(const TreeParams& p, int* cum, int* lens) {
-    if (threadIdx.x < 64) {
-        const int lane = threadIdx.x;
-        int carry = 0;
-        for (int s0 = 0; s0 < p.batch; s0 += 64) {
-            const int len = s0 + lane < p.batch ? tree_len(p, s0 + lane) : 0;
-            int x = s0 + lane < p.batch ? (len + p.n + BN - 1) / BN : 0;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const int y = __shfl_up(x, off);
-                if (lane >= off) x += y;
-            }
-            if (s0 + lane < p.batch) {
-                cum[s0 + lane] = carry + x;
-                if (lens) lens[s0 + lane] = len;
-            }
-            carry += __shfl(x, 63);
-        }
-    }
-    __syncthreads();
-}
-
-// The list dealt to the shares: `total` tiles, the first total % G shares one more than the rest.
-struct TreeDeal {
-    uint32_t G, each, extra;
-    __device__ TreeDeal(uint32_t shares, uint32_t total) : G(min(shares, total)), each(total / G), extra(total - each * G) {}
-    __device__ int first(uint32_t g) const { return (int)(g * each + min(g, extra)); }
-    __device__ int share_of(uint32_t tile) const {
-        const uint32_t head = extra * (each + 1);
-        return (int)(tile < head ? tile / (each + 1) : extra + (tile - head) / each);
-    }
-};
-
-// Direct global -> LDS load, 16 bytes per lane, lane i -> LDS byte lds_dst + 16 i (M0 carries lds_dst; nothing else in this
-// file uses M0, so it is not restored).  As asm so that the
-// compiler does not count it; completion is waited for by hand.
-__device__ __forceinline__ void tree_dma16(__amdgpu_buffer_rsrc_t rs, int voff, uint32_t lds_dst) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rs), "s"(lds_dst) : "memory");
-}
 
 // [slots of K / V tiles][cum][lens][par][depth][anc][stat]
 #define LV_TREE_LDS_FIXED (LV_TREE_MAX_BATCH * 8 + LV_TREE_MAX_TOKENS * 8 + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4 + 2048)
@@ -141,8 +84,8 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
     if (unit >= p.hkv * p.shares) return;
     const int kvh = unit % p.hkv, g = unit / p.hkv;
 
-    tree_scan<BN>(p, cum, lens);
-    const TreeDeal deal(p.shares, __builtin_amdgcn_readfirstlane(cum[p.batch - 1]));
+    list_scan<BN>(p.cache_lens, p.batch, p.rows, p.n, cum, lens);
+    const ListDeal deal(p.shares, __builtin_amdgcn_readfirstlane(cum[p.batch - 1]));
     if (g >= (int)deal.G) return;
     int tile = __builtin_amdgcn_readfirstlane(deal.first(g));
     const int tile_end = __builtin_amdgcn_readfirstlane(deal.first(g + 1));
@@ -161,7 +104,7 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
         Rows x{base + (int64_t)kvh * hs, bs, rs, {}};
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-            x.voff[j] = lane / CPR * (int)(rs * 2) + lds_off_tree<D>(RPP * j + lane / CPR, lane % CPR) - (RPP * j + lane / CPR) * ROWB;
+            x.voff[j] = lane / CPR * (int)(rs * 2) + list_lds_off<D>(RPP * j + lane / CPR, lane % CPR) - (RPP * j + lane / CPR) * ROWB;
         return x;
     };
     const bool v_part = WR > 1 && (wr & 1);          // WR > 1: even row waves bring K, odd ones V
@@ -179,11 +122,11 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
         const int rs2 = (int)(x.rs * 2);
         if (valid <= 0 || valid >= WN) {
 #pragma unroll
-            for (int j = 0; j < NP; ++j) tree_dma16(rsrc, x.voff[j % NV] + RPP * j * rs2, dst + j * 1024);
+            for (int j = 0; j < NP; ++j) list_dma16(rsrc, x.voff[j % NV] + RPP * j * rs2, dst + j * 1024);
         } else {                                     // rows past the last key repeat it: never bytes that are no key's
             const int lr = lane / CPR;
 #pragma unroll
-            for (int j = 0; j < NP; ++j) tree_dma16(rsrc, x.voff[j % NV] + (min(RPP * j + lr, valid - 1) - lr) * rs2, dst + j * 1024);
+            for (int j = 0; j < NP; ++j) list_dma16(rsrc, x.voff[j % NV] + (min(RPP * j + lr, valid - 1) - lr) * rs2, dst + j * 1024);
         }
     };
     static_assert(WR == 1 ? SUB == 1 : 2 * SUB == WR, "WR > 1: every wave brings one slice's K or V rows");
@@ -197,14 +140,14 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
 
     int k_off[KS];     // K row read: row r, chunk 2ks + h
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) k_off[ks] = lds_off_tree<D>(r, 2 * ks + h);
+    for (int ks = 0; ks < KS; ++ks) k_off[ks] = list_lds_off<D>(r, 2 * ks + h);
     const int i16 = lane & 15, q4 = i16 >> 2, p4 = i16 & 3, gl = (lane >> 4) & 1;
     int v_off[MT][2];  // V transposed read
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int jh = 0; jh < 2; ++jh)
-            v_off[mt][jh] = SLICEB + lds_off_tree<D>(8 * jh + 4 * h + q4, 4 * mt + 2 * gl + (p4 >> 1)) + 8 * (p4 & 1);
+            v_off[mt][jh] = SLICEB + list_lds_off<D>(8 * jh + 4 * h + q4, 4 * mt + 2 * gl + (p4 >> 1)) + 8 * (p4 & 1);
 
     // this lane's query row: row -> (token, head of the group)
     const int n_rows = p.n * p.group;
@@ -246,26 +189,7 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
         int my_depth = token;             // without parents the tokens are a chain
         bool live = row < n_rows;
         if (p.parents) {
-            const int* pp = p.parents + (int64_t)s * p.parents_bs;
-            __syncthreads();              // the previous sequence's arrays are no longer read
-            for (int i = tid; i < p.n; i += NT) {
-                const int x = pp[i];
-                par[i] = x < i ? x : -1;  // a parent stands before its child: the walk below always ends
-            }
-            __syncthreads();
-            for (int i = tid; i < p.n; i += NT) {
-                if (sees_tree)
-                    for (int x = 0; x < words; ++x) anc[i * words + x] = 0;
-                int dep = -1, at = i;
-                if (par[i] != LV_TREE_UNUSED)
-                    while (at >= 0) {
-                        if (sees_tree) anc[i * words + (at >> 5)] |= 1u << (at & 31);
-                        ++dep;
-                        at = par[at];
-                    }
-                depth[i] = max(dep, 0);
-            }
-            __syncthreads();
+            list_tree(p.parents + (int64_t)s * p.parents_bs, p.n, words, sees_tree, par, depth, anc, tid, NT);
             my_depth = depth[token];
             live = live && par[token] != LV_TREE_UNUSED;
         }
@@ -571,8 +495,8 @@ __global__ __launch_bounds__(256) void lv_tree_join_kernel(TreeParams p) {
     __shared__ float red[8];
     __shared__ f32x4 osum[GR][TPR];
     const int tid = threadIdx.x, gr = tid / TPR, col = tid % TPR * 4;
-    tree_scan<TreeShape<WR>::TILE>(p, cum, nullptr);
-    const TreeDeal deal(p.shares, cum[p.batch - 1]);
+    list_scan<TreeShape<WR>::TILE>(p.cache_lens, p.batch, p.rows, p.n, cum, nullptr);
+    const ListDeal deal(p.shares, cum[p.batch - 1]);
     const int n_rows = p.n * p.group;
     const int64_t idx = ONE_ROW ? blockIdx.x : (int64_t)blockIdx.x * GR + gr;     // (sequence, KV head, row)
     if (idx >= (int64_t)p.batch * p.hkv * n_rows) return;

@@ -3,49 +3,289 @@
 //   w_out[kvh, j] = w_in[kvh, j] + sum over tokens i and query heads h of kvh's group of rho_i exp(t_ij - lse_ih)
 //
 // t and the visible keys are those of attn_tree.hip, lse comes from the attention itself, rho is an optional weight per token
-// (0 for drafted tokens that were not accepted).  One product, S = Q K^T, with the KEY on the lane (32x32x16 MFMA, A = query
-// rows from LDS, B = keys): a wave keeps the fragments of its 64 keys in registers for the whole kernel, so K is read once,
-// and a key's sum over a tile of query rows is a sum over its lane's 16 accumulators.  Nothing is ever summed by atomics.
+// (0 for drafted tokens that were not accepted); it enters as log2(rho) beside lse, so it costs nothing per score.  One product,
+// S = Q K^T, with the KEY on the lane (32x32x16 MFMA, A = query rows, B = keys): a key's sum over 32 query rows is a sum over
+// its lane's 16 accumulators.  Nothing is ever summed by atomics.  Two kernels:
 //
-// A workgroup is 4 waves: 4 / RW over keys, RW over alternate tiles of 32 query rows (few rows: one tile, all waves on keys;
-// a whole prompt's rows: two).  When there are fewer key blocks than the chip has room for, the rows are cut into pieces
-// whose sums go to a workspace and are added in order.  Few rows: bound by K's bytes.  Many: 8 MFMAs (256 cycles) against 16
-// exponentials, multiply-adds and adds per 32 x 32 scores, so the vector work bounds it.
-#include "internal.h"
+// - up to 64 query rows per KV head (a decode step, a small tree): bound by K's bytes.  The query fragments and the rows'
+//   constants stay in registers, eight waves per workgroup stream K, each its own 32-key slices through its own LDS slots by
+//   direct global -> LDS loads, without a barrier; tiles of all sequences are dealt evenly (cache_list.h).  The old weight of a
+//   key travels with its slice, so w_out is written on the spot.
+// - more rows (a large tree, a prompt): a workgroup holds the fragments of 128 keys in registers and the query rows stream
+//   through an LDS ring of 64-row tiles shared by its four waves, two on each half of the keys, on alternate 32 rows.  A
+//   first small kernel prepares the rows' constants.  When there are fewer key blocks than the chip has room for, the rows
+//   are cut into pieces whose sums are added in order by a last kernel.  8 MFMAs (256 cycles) stand against 16 exponentials,
+//   multiply-adds and adds per 32 x 32 scores, so the vector work bounds it.
+#include "cache_list.h"
 #include "../../include/lvattn.h"
 
-typedef __attribute__((address_space(3))) char lds_char;
-
-template <int D>
-__device__ __forceinline__ int lds_off_w(int row, int chunk) {
-    if constexpr (D == 128) return lds_off128(row, chunk);
-    else return lds_off64(row, chunk);
+// Direct global -> LDS load of one float per lane: lane i -> LDS byte lds_dst + 4 i
+__device__ __forceinline__ void weight_dma4(const float* g, uint32_t lds_dst) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_dst) : "memory");
 }
 
-template <int D, int MOD, int RW>
-__global__ __launch_bounds__(256, 2) void lv_key_weights_kernel(WeightParams p) {
-    constexpr int KWAVES = 4 / RW;
-    constexpr int KB = 64 * KWAVES;       // keys per workgroup
-    constexpr int KS = D / 16;
-    constexpr int CPR = D / 8;
-    constexpr int ROWB = D * 2;
-    constexpr int TR = 32 * RW;           // query rows per step
-    constexpr int NLD = TR * CPR / 256;   // 16-byte chunks per thread and step
-    static_assert(TR * CPR % 256 == 0, "whole chunks per thread");
+// log2(rho) - lse log2(e) of a row: what its scores' exponents start from; -inf for a row that counts for nothing
+__device__ __forceinline__ float row_constant(const WeightParams& p, int s, int token, int head) {
+    const float rho = p.row_weight ? p.row_weight[(int64_t)s * p.n + token] : 1.f;
+    const float l = p.lse[((int64_t)s * p.n + token) * p.hq + head];
+    if (!(rho > 0.f) || !(l > -INFINITY)) return -INFINITY;
+    return (p.row_weight ? __builtin_amdgcn_logf(rho) : 0.f) - l * 1.4426950408889634f;
+}
 
-    __shared__ __attribute__((aligned(16))) char qbuf[2][TR * ROWB];
-    __shared__ __attribute__((aligned(16))) float cst[2][TR];     // log2(rho) - lse log2(e); -inf: the row counts for nothing
-    __shared__ __attribute__((aligned(16))) float rpos[2][TR];    // position of the row's token, counted from the cache's start
-    __shared__ __attribute__((aligned(16))) float rslope[2][TR];  // -log2(e) slope of the row's head
-    __shared__ int rtok[2][TR];
-    __shared__ float red[RW > 1 ? (RW - 1) * KB : 1];
-    __shared__ int par[LV_TREE_MAX_TOKENS], depth[LV_TREE_MAX_TOKENS];
-    __shared__ uint32_t anc[LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32)];
+// ---------------------------------------------------------------------------
+// up to 32 RT query rows
+// ---------------------------------------------------------------------------
+#define LV_WEIGHT_TILE 256                    // keys per tile: 32 for each of eight waves
+template <int D> constexpr int weight_slots() { return D == 128 ? 2 : 4; }
+template <int D> constexpr int weight_slot_bytes() { return 32 * D * 2 + 256; }        // a slice of K, the 32 old weights
+template <int D> constexpr int weight_lds_bytes() {
+    return 8 * weight_slots<D>() * weight_slot_bytes<D>() + LV_TREE_MAX_BATCH * 8 + LV_TREE_MAX_TOKENS * 8 + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4 + 4 * 64 * 4;
+}
+
+template <int D, int RT, int MOD>
+__global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p) {
+    constexpr int KS = D / 16;
+    constexpr int ROWB = D * 2;
+    constexpr int CPR = D / 8;
+    constexpr int RPP = 64 / CPR;             // rows per 1-KiB request
+    constexpr int NP = 32 * ROWB / 1024;      // K requests per slice: 8 (d = 128) or 4
+    constexpr int NV = 16 / RPP;
+    constexpr int NS = weight_slots<D>();
+    constexpr int SLOTB = weight_slot_bytes<D>();
+    constexpr int BN = LV_WEIGHT_TILE;
+
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    int* const cum = reinterpret_cast<int*>(smem + 8 * NS * SLOTB);     // [LV_TREE_MAX_BATCH]
+    int* const lens = cum + LV_TREE_MAX_BATCH;
+    int* const par = lens + LV_TREE_MAX_BATCH;                          // [LV_TREE_MAX_TOKENS]
+    int* const depth = par + LV_TREE_MAX_TOKENS;
+    uint32_t* const anc = reinterpret_cast<uint32_t*>(depth + LV_TREE_MAX_TOKENS);
+    float* const rc = reinterpret_cast<float*>(anc + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32));   // [3][64]: constant, position, slope
+    int* const rtok = reinterpret_cast<int*>(rc + 3 * 64);              // [64]: token of a row
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int kw = w % KWAVES, rw = w / KWAVES;
+    const int r = lane & 31, h = lane >> 5;
+    const int words = (p.n + 31) >> 5;
+    const int n_rows = p.n * p.group;
+
+    if (blockIdx.x >= (unsigned)(p.hkv * p.shares)) {
+        // rows that hold no key keep their weights: the last workgroups copy them, one (sequence, KV head) after another
+        const int first = blockIdx.x - p.hkv * p.shares, step = gridDim.x - p.hkv * p.shares;
+        for (int bh = first; bh < p.batch * p.hkv; bh += step) {
+            const int s = bh / p.hkv, kvh = bh % p.hkv;
+            const float* src = p.w_in + (int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs;
+            float* dst = p.w_out + (int64_t)s * p.wo_bs + (int64_t)kvh * p.wo_hs;
+            for (int j = list_len(p.cache_lens, s, p.rows, p.n) + p.n + tid; j < p.rows; j += 512) dst[j] = src[j];
+        }
+        return;
+    }
+    const int kvh = blockIdx.x % p.hkv, g = blockIdx.x / p.hkv;
+
+    list_scan<BN>(p.cache_lens, p.batch, p.rows, p.n, cum, lens);
+    const ListDeal deal(p.shares, __builtin_amdgcn_readfirstlane(cum[p.batch - 1]));
+    if (g >= (int)deal.G) return;
+    int tile = __builtin_amdgcn_readfirstlane(deal.first(g));
+    const int tile_end = __builtin_amdgcn_readfirstlane(deal.first(g + 1));
+    int s = 0;
+    while (__builtin_amdgcn_readfirstlane(cum[s]) <= tile) ++s;
+
+    lds_char* const my = (lds_char*)smem + w * NS * SLOTB;
+    const uint32_t my_addr = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)my);
+    int voff[NV];      // this lane's part of a request: the LDS image is swizzled inside a row, which goes on the source address
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+        voff[j] = lane / CPR * (int)(p.k_rs * 2) + list_lds_off<D>(RPP * j + lane / CPR, lane % CPR) - (RPP * j + lane / CPR) * ROWB;
+    int k_off[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) k_off[ks] = list_lds_off<D>(r, 2 * ks + h);
+
+    while (tile < tile_end) {
+        const int len = __builtin_amdgcn_readfirstlane(lens[s]), keys = len + p.n;
+        const int list0 = s ? __builtin_amdgcn_readfirstlane(cum[s - 1]) : 0;
+        const int t0 = tile - list0, t1 = min(tile_end, __builtin_amdgcn_readfirstlane(cum[s])) - list0;
+        const __bf16* const k0 = p.k + (int64_t)s * p.k_bs + (int64_t)kvh * p.k_hs;
+        const float* const w0 = p.w_in + (int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs;
+        float* const wo0 = p.w_out + (int64_t)s * p.wo_bs + (int64_t)kvh * p.wo_hs;
+
+        // a slice of K and its old weights; rows past the last key repeat it, slices past the share bring nothing of K
+        auto request = [&](int t, int sl) __attribute__((always_inline)) {
+            const int first = t * BN + 32 * w;
+            const int valid = t < t1 ? min(keys - first, 32) : 0;
+            const uint32_t rec = valid > 0 ? (uint32_t)((valid - 1) * p.k_rs * 2 + ROWB) : 0u;
+            auto rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(k0 + (valid > 0 ? (int64_t)first * p.k_rs : 0)), 0, rec, 0x00020000);
+            const int rs2 = (int)(p.k_rs * 2), lr = lane / CPR;
+            const uint32_t dst = my_addr + sl * SLOTB;
+            if (valid <= 0 || valid >= 32) {
+#pragma unroll
+                for (int j = 0; j < NP; ++j) list_dma16(rsrc, voff[j % NV] + RPP * j * rs2, dst + j * 1024);
+            } else {
+#pragma unroll
+                for (int j = 0; j < NP; ++j) list_dma16(rsrc, voff[j % NV] + (min(RPP * j + lr, valid - 1) - lr) * rs2, dst + j * 1024);
+            }
+            weight_dma4(w0 + min(first + r, keys - 1), dst + 32 * ROWB);       // (always inside: keys >= 1)
+        };
+#pragma unroll
+        for (int i = 0; i < NS; ++i) request(t0 + i, i);
+
+        const bool sees_tree = t1 * BN > len;
+        if (p.parents) list_tree(p.parents + (int64_t)s * p.parents_bs, p.n, words, sees_tree, par, depth, anc, tid, 512);
+
+        // query fragments (lane r: row 32 b + r), and the rows' constants in LDS
+        __syncthreads();                  // the previous sequence's constants are no longer read
+        if (tid < 64) {
+            const int tc = min(tid, n_rows - 1), token = tc / p.group, head = kvh * p.group + tc % p.group;
+            rc[tid] = (tid < n_rows && !(p.parents && par[token] == LV_TREE_UNUSED)) ? row_constant(p, s, token, head) : -INFINITY;
+            if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
+                rc[64 + tid] = (float)(len + (p.parents ? depth[token] : token));
+                rc[128 + tid] = -1.4426950408889634f * p.score.slopes[head];
+            }
+            rtok[tid] = token;
+        }
+        bf16x8 qf[RT][KS];
+#pragma unroll
+        for (int b = 0; b < RT; ++b) {
+            const int row = 32 * b + r, rowc = min(row, n_rows - 1), token = rowc / p.group;
+            const bool on = row < n_rows && (!p.row_weight || p.row_weight[(int64_t)s * p.n + token] > 0.f) && !(p.parents && par[token] == LV_TREE_UNUSED);
+            const __bf16* qp = p.q + (int64_t)s * p.q_bs + (int64_t)token * p.q_ns + (int64_t)(kvh * p.group + rowc % p.group) * p.q_hs + 8 * h;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                qf[b][ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
+                if (!on) qf[b][ks] = bf16x8{};      // a row that counts for nothing may hold anything
+            }
+        }
+        // every ordinary load and store retires here: from now on the counter holds requests and the loop's stores
+#pragma unroll
+        for (int b = 0; b < RT; ++b)
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[b][ks]));
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+
+        int sl = 0;
+        for (int t = t0; t < t1; ++t) {
+            const int kb0 = t * BN + 32 * w, key = kb0 + r;
+            lds_char* const kb = my + sl * SLOTB;
+            // this slice has landed when no more than the slices behind it are on their way (the loop's stores, in between, only
+            // make the wait a little longer than it has to be)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * (NP + 1)) : "memory");
+            if (kb0 < keys) {
+                f32x16 x[RT];
+#pragma unroll
+                for (int b = 0; b < RT; ++b)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[b][i] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    const bf16x8 kf = *(LDS_PTR(bf16x8, kb + k_off[ks]));
+#pragma unroll
+                    for (int b = 0; b < RT; ++b) x[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[b][ks], kf, x[b], 0, 0, 0);
+                }
+                const float old = *(LDS_PTR(float, kb + 32 * ROWB + 4 * r));
+                const bool masked = kb0 + 32 > len;
+                const int jt = key - len;
+                float kpos = (float)key;
+                if constexpr ((MOD & LV_SCORE_BIAS) != 0)
+                    if (p.parents && jt >= 0 && jt < p.n) kpos = (float)(len + depth[jt]);
+                float sum = 0.f;
+#pragma unroll
+                for (int b = 0; b < RT; ++b) {
+                    float pv[16];
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4) {
+                        const int ar = 32 * b + 8 * q4 + 4 * h;      // rows of accumulators 4 q4 .. + 3
+                        const f32x4 cc = *reinterpret_cast<const f32x4*>(rc + ar);
+                        f32x4 pos = {}, slope = {};
+                        if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
+                            pos = *reinterpret_cast<const f32x4*>(rc + 64 + ar);
+                            slope = *reinterpret_cast<const f32x4*>(rc + 128 + ar);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int i = 4 * q4 + e;
+                            float t2;
+                            if constexpr (MOD != 0) t2 = lv_score<MOD>(x[b][i], p.scale_log2e, p.score, slope[e], pos[e] - kpos) + cc[e];
+                            else t2 = __builtin_fmaf(x[b][i], p.scale_log2e, cc[e]);
+                            pv[i] = fast_exp2(t2);
+                        }
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int token = rtok[32 * b + (i & 3) + 8 * (i >> 2) + 4 * h];
+                            bool vis = key < keys;
+                            if (vis && jt >= 0) vis = p.parents ? (anc[token * words + (jt >> 5)] >> (jt & 31)) & 1 : jt <= token;
+                            pv[i] = vis ? pv[i] : 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+                        for (int i = 0; i < o; ++i) pv[i] += pv[i + o];
+                    sum += pv[0];
+                }
+                sum = pair32_sum(sum);
+                if (h == 0 && key < keys) wo0[key] = old + sum;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // this wave is done with the slot
+            request(t + NS, sl);
+            sl = sl + 1 == NS ? 0 : sl + 1;
+            ++tile;
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");            // (what was asked for past the end is over before the slots are filled anew)
+        ++s;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// more rows
+// ---------------------------------------------------------------------------
+#define LV_WEIGHT_KEYS 128                    // keys per workgroup
+#define LV_WEIGHT_ROWS 64                     // query rows per step
+
+// constants of the rows of (sequence, KV head): [3][rows padded to 64] = exponent offset, position, -log2(e) slope
+__global__ __launch_bounds__(256) void lv_weight_rows_kernel(WeightParams p) {
+    __shared__ int par[LV_TREE_MAX_TOKENS], depth[LV_TREE_MAX_TOKENS];
+    const int bh = blockIdx.y, s = bh / p.hkv, kvh = bh % p.hkv;
+    if (p.parents) list_tree(p.parents + (int64_t)s * p.parents_bs, p.n, 0, false, par, depth, nullptr, threadIdx.x, 256);
+    const int row = blockIdx.x * 256 + threadIdx.x;
+    if (row >= p.rows_pad) return;
+    float* out = p.row_const + (int64_t)bh * 3 * p.rows_pad + row;
+    float cst = -INFINITY, pos = 0.f, slope = 0.f;
+    if (row < p.n * p.group) {
+        const int token = row / p.group, head = kvh * p.group + row % p.group;
+        if (!(p.parents && par[token] == LV_TREE_UNUSED)) cst = row_constant(p, s, token, head);
+        pos = (float)(list_len(p.cache_lens, s, p.rows, p.n) + (p.parents ? depth[token] : token));
+        if (p.score.slopes) slope = -1.4426950408889634f * p.score.slopes[head];
+    }
+    out[0] = cst;
+    out[p.rows_pad] = pos;
+    out[2 * (int64_t)p.rows_pad] = slope;
+}
+
+template <int D, int MOD, bool GUARD>
+__global__ __launch_bounds__(256, 2) void lv_weight_block_kernel(WeightParams p) {
+    constexpr int KS = D / 16;
+    constexpr int CPR = D / 8;
+    constexpr int ROWB = D * 2;
+    constexpr int TR = LV_WEIGHT_ROWS;
+    constexpr int RPP = 64 / CPR;
+    constexpr int NP = TR * ROWB / 1024 / 4;  // Q requests per wave and step: 4 or 2
+    constexpr int QB = TR * ROWB;
+    constexpr int SLOTB = QB + 3 * TR * 4;    // Q rows, three constants per row
+    constexpr int NS = 4;
+
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    float* const red = reinterpret_cast<float*>(smem + NS * SLOTB);                 // [LV_WEIGHT_KEYS]
+    int* const par = reinterpret_cast<int*>(red + LV_WEIGHT_KEYS);                  // [LV_TREE_MAX_TOKENS]
+    int* const depth = par + LV_TREE_MAX_TOKENS;
+    uint32_t* const anc = reinterpret_cast<uint32_t*>(depth + LV_TREE_MAX_TOKENS);
+
+    const int tid = threadIdx.x;
+    const int lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kw = w & 1, rw = w >> 1;
     const int r = lane & 31, h = lane >> 5;
 
     // heads and sequences fastest, then row pieces, then key blocks from the first (under a causal rule the heaviest) on
@@ -53,40 +293,18 @@ __global__ __launch_bounds__(256, 2) void lv_key_weights_kernel(WeightParams p) 
     const int rest = blockIdx.x / (p.batch * p.hkv);
     const int piece = rest % p.pieces, kb = rest / p.pieces;
     const int s = bh / p.hkv, kvh = bh % p.hkv;
-    const int len = min(max(p.cache_lens[s], 0), p.rows - p.n), keys = len + p.n;
-    const int k0 = kb * KB;
-    const int64_t w_in0 = (int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs, w_out0 = (int64_t)s * p.wo_bs + (int64_t)kvh * p.wo_hs;
+    const int len = list_len(p.cache_lens, s, p.rows, p.n), keys = len + p.n;
+    const int k0 = kb * LV_WEIGHT_KEYS;
+    const float* const wi = p.w_in + (int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs;
+    float* const wo = p.w_out + (int64_t)s * p.wo_bs + (int64_t)kvh * p.wo_hs;
     if (k0 >= keys) {                     // behind the last key: the weights stay as they are
         if (piece == 0 && p.w_in != p.w_out)
-            for (int j = k0 + tid; j < min(k0 + KB, p.rows); j += 256) p.w_out[w_out0 + j] = p.w_in[w_in0 + j];
+            for (int j = k0 + tid; j < min(k0 + LV_WEIGHT_KEYS, p.rows); j += 256) wo[j] = wi[j];
         return;
     }
     const int n_rows = p.n * p.group;
     const int words = (p.n + 31) >> 5;
-
-    if (p.parents) {
-        const int* pp = p.parents + (int64_t)s * p.parents_bs;
-        for (int i = tid; i < p.n; i += 256) {
-            const int x = pp[i];
-            par[i] = x < i ? x : -1;      // a parent stands before its child: the walk below always ends
-        }
-        __syncthreads();
-        const bool sees_tree = k0 + KB > len;
-        if (sees_tree || (MOD & LV_SCORE_BIAS) != 0) {
-            for (int i = tid; i < p.n; i += 256) {
-                for (int x = 0; x < words; ++x) anc[i * words + x] = 0;
-                int dep = -1, at = i;
-                if (par[i] != -2)
-                    while (at >= 0) {
-                        anc[i * words + (at >> 5)] |= 1u << (at & 31);
-                        ++dep;
-                        at = par[at];
-                    }
-                depth[i] = max(dep, 0);
-            }
-            __syncthreads();
-        }
-    }
+    if (p.parents) list_tree(p.parents + (int64_t)s * p.parents_bs, p.n, words, k0 + LV_WEIGHT_KEYS > len, par, depth, anc, tid, 256);
 
     // ---- this wave's keys: two groups of 32, fragments for the whole kernel
     bf16x8 kf[2][KS];
@@ -97,7 +315,7 @@ __global__ __launch_bounds__(256, 2) void lv_key_weights_kernel(WeightParams p) 
         const int base = k0 + 64 * kw + 32 * g;
         key[g] = base + r;
         const int valid = min(max(keys - base, 0), 32);      // rows past the last key read as zero and count for nothing
-        auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(p.k + (int64_t)s * p.k_bs + (int64_t)kvh * p.k_hs + (int64_t)base * p.k_rs), 0,
+        auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(p.k + (int64_t)s * p.k_bs + (int64_t)kvh * p.k_hs + (valid ? (int64_t)base * p.k_rs : 0)), 0,
                                                     valid ? (uint32_t)((valid - 1) * p.k_rs * 2 + ROWB) : 0u, 0x00020000);
         const int off = (int)(r * p.k_rs * 2) + 16 * h;
 #pragma unroll
@@ -106,6 +324,10 @@ __global__ __launch_bounds__(256, 2) void lv_key_weights_kernel(WeightParams p) 
         if constexpr ((MOD & LV_SCORE_BIAS) != 0)
             if (p.parents && key[g] >= len && key[g] < keys) kpos[g] = (float)(len + depth[key[g] - len]);
     }
+#pragma unroll
+    for (int g = 0; g < 2; ++g)
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[g][ks]));
 
     // ---- the rows that see any key of the block, this piece's share of them
     int row_lo = 0;
@@ -113,65 +335,64 @@ __global__ __launch_bounds__(256, 2) void lv_key_weights_kernel(WeightParams p) 
     const int steps = (n_rows - row_lo + TR - 1) / TR;
     const int st0 = (int)((int64_t)steps * piece / p.pieces), st1 = (int)((int64_t)steps * (piece + 1) / p.pieces);
 
-    u32x4 qreg[NLD];
-    float creg = -INFINITY, preg = 0.f, sreg = 0.f;
-    int treg = 0;
-    auto load_step = [&](int st) __attribute__((always_inline)) {
+    // ---- requests: wave w brings rows 16 w .. 16 w + 15 of a step (d = 64: the same) and one of the constants' arrays.  A lane's
+    // rows move on by TR per step, so (token, head of the group) is carried along instead of divided for.
+    const int step_tok = TR / p.group, step_head = TR % p.group;
+    int rq_tok[NP], rq_g[NP], rq_ch[NP];
 #pragma unroll
-        for (int i = 0; i < NLD; ++i) {
-            const int cidx = tid + 256 * i;
-            const int row = row_lo + st * TR + cidx / CPR;
-            qreg[i] = u32x4{0, 0, 0, 0};          // rows that count for nothing are zero: whatever they hold cannot reach a sum
-            if (row < n_rows) {
-                const int token = row / p.group, head = kvh * p.group + row % p.group;
-                const bool on = (!p.row_weight || p.row_weight[(int64_t)s * p.n + token] > 0.f) && !(p.parents && par[token] == -2);
-                if (on) qreg[i] = *reinterpret_cast<const u32x4*>(p.q + (int64_t)s * p.q_bs + (int64_t)token * p.q_ns + (int64_t)head * p.q_hs + cidx % CPR * 8);
-            }
-        }
-        if (tid < TR) {
-            const int row = row_lo + st * TR + tid;
-            creg = -INFINITY;
-            if (row < n_rows) {
-                const int token = row / p.group, head = kvh * p.group + row % p.group;
-                const float rho = p.row_weight ? p.row_weight[(int64_t)s * p.n + token] : 1.f;
-                const float l = p.lse[((int64_t)s * p.n + token) * p.hq + head];
-                treg = token;
-                if (rho > 0.f && l > -INFINITY && !(p.parents && par[token] == -2))
-                    creg = (p.row_weight ? __builtin_amdgcn_logf(rho) : 0.f) - l * 1.4426950408889634f;
-                if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
-                    preg = (float)(len + (p.parents ? depth[token] : token));
-                    sreg = -1.4426950408889634f * p.score.slopes[head];
-                }
-            }
-        }
-    };
-    auto write_step = [&](int buf) __attribute__((always_inline)) {
+    for (int j = 0; j < NP; ++j) {
+        const int tr = RPP * (NP * w + j) + lane / CPR;       // row of the tile
+        const int row = row_lo + st0 * TR + tr;
+        rq_tok[j] = row / p.group;
+        rq_g[j] = row % p.group;
+        rq_ch[j] = (list_lds_off<D>(tr, lane % CPR) - tr * ROWB) / 2;
+    }
+    const __bf16* const q0 = p.q + (int64_t)s * p.q_bs + (int64_t)kvh * p.group * p.q_hs;
+    const float* rq_c = p.row_const + ((int64_t)bh * 3 + (((MOD & LV_SCORE_BIAS) != 0 && w < 3) ? w : 0)) * p.rows_pad + row_lo + st0 * TR + lane;
+    const float* const c_last = p.row_const + ((int64_t)bh * 3 + (((MOD & LV_SCORE_BIAS) != 0 && w < 3) ? w : 0)) * p.rows_pad + p.rows_pad - TR + lane;
+    const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)smem);
+    const uint32_t c_dst = QB + (((MOD & LV_SCORE_BIAS) != 0 && w < 3) ? w : 0) * TR * 4;
+    auto request = [&](int sl) __attribute__((always_inline)) {
+        const uint32_t dst = lds_base + sl * SLOTB;
 #pragma unroll
-        for (int i = 0; i < NLD; ++i) {
-            const int cidx = tid + 256 * i;
-            *reinterpret_cast<u32x4*>(qbuf[buf] + lds_off_w<D>(cidx / CPR, cidx % CPR)) = qreg[i];
+        for (int j = 0; j < NP; ++j) {
+            // rows past the last one repeat it (their constant is -inf)
+            const int tok = min(rq_tok[j], p.n - 1), gg = rq_tok[j] < p.n ? rq_g[j] : p.group - 1;
+            const __bf16* src = q0 + (int64_t)tok * p.q_ns + (int64_t)gg * p.q_hs + rq_ch[j];
+            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst + (NP * w + j) * 1024) : "memory");
+            rq_tok[j] += step_tok;
+            rq_g[j] += step_head;
+            if (rq_g[j] >= p.group) { rq_g[j] -= p.group; ++rq_tok[j]; }
         }
-        if (tid < TR) {
-            cst[buf][tid] = creg;
-            rtok[buf][tid] = treg;
-            if constexpr ((MOD & LV_SCORE_BIAS) != 0) { rpos[buf][tid] = preg; rslope[buf][tid] = sreg; }
-        }
+        weight_dma4(rq_c < c_last ? rq_c : c_last, dst + c_dst);       // (steps past the last repeat the last rows: never used)
+        rq_c += TR;
     };
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (st0 < st1) {
+#pragma unroll
+        for (int i = 0; i < NS - 1; ++i) request(i);
+    }
 
     float sum[2] = {0.f, 0.f}, lost[2] = {0.f, 0.f};     // a key may collect tens of thousands of terms: compensated sums
-    if (st0 < st1) {
-        load_step(st0);
-        write_step(0);
-    }
-    __syncthreads();
+    int sl = 0;
     for (int st = st0; st < st1; ++st) {
-        const int buf = (st - st0) & 1;
-        if (st + 1 < st1) load_step(st + 1);
+        // this wave's part of the step has landed; behind the barrier everyone's has, and everyone is done with the step before,
+        // whose slot takes the next request
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * (NP + 1)) : "memory");
+        request(sl == 0 ? NS - 1 : sl - 1);
+        lds_char* const qb = (lds_char*)smem + sl * SLOTB;
         const int row0 = row_lo + st * TR + 32 * rw;      // first row of this wave's tile
         if (row0 < n_rows) {
-            f32x4 cv[4];
+            f32x4 cv[4], pv4[4], sv4[4];
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) cv[q4] = *reinterpret_cast<const f32x4*>(&cst[buf][32 * rw + 8 * q4 + 4 * h]);
+            for (int q4 = 0; q4 < 4; ++q4) {
+                lds_char* const cp = qb + QB + (32 * rw + 8 * q4 + 4 * h) * 4;
+                cv[q4] = *(LDS_PTR(f32x4, cp));
+                if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
+                    pv4[q4] = *(LDS_PTR(f32x4, cp + TR * 4));
+                    sv4[q4] = *(LDS_PTR(f32x4, cp + 2 * TR * 4));
+                }
+            }
             f32x16 x[2];
 #pragma unroll
             for (int g = 0; g < 2; ++g)
@@ -179,40 +400,39 @@ __global__ __launch_bounds__(256, 2) void lv_key_weights_kernel(WeightParams p) 
                 for (int i = 0; i < 16; ++i) x[g][i] = 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const bf16x8 qf = *(LDS_PTR(bf16x8, (lds_char*)qbuf[buf] + lds_off_w<D>(32 * rw + r, 2 * ks + h)));
+                const bf16x8 qf = *(LDS_PTR(bf16x8, qb + list_lds_off<D>(32 * rw + r, 2 * ks + h)));
                 x[0] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf, kf[0][ks], x[0], 0, 0, 0);
                 x[1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf, kf[1][ks], x[1], 0, 0, 0);
             }
-            // smallest token of the tile against the last key of the wave: every row sees every key?
-            const int first_token = row0 / p.group;
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const int kl = k0 + 64 * kw + 32 * g + 31;            // last key of the group
-                const bool masked = kl >= keys || (kl >= len && (p.parents || kl - len > first_token));
+                // does any row of the tile miss any key of the group?  (chain: the tile's first token, row0 / group, is the smallest;
+                // kl - len > token <=> (kl - len) * group > row0 - row0 % group, and row0 < (kl - len) * group says as much)
+                const bool masked = kl >= keys || (kl >= len && (p.parents || (int64_t)(kl - len) * p.group > row0 - p.group));
                 const int jt = key[g] - len;
                 float pv[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int rr = 32 * rw + (i & 3) + 8 * (i >> 2) + 4 * h;
-                    float t;
+                    const float cc = cv[i >> 2][i & 3];
+                    float e;
                     if constexpr (MOD != 0) {
-                        float dist = 0.f, sl = 0.f;
-                        if constexpr ((MOD & LV_SCORE_BIAS) != 0) { dist = rpos[buf][rr] - kpos[g]; sl = rslope[buf][rr]; }
-                        t = lv_score<MOD>(x[g][i], p.scale_log2e, p.score, sl, dist) + cv[i >> 2][i & 3];
+                        float dist = 0.f, sl2 = 0.f;
+                        if constexpr ((MOD & LV_SCORE_BIAS) != 0) { dist = pv4[i >> 2][i & 3] - kpos[g]; sl2 = sv4[i >> 2][i & 3]; }
+                        e = lv_score<MOD>(x[g][i], p.scale_log2e, p.score, sl2, dist) + cc;
                     } else {
-                        t = __builtin_fmaf(x[g][i], p.scale_log2e, cv[i >> 2][i & 3]);
+                        e = __builtin_fmaf(x[g][i], p.scale_log2e, cc);
                     }
-                    pv[i] = fast_exp2(t);
+                    pv[i] = fast_exp2(e);
+                    // GUARD: rows that count for nothing may hold anything, NaN included: min(NaN, 0) = 0
+                    if constexpr (GUARD) pv[i] = fminf(pv[i], cc > -INFINITY ? INFINITY : 0.f);
                 }
                 if (masked) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const int rr = 32 * rw + (i & 3) + 8 * (i >> 2) + 4 * h;
+                        const int token = min((row0 + (i & 3) + 8 * (i >> 2) + 4 * h) / p.group, p.n - 1);
                         bool vis = key[g] < keys;
-                        if (jt >= 0 && vis) {
-                            const int token = rtok[buf][rr];
-                            vis = p.parents ? (anc[token * words + (jt >> 5)] >> (jt & 31)) & 1 : jt <= token;
-                        }
+                        if (vis && jt >= 0) vis = p.parents ? (anc[token * words + (jt >> 5)] >> (jt & 31)) & 1 : jt <= token;
                         pv[i] = vis ? pv[i] : 0.f;
                     }
                 }
@@ -225,45 +445,41 @@ __global__ __launch_bounds__(256, 2) void lv_key_weights_kernel(WeightParams p) 
                 sum[g] = z;
             }
         }
-        if (st + 1 < st1) write_step(buf ^ 1);     // (that buffer's last readers passed the barrier below a step ago)
-        __syncthreads();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        sl = sl + 1 == NS ? 0 : sl + 1;
     }
+    // no request may outlive the workgroup: its LDS could already belong to another one
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
     float tot[2];
 #pragma unroll
     for (int g = 0; g < 2; ++g) tot[g] = pair32_sum(sum[g] - lost[g]);
-    if constexpr (RW > 1) {
-        if (rw > 0 && h == 0)
+    if (rw == 1 && h == 0)
 #pragma unroll
-            for (int g = 0; g < 2; ++g) red[(rw - 1) * KB + 64 * kw + 32 * g + r] = tot[g];
-        __syncthreads();
-        if (rw == 0)
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int x = 0; x < RW - 1; ++x) tot[g] += red[x * KB + 64 * kw + 32 * g + r];
-    }
+        for (int g = 0; g < 2; ++g) red[64 * kw + 32 * g + r] = tot[g];
+    __syncthreads();
     if (rw == 0 && h == 0) {
 #pragma unroll
         for (int g = 0; g < 2; ++g) {
             if (key[g] >= p.rows) continue;
+            tot[g] += red[64 * kw + 32 * g + r];
             if (p.pieces > 1) {
                 if (key[g] < keys) p.part[((int64_t)piece * p.batch * p.hkv + bh) * p.rows + key[g]] = tot[g];
             } else {
-                p.w_out[w_out0 + key[g]] = p.w_in[w_in0 + key[g]] + (key[g] < keys ? tot[g] : 0.f);
+                wo[key[g]] = wi[key[g]] + (key[g] < keys ? tot[g] : 0.f);
             }
         }
     }
 }
 
 // w_out = w_in + the pieces' sums, first piece first
-__global__ __launch_bounds__(256) void lv_key_weights_join_kernel(WeightParams p, int key_block) {
+__global__ __launch_bounds__(256) void lv_weight_join_kernel(WeightParams p) {
     const int bh = blockIdx.y;
     const int s = bh / p.hkv, kvh = bh % p.hkv;
     const int j = blockIdx.x * 256 + threadIdx.x;
-    const int keys = min(max(p.cache_lens[s], 0), p.rows - p.n) + p.n;
-    // blocks that begin behind the last key were copied by the first kernel
-    if (j >= p.rows || j / key_block * key_block >= keys) return;
+    const int keys = list_len(p.cache_lens, s, p.rows, p.n) + p.n;
+    // blocks that begin behind the last key were copied by the kernel before
+    if (j >= p.rows || j / LV_WEIGHT_KEYS * LV_WEIGHT_KEYS >= keys) return;
     float x = p.w_in[(int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs + j];
     if (j < keys) {
         float add = 0.f;
@@ -273,38 +489,69 @@ __global__ __launch_bounds__(256) void lv_key_weights_join_kernel(WeightParams p
     p.w_out[(int64_t)s * p.wo_bs + (int64_t)kvh * p.wo_hs + j] = x;
 }
 
-struct WeightPlan { int rw, key_block, key_blocks, pieces; };
+// ---------------------------------------------------------------------------
+struct WeightPlan { bool stream; int shares, pieces, key_blocks, rows_pad; int64_t part_floats, const_floats; };
 static WeightPlan weight_plan(int batch, int n, int rows, int hq, int hkv) {
-    WeightPlan t;
+    WeightPlan t{};
     const int n_rows = n * (hq / hkv);
-    t.rw = n_rows <= 32 ? 1 : 2;
-    t.key_block = 64 * (4 / t.rw);
-    t.key_blocks = (rows + t.key_block - 1) / t.key_block;
+    t.stream = n_rows <= 64 && n <= LV_TREE_MAX_TOKENS && batch <= LV_TREE_MAX_BATCH;
+    if (t.stream) {
+        const int64_t tiles = (int64_t)batch * ((rows + LV_WEIGHT_TILE - 1) / LV_WEIGHT_TILE);
+        int64_t g = 256 / hkv;                // a workgroup's slots fill a compute unit's LDS
+        if (g > tiles) g = tiles;
+        t.shares = (int)(g < 1 ? 1 : g);
+        return t;
+    }
+    t.rows_pad = (n_rows + LV_WEIGHT_ROWS - 1) / LV_WEIGHT_ROWS * LV_WEIGHT_ROWS;
+    t.key_blocks = (rows + LV_WEIGHT_KEYS - 1) / LV_WEIGHT_KEYS;
+    // two workgroups fit a compute unit: at least twice that many, so that the heavy ones start first and the light ones fill
+    // in; a piece keeps at least 8 steps so that its keys' fragments are worth fetching
     const int64_t units = (int64_t)batch * hkv * t.key_blocks;
-    // two workgroups fit a compute unit; a piece keeps at least 8 steps so that its keys' fragments are worth fetching
-    const int steps = (n_rows + 32 * t.rw - 1) / (32 * t.rw);
+    const int steps = t.rows_pad / LV_WEIGHT_ROWS;
     int64_t g = units >= 1024 ? 1 : (1024 + units - 1) / units;
     if (g > (steps + 7) / 8) g = (steps + 7) / 8;
     t.pieces = (int)(g < 1 ? 1 : g);
+    t.part_floats = t.pieces > 1 ? (int64_t)t.pieces * batch * hkv * rows : 0;
+    t.const_floats = (int64_t)batch * hkv * 3 * t.rows_pad;
     return t;
 }
 
 template <int D>
-static void launch_weights(const WeightParams& p, int mod, int rw, dim3 grid, hipStream_t stream) {
-#define LV_W(M, R) hipLaunchKernelGGL((lv_key_weights_kernel<D, M, R>), grid, dim3(256), 0, stream, p)
+static void launch_stream(const WeightParams& p, int mod, int rt, unsigned blocks, hipStream_t stream) {
+#define LV_W(M) do { \
+        if (rt == 1) hipLaunchKernelGGL((lv_weight_stream_kernel<D, 1, M>), dim3(blocks), dim3(512), weight_lds_bytes<D>(), stream, p); \
+        else hipLaunchKernelGGL((lv_weight_stream_kernel<D, 2, M>), dim3(blocks), dim3(512), weight_lds_bytes<D>(), stream, p); } while (0)
+    static_assert(weight_lds_bytes<D>() <= 160 * 1024, "one workgroup per compute unit");
     switch (mod) {
-        case 0: if (rw == 1) LV_W(0, 1); else LV_W(0, 2); break;
-        case LV_SCORE_CAP: if (rw == 1) LV_W(LV_SCORE_CAP, 1); else LV_W(LV_SCORE_CAP, 2); break;
-        case LV_SCORE_BIAS: if (rw == 1) LV_W(LV_SCORE_BIAS, 1); else LV_W(LV_SCORE_BIAS, 2); break;
-        default: if (rw == 1) LV_W(3, 1); else LV_W(3, 2);
+        case 0: LV_W(0); break;
+        case LV_SCORE_CAP: LV_W(LV_SCORE_CAP); break;
+        case LV_SCORE_BIAS: LV_W(LV_SCORE_BIAS); break;
+        default: LV_W((LV_SCORE_CAP | LV_SCORE_BIAS));
+    }
+#undef LV_W
+}
+
+template <int D>
+static void launch_block(const WeightParams& p, int mod, bool guard, unsigned blocks, hipStream_t stream) {
+    constexpr size_t lds = (size_t)4 * (LV_WEIGHT_ROWS * D * 2 + 3 * LV_WEIGHT_ROWS * 4) + LV_WEIGHT_KEYS * 4 + LV_TREE_MAX_TOKENS * 8 +
+                           LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4;
+    static_assert(2 * lds <= 160 * 1024, "two workgroups per compute unit");
+#define LV_W(M) do { \
+        if (guard) hipLaunchKernelGGL((lv_weight_block_kernel<D, M, true>), dim3(blocks), dim3(256), lds, stream, p); \
+        else hipLaunchKernelGGL((lv_weight_block_kernel<D, M, false>), dim3(blocks), dim3(256), lds, stream, p); } while (0)
+    switch (mod) {
+        case 0: LV_W(0); break;
+        case LV_SCORE_CAP: LV_W(LV_SCORE_CAP); break;
+        case LV_SCORE_BIAS: LV_W(LV_SCORE_BIAS); break;
+        default: LV_W((LV_SCORE_CAP | LV_SCORE_BIAS));
     }
 #undef LV_W
 }
 
 extern "C" int64_t lv_key_weights_workspace_bytes(int batch, int n, int rows, int hq, int hkv) {
-    if (batch <= 0 || n <= 0 || rows < n || hq <= 0 || hkv <= 0 || hq % hkv) return 0;
+    if (batch <= 0 || n <= 0 || rows < n || hq <= 0 || hkv <= 0 || hq % hkv || (int64_t)n * (hq / hkv) > 0x7ffff000LL) return 0;
     const WeightPlan t = weight_plan(batch, n, rows, hq, hkv);
-    return t.pieces > 1 ? (int64_t)t.pieces * batch * hkv * rows * (int64_t)sizeof(float) : 0;
+    return (t.part_floats + t.const_floats) * (int64_t)sizeof(float);
 }
 
 extern "C" int lv_key_weights(const void* q, const void* k, const float* lse, const float* row_weight, const float* w_in, float* w_out,
@@ -322,24 +569,36 @@ extern "C" int lv_key_weights(const void* q, const void* k, const float* lse, co
     if (!(softcap >= 0.f) || softcap > 1e30f) return lv_fail(LV_EINVAL, "lv_key_weights: softcap %g must be a finite number above 0 (0: no cap)", (double)softcap);
     if (!(softmax_scale > -1e30f && softmax_scale < 1e30f)) return lv_fail(LV_EINVAL, "lv_key_weights: softmax_scale is not finite");
     const WeightPlan t = weight_plan(batch, n, rows, hq, hkv);
-    const int64_t need = lv_key_weights_workspace_bytes(batch, n, rows, hq, hkv);
-    if (need && !workspace) return lv_fail(LV_EINVAL, "lv_key_weights: null workspace");
+    const int64_t need = (t.part_floats + t.const_floats) * (int64_t)sizeof(float);
+    if (need && (!workspace || ((uintptr_t)workspace & 15))) return lv_fail(LV_EINVAL, "lv_key_weights: workspace must be there and 16-byte aligned");
     if (workspace_bytes < need) return lv_fail(LV_ESIZE, "lv_key_weights: %lld bytes of workspace needed, room for %lld", (long long)need, (long long)workspace_bytes);
-    const int64_t blocks = (int64_t)batch * hkv * t.key_blocks * t.pieces;
-    if (blocks > 0x7fffffffLL || (int64_t)batch * hkv > 65535) return lv_fail(LV_EINVAL, "lv_key_weights: grid too large");
+    if ((int64_t)batch * hkv > 65535 || (int64_t)batch * (rows / LV_WEIGHT_TILE + 1) > 0x7fffffffLL) return lv_fail(LV_EINVAL, "lv_key_weights: grid too large");
     WeightParams p{};
     p.q = (const __bf16*)q; p.k = (const __bf16*)k; p.lse = lse; p.row_weight = row_weight; p.w_in = w_in; p.w_out = w_out;
-    p.cache_lens = cache_lens; p.parents = parents; p.parents_bs = parents_bs; p.part = (float*)workspace;
-    p.batch = batch; p.n = n; p.rows = rows; p.hq = hq; p.hkv = hkv; p.group = hq / hkv; p.pieces = t.pieces;
+    p.cache_lens = cache_lens; p.parents = parents; p.parents_bs = parents_bs;
+    p.row_const = (float*)workspace; p.part = p.row_const + t.const_floats;
+    p.batch = batch; p.n = n; p.rows = rows; p.hq = hq; p.hkv = hkv; p.group = hq / hkv; p.pieces = t.pieces; p.shares = t.shares; p.rows_pad = t.rows_pad;
     p.q_bs = q_bs; p.q_ns = q_ns; p.q_hs = q_hs; p.k_bs = k_bs; p.k_rs = k_rs; p.k_hs = k_hs;
     p.wi_bs = wi_bs; p.wi_hs = wi_hs; p.wo_bs = wo_bs; p.wo_hs = wo_hs;
     p.scale_log2e = softmax_scale * 1.4426950408889634f;
     p.score = lv_score_rule(softmax_scale, softcap, slopes);
     const int mod = lv_score_mod(softcap, slopes) & (LV_SCORE_CAP | LV_SCORE_BIAS);
-    if (d == 128) launch_weights<128>(p, mod, t.rw, dim3((unsigned)blocks), (hipStream_t)stream);
-    else launch_weights<64>(p, mod, t.rw, dim3((unsigned)blocks), (hipStream_t)stream);
-    if (hipGetLastError() != hipSuccess) return lv_fail(LV_ELAUNCH, "lv_key_weights: launch failed");
-    if (t.pieces > 1)
-        hipLaunchKernelGGL(lv_key_weights_join_kernel, dim3((unsigned)((rows + 255) / 256), (unsigned)(batch * hkv)), dim3(256), 0, (hipStream_t)stream, p, t.key_block);
+    hipStream_t st = (hipStream_t)stream;
+    if (t.stream) {
+        const int rt = n * p.group <= 32 ? 1 : 2;
+        const unsigned copy = w_in == w_out ? 0u : (unsigned)(batch * hkv < 256 ? batch * hkv : 256);
+        const unsigned blocks = (unsigned)(hkv * t.shares) + copy;
+        if (d == 128) launch_stream<128>(p, mod, rt, blocks, st);
+        else launch_stream<64>(p, mod, rt, blocks, st);
+    } else {
+        const int64_t blocks = (int64_t)batch * hkv * t.key_blocks * t.pieces;
+        if (blocks > 0x7fffffffLL) return lv_fail(LV_EINVAL, "lv_key_weights: grid too large");
+        hipLaunchKernelGGL(lv_weight_rows_kernel, dim3((unsigned)((t.rows_pad + 255) / 256), (unsigned)(batch * hkv)), dim3(256), 0, st, p);
+        const bool guard = parents || row_weight;
+        if (d == 128) launch_block<128>(p, mod, guard, (unsigned)blocks, st);
+        else launch_block<64>(p, mod, guard, (unsigned)blocks, st);
+        if (t.pieces > 1)
+            hipLaunchKernelGGL(lv_weight_join_kernel, dim3((unsigned)((rows + 255) / 256), (unsigned)(batch * hkv)), dim3(256), 0, st, p);
+    }
     return hipGetLastError() == hipSuccess ? LV_OK : lv_fail(LV_ELAUNCH, "lv_key_weights: launch failed");
 }

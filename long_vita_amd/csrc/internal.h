@@ -146,8 +146,9 @@ struct WeightParams {
     const int32_t* cache_lens;
     const int32_t* parents;
     int64_t parents_bs;
+    float* row_const;            // [batch * hkv][3][rows_pad]
     float* part;                 // [pieces][batch * hkv][rows]
-    int batch, n, rows, hq, hkv, group, pieces;
+    int batch, n, rows, hq, hkv, group, pieces, shares, rows_pad;
     int64_t q_bs, q_ns, q_hs, k_bs, k_rs, k_hs, wi_bs, wi_hs, wo_bs, wo_hs;
     float scale_log2e;
     ScoreRule score;
