@@ -32,6 +32,18 @@ __device__ __forceinline__ float row_constant(const WeightParams& p, int s, int 
     return (p.row_weight ? __builtin_amdgcn_logf(rho) : 0.f) - l * 1.4426950408889634f;
 }
 
+// rows that hold no key keep their weights (launched when w_out is not w_in); 4096 rows of one (sequence, KV head) per workgroup
+__global__ __launch_bounds__(256) void lv_weight_copy_kernel(WeightParams p) {
+    const int bh = blockIdx.y, s = bh / p.hkv, kvh = bh % p.hkv;
+    const int keys = list_len(p.cache_lens, s, p.rows, p.n) + p.n;
+    const int j0 = blockIdx.x * 4096, j1 = min(j0 + 4096, p.rows);
+    if (j1 <= keys) return;
+    const float* src = p.w_in + (int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs;
+    float* dst = p.w_out + (int64_t)s * p.wo_bs + (int64_t)kvh * p.wo_hs;
+#pragma unroll 8
+    for (int j = max(j0, keys) + threadIdx.x; j < j1; j += 256) dst[j] = src[j];
+}
+
 // ---------------------------------------------------------------------------
 // up to 32 RT query rows
 // ---------------------------------------------------------------------------
@@ -70,17 +82,6 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
     const int words = (p.n + 31) >> 5;
     const int n_rows = p.n * p.group;
 
-    if (blockIdx.x >= (unsigned)(p.hkv * p.shares)) {
-        // rows that hold no key keep their weights: the last workgroups copy them, one (sequence, KV head) after another
-        const int first = blockIdx.x - p.hkv * p.shares, step = gridDim.x - p.hkv * p.shares;
-        for (int bh = first; bh < p.batch * p.hkv; bh += step) {
-            const int s = bh / p.hkv, kvh = bh % p.hkv;
-            const float* src = p.w_in + (int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs;
-            float* dst = p.w_out + (int64_t)s * p.wo_bs + (int64_t)kvh * p.wo_hs;
-            for (int j = list_len(p.cache_lens, s, p.rows, p.n) + p.n + tid; j < p.rows; j += 512) dst[j] = src[j];
-        }
-        return;
-    }
     const int kvh = blockIdx.x % p.hkv, g = blockIdx.x / p.hkv;
 
     list_scan<BN>(p.cache_lens, p.batch, p.rows, p.n, cum, lens);
@@ -211,12 +212,16 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
                         }
                     }
                     if (masked) {
+                        // a chain: row R (token R / group) sees drafted key jt from row jt * group on; a tree's keys are looked up
+                        const int first_row = key >= keys ? 0x7fffffff : max(jt, 0) * p.group;
+                        const bool look = p.parents && key < keys && jt >= 0;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const int token = rtok[32 * b + (i & 3) + 8 * (i >> 2) + 4 * h];
-                            bool vis = key < keys;
-                            if (vis && jt >= 0) vis = p.parents ? (anc[token * words + (jt >> 5)] >> (jt & 31)) & 1 : jt <= token;
+                            const int ar = 32 * b + (i & 3) + 8 * (i >> 2) + 4 * h;
+                            bool vis = ar >= first_row;
+                            if (look) vis = (anc[rtok[ar] * words + (jt >> 5)] >> (jt & 31)) & 1;
                             pv[i] = vis ? pv[i] : 0.f;
+                            asm volatile("" : "+v"(pv[i]));      // keeps this a branch
                         }
                     }
 #pragma unroll
@@ -264,8 +269,9 @@ __global__ __launch_bounds__(256) void lv_weight_rows_kernel(WeightParams p) {
     out[2 * (int64_t)p.rows_pad] = slope;
 }
 
+// three workgroups fit a compute unit (without a tree; with one, or with the positions and slopes of a bias in registers, two)
 template <int D, int MOD, bool GUARD>
-__global__ __launch_bounds__(256, 2) void lv_weight_block_kernel(WeightParams p) {
+__global__ __launch_bounds__(256, (MOD & LV_SCORE_BIAS) || GUARD ? 2 : 3) void lv_weight_block_kernel(WeightParams p) {
     constexpr int KS = D / 16;
     constexpr int CPR = D / 8;
     constexpr int ROWB = D * 2;
@@ -274,7 +280,7 @@ __global__ __launch_bounds__(256, 2) void lv_weight_block_kernel(WeightParams p)
     constexpr int NP = TR * ROWB / 1024 / 4;  // Q requests per wave and step: 4 or 2
     constexpr int QB = TR * ROWB;
     constexpr int SLOTB = QB + 3 * TR * 4;    // Q rows, three constants per row
-    constexpr int NS = 4;
+    constexpr int NS = 3;
 
     extern __shared__ __attribute__((aligned(16))) char smem[];
     float* const red = reinterpret_cast<float*>(smem + NS * SLOTB);                 // [LV_WEIGHT_KEYS]
@@ -335,42 +341,71 @@ __global__ __launch_bounds__(256, 2) void lv_weight_block_kernel(WeightParams p)
     const int steps = (n_rows - row_lo + TR - 1) / TR;
     const int st0 = (int)((int64_t)steps * piece / p.pieces), st1 = (int)((int64_t)steps * (piece + 1) / p.pieces);
 
-    // ---- requests: wave w brings rows 16 w .. 16 w + 15 of a step (d = 64: the same) and one of the constants' arrays.  A lane's
-    // rows move on by TR per step, so (token, head of the group) is carried along instead of divided for.
+    // ---- requests: wave w brings rows 16 w .. 16 w + 15 of a step and one of the constants' arrays.  A lane's rows move on by TR
+    // per step, so their offsets from the step's first token are carried along instead of divided and multiplied for.
+    const int ns2 = (int)(p.q_ns * 2), hs2 = (int)(p.q_hs * 2);
     const int step_tok = TR / p.group, step_head = TR % p.group;
-    int rq_tok[NP], rq_g[NP], rq_ch[NP];
+    const int wrap = ns2 - p.group * hs2;                      // (a head number past the group: the next token's)
+    int rq_row = row_lo + st0 * TR;                            // first row of the next step
+    int tok0 = __builtin_amdgcn_readfirstlane(rq_row / p.group), g0 = __builtin_amdgcn_readfirstlane(rq_row % p.group);
+    int rq_g[NP], rq_off[NP], rq_ch[NP];
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
         const int tr = RPP * (NP * w + j) + lane / CPR;       // row of the tile
-        const int row = row_lo + st0 * TR + tr;
-        rq_tok[j] = row / p.group;
-        rq_g[j] = row % p.group;
-        rq_ch[j] = (list_lds_off<D>(tr, lane % CPR) - tr * ROWB) / 2;
+        rq_ch[j] = list_lds_off<D>(tr, lane % CPR) - tr * ROWB;
+        rq_g[j] = (g0 + tr) % p.group;
+        rq_off[j] = (g0 + tr) / p.group * ns2 + rq_g[j] * hs2 + rq_ch[j];
     }
     const __bf16* const q0 = p.q + (int64_t)s * p.q_bs + (int64_t)kvh * p.group * p.q_hs;
-    const float* rq_c = p.row_const + ((int64_t)bh * 3 + (((MOD & LV_SCORE_BIAS) != 0 && w < 3) ? w : 0)) * p.rows_pad + row_lo + st0 * TR + lane;
-    const float* const c_last = p.row_const + ((int64_t)bh * 3 + (((MOD & LV_SCORE_BIAS) != 0 && w < 3) ? w : 0)) * p.rows_pad + p.rows_pad - TR + lane;
+    const int which = ((MOD & LV_SCORE_BIAS) != 0 && w < 3) ? w : 0;
+    const float* const c0 = p.row_const + ((int64_t)bh * 3 + which) * p.rows_pad + lane;
     const uint32_t lds_base = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_char*)smem);
-    const uint32_t c_dst = QB + (((MOD & LV_SCORE_BIAS) != 0 && w < 3) ? w : 0) * TR * 4;
     auto request = [&](int sl) __attribute__((always_inline)) {
         const uint32_t dst = lds_base + sl * SLOTB;
+        if (rq_row + TR <= n_rows) {
+            auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(q0 + (int64_t)tok0 * p.q_ns), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+            for (int j = 0; j < NP; ++j) list_dma16(rs, rq_off[j], dst + (NP * w + j) * 1024);
+        } else {                                               // rows past the last one repeat it (their constant is -inf)
+            const int tb = min(tok0, p.n - 1);
+            auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<__bf16*>(q0 + (int64_t)tb * p.q_ns), 0, 0x7fffffff, 0x00020000);
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                const int row = min(rq_row + RPP * (NP * w + j) + lane / CPR, n_rows - 1);
+                list_dma16(rs, (row / p.group - tb) * ns2 + row % p.group * hs2 + rq_ch[j], dst + (NP * w + j) * 1024);
+            }
+        }
+        weight_dma4(c0 + min(rq_row, p.rows_pad - TR), dst + QB + which * TR * 4);     // (steps past the last are never used)
+        rq_row += TR;
+        tok0 += step_tok;
+        g0 += step_head;
+        const bool over = g0 >= p.group;                       // the step's own first token moves on by one more: so do the offsets' zero
+        if (over) { g0 -= p.group; ++tok0; }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-            // rows past the last one repeat it (their constant is -inf)
-            const int tok = min(rq_tok[j], p.n - 1), gg = rq_tok[j] < p.n ? rq_g[j] : p.group - 1;
-            const __bf16* src = q0 + (int64_t)tok * p.q_ns + (int64_t)gg * p.q_hs + rq_ch[j];
-            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(dst + (NP * w + j) * 1024) : "memory");
-            rq_tok[j] += step_tok;
             rq_g[j] += step_head;
-            if (rq_g[j] >= p.group) { rq_g[j] -= p.group; ++rq_tok[j]; }
+            const bool next = rq_g[j] >= p.group;
+            rq_g[j] -= next ? p.group : 0;
+            rq_off[j] += step_head * hs2 + (next ? wrap : 0) - (over ? ns2 : 0);
         }
-        weight_dma4(rq_c < c_last ? rq_c : c_last, dst + c_dst);       // (steps past the last repeat the last rows: never used)
-        rq_c += TR;
     };
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (st0 < st1) {
 #pragma unroll
         for (int i = 0; i < NS - 1; ++i) request(i);
+    }
+
+    // Who sees which key.  A chain: row R (token R / group) sees drafted key jt from row jt * group on; so a lane's key has a first
+    // row, and a group of keys a row from which on every row sees all of it.  A tree's keys are looked up.
+    int first_row[2], full_row[2];
+    bool tree_group[2];
+    uint32_t seen = 0;
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+        const int kl = k0 + 64 * kw + 32 * g + 31;            // last key of the group
+        tree_group[g] = p.parents && kl >= len;
+        full_row[g] = tree_group[g] || kl >= keys ? 0x7fffffff : max(kl - len, 0) * p.group;
+        first_row[g] = key[g] >= keys ? 0x7fffffff : max(key[g] - len, 0) * p.group;
     }
 
     float sum[2] = {0.f, 0.f}, lost[2] = {0.f, 0.f};     // a key may collect tens of thousands of terms: compensated sums
@@ -406,11 +441,6 @@ __global__ __launch_bounds__(256, 2) void lv_weight_block_kernel(WeightParams p)
             }
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
-                const int kl = k0 + 64 * kw + 32 * g + 31;            // last key of the group
-                // does any row of the tile miss any key of the group?  (chain: the tile's first token, row0 / group, is the smallest;
-                // kl - len > token <=> (kl - len) * group > row0 - row0 % group, and row0 < (kl - len) * group says as much)
-                const bool masked = kl >= keys || (kl >= len && (p.parents || (int64_t)(kl - len) * p.group > row0 - p.group));
-                const int jt = key[g] - len;
                 float pv[16];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
@@ -427,13 +457,28 @@ __global__ __launch_bounds__(256, 2) void lv_weight_block_kernel(WeightParams p)
                     // GUARD: rows that count for nothing may hold anything, NaN included: min(NaN, 0) = 0
                     if constexpr (GUARD) pv[i] = fminf(pv[i], cc > -INFINITY ? INFINITY : 0.f);
                 }
-                if (masked) {
+                if (row0 < full_row[g]) {          // some row of the tile misses some key of the group
+                    const int base = row0 + 4 * h;
+                    if (tree_group[g]) {
+                        const int jt = key[g] - len;
+#pragma unroll 1
+                        for (int i = 0; i < 16; ++i) {
+                            const int token = min((base + (i & 3) + 8 * (i >> 2)) / p.group, p.n - 1);
+                            bool vis = key[g] < keys;
+                            if (vis && jt >= 0) vis = (anc[token * words + (jt >> 5)] >> (jt & 31)) & 1;
+                            seen = (seen & ~(1u << i)) | ((uint32_t)vis << i);
+                        }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const int token = min((row0 + (i & 3) + 8 * (i >> 2) + 4 * h) / p.group, p.n - 1);
-                        bool vis = key[g] < keys;
-                        if (vis && jt >= 0) vis = p.parents ? (anc[token * words + (jt >> 5)] >> (jt & 31)) & 1 : jt <= token;
-                        pv[i] = vis ? pv[i] : 0.f;
+                        for (int i = 0; i < 16; ++i) {
+                            pv[i] = (seen >> i) & 1 ? pv[i] : 0.f;
+                            asm volatile("" : "+v"(pv[i]));      // keeps this a branch
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            pv[i] = base + (i & 3) + 8 * (i >> 2) >= first_row[g] ? pv[i] : 0.f;
+                            asm volatile("" : "+v"(pv[i]));
+                        }
                     }
                 }
 #pragma unroll
@@ -504,11 +549,11 @@ static WeightPlan weight_plan(int batch, int n, int rows, int hq, int hkv) {
     }
     t.rows_pad = (n_rows + LV_WEIGHT_ROWS - 1) / LV_WEIGHT_ROWS * LV_WEIGHT_ROWS;
     t.key_blocks = (rows + LV_WEIGHT_KEYS - 1) / LV_WEIGHT_KEYS;
-    // two workgroups fit a compute unit: at least twice that many, so that the heavy ones start first and the light ones fill
+    // three workgroups fit a compute unit: at least twice that many, so that the heavy ones start first and the light ones fill
     // in; a piece keeps at least 8 steps so that its keys' fragments are worth fetching
     const int64_t units = (int64_t)batch * hkv * t.key_blocks;
     const int steps = t.rows_pad / LV_WEIGHT_ROWS;
-    int64_t g = units >= 1024 ? 1 : (1024 + units - 1) / units;
+    int64_t g = units >= 1536 ? 1 : (1536 + units - 1) / units;
     if (g > (steps + 7) / 8) g = (steps + 7) / 8;
     t.pieces = (int)(g < 1 ? 1 : g);
     t.part_floats = t.pieces > 1 ? (int64_t)t.pieces * batch * hkv * rows : 0;
@@ -533,9 +578,10 @@ static void launch_stream(const WeightParams& p, int mod, int rt, unsigned block
 
 template <int D>
 static void launch_block(const WeightParams& p, int mod, bool guard, unsigned blocks, hipStream_t stream) {
-    constexpr size_t lds = (size_t)4 * (LV_WEIGHT_ROWS * D * 2 + 3 * LV_WEIGHT_ROWS * 4) + LV_WEIGHT_KEYS * 4 + LV_TREE_MAX_TOKENS * 8 +
-                           LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4;
-    static_assert(2 * lds <= 160 * 1024, "two workgroups per compute unit");
+    constexpr size_t base = (size_t)3 * (LV_WEIGHT_ROWS * D * 2 + 3 * LV_WEIGHT_ROWS * 4) + LV_WEIGHT_KEYS * 4;
+    constexpr size_t tree = LV_TREE_MAX_TOKENS * 8 + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4;
+    static_assert(3 * base <= 160 * 1024 && 2 * (base + tree) <= 160 * 1024, "workgroups per compute unit");
+    const size_t lds = base + (p.parents ? tree : 0);
 #define LV_W(M) do { \
         if (guard) hipLaunchKernelGGL((lv_weight_block_kernel<D, M, true>), dim3(blocks), dim3(256), lds, stream, p); \
         else hipLaunchKernelGGL((lv_weight_block_kernel<D, M, false>), dim3(blocks), dim3(256), lds, stream, p); } while (0)
@@ -565,6 +611,9 @@ extern "C" int lv_key_weights(const void* q, const void* k, const float* lse, co
     if (batch <= 0 || n <= 0 || rows < n) return lv_fail(LV_EINVAL, "lv_key_weights: batch %d, %d tokens, %d cache rows", batch, n, rows);
     if (parents && n > LV_TREE_MAX_TOKENS) return lv_fail(LV_EINVAL, "lv_key_weights: a tree of %d tokens (at most %d)", n, LV_TREE_MAX_TOKENS);
     if ((int64_t)n * (hq / hkv) > 0x7ffff000LL) return lv_fail(LV_EINVAL, "lv_key_weights: too many query rows");
+    // a step of 64 query rows is addressed with 32-bit byte offsets from its first token
+    if (q_hs < 0 || (66 * q_ns + (hq / hkv) * q_hs) * 2 > 0x7fffffffLL || q_ns > 0x3fffffffLL || q_hs > 0x3fffffffLL)
+        return lv_fail(LV_EINVAL, "lv_key_weights: q token / head strides %lld / %lld out of range", (long long)q_ns, (long long)q_hs);
     if (k_bs < 0 || (k_bs & 7) || parents_bs < 0) return lv_fail(LV_EINVAL, "lv_key_weights: batch strides must not be negative, K's a multiple of 8 elements");
     if (!(softcap >= 0.f) || softcap > 1e30f) return lv_fail(LV_EINVAL, "lv_key_weights: softcap %g must be a finite number above 0 (0: no cap)", (double)softcap);
     if (!(softmax_scale > -1e30f && softmax_scale < 1e30f)) return lv_fail(LV_EINVAL, "lv_key_weights: softmax_scale is not finite");
@@ -586,8 +635,9 @@ extern "C" int lv_key_weights(const void* q, const void* k, const float* lse, co
     hipStream_t st = (hipStream_t)stream;
     if (t.stream) {
         const int rt = n * p.group <= 32 ? 1 : 2;
-        const unsigned copy = w_in == w_out ? 0u : (unsigned)(batch * hkv < 256 ? batch * hkv : 256);
-        const unsigned blocks = (unsigned)(hkv * t.shares) + copy;
+        if (w_in != w_out)
+            hipLaunchKernelGGL(lv_weight_copy_kernel, dim3((unsigned)((rows + 4095) / 4096), (unsigned)(batch * hkv)), dim3(256), 0, st, p);
+        const unsigned blocks = (unsigned)(hkv * t.shares);
         if (d == 128) launch_stream<128>(p, mod, rt, blocks, st);
         else launch_stream<64>(p, mod, rt, blocks, st);
     } else {

@@ -434,7 +434,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: tor
             raise LvAttnError(f"{who}: out must be weight itself or not overlap it")
     if any(x == 0 and m > 1 for x, m in zip(out.stride(), out.shape)):
         raise LvAttnError(f"{who}: an expanded tensor cannot be written")
-    if q.stride(3) != 1 or q.data_ptr() % 16 or any(x < 0 or x % 8 for x in q.stride()[:3]):
+    if (q.stride(3) != 1 or q.data_ptr() % 16 or any(x < 0 or x % 8 for x in q.stride()[:3]) or
+            (66 * q.stride(1) + hq // hkv * q.stride(2)) * 2 >= 1 << 31):      # (a step of 64 rows is addressed with 32-bit offsets)
         q = q.clone(memory_format=torch.contiguous_format)
     lse, cache_lens = lse.contiguous(), cache_lens.contiguous()
     row_weight = None if row_weight is None else row_weight.contiguous()
