@@ -7,13 +7,13 @@
 // puts it; -0 equal to 0), the threshold is found digit by digit from histograms, and what lies above it, plus the first few
 // equal to it, is numbered by counting.  Counts are integers, so the order in which they are added does not matter.  Caches of
 // up to 16,384 rows: one workgroup per head holds all keys in registers and does everything in LDS, one launch.  Longer ones:
-// workgroups of 8,192 rows, five short launches, each a read of the weights (which stay in the last-level cache).
+// workgroups of 2,048 rows, six short launches, each a read of the weights (which stay in the last-level cache).
 // Then the kept rows are gathered; that is where the bytes are: K and V, read and written once.
 #include "internal.h"
 #include "../../include/lvattn.h"
 
 #define LV_EVICT_SMALL 16384
-#define LV_EVICT_CHUNK 8192
+#define LV_EVICT_CHUNK 2048
 
 __device__ __forceinline__ uint32_t order_key(float x) {
     if (x != x) return 0xffffffffu;
@@ -33,10 +33,10 @@ __device__ __forceinline__ EvictRange evict_range(const EvictParams& p, int s) {
 }
 
 // ---------------------------------------------------------------------------
-// up to LV_EVICT_SMALL rows: 1024 threads, row 1024 i + tid in register i
+// up to 1024 PER rows: 1024 threads, row 1024 i + tid in register i
 // ---------------------------------------------------------------------------
+template <int PER>
 __global__ __launch_bounds__(1024) void lv_evict_small_kernel(EvictParams p) {
-    constexpr int PER = LV_EVICT_SMALL / 1024;
     constexpr int COPIES = 8;                       // of the histogram: lanes that hit one bin are spread over them
     __shared__ uint32_t hist[COPIES][257];
     __shared__ uint32_t digit_s, left_s;
@@ -124,7 +124,7 @@ __global__ __launch_bounds__(1024) void lv_evict_small_kernel(EvictParams p) {
             if (lane == 0) cnt[i * 16 + w] = __popcll(m);
         }
         __syncthreads();
-        if (tid < PER * 16) {                       // exclusive scan of 256 counts by four waves
+        if (tid < PER * 16) {                       // exclusive scan of the counts, a wave to 64 of them
             const uint32_t mine = cnt[tid];
             uint32_t incl = mine;
 #pragma unroll
@@ -203,25 +203,30 @@ __global__ __launch_bounds__(256) void lv_evict_clear_kernel(EvictParams p) {
 }
 
 __global__ __launch_bounds__(256) void lv_evict_hist_kernel(EvictParams p, int pass) {
-    constexpr int COPIES = 4;
+    constexpr int COPIES = 2;
+    constexpr int PER = LV_EVICT_CHUNK / 256;
     __shared__ uint32_t hist[COPIES][2049];
     const int bh = blockIdx.y, s = bh / p.hkv, kvh = bh % p.hkv, tid = threadIdx.x;
     const EvictRange e = evict_range(p, s);
     const int c0 = blockIdx.x * LV_EVICT_CHUNK, c1 = min(c0 + LV_EVICT_CHUNK, e.hi);
     if (!e.cut || e.want <= 0 || c0 >= e.hi) return;
+    const float* wt = p.w_in + (int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs;
+    float x[PER];                                                  // on their way while the threshold's digits so far are found
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int j = c0 + 256 * i + tid;
+        x[i] = j >= e.lo && j < c1 ? wt[j] : 0.f;
+    }
     for (int i = tid; i < COPIES * 2049; i += 256) (&hist[0][0])[i] = 0;
-    const Select sel = evict_select(p, bh, e.want, pass);          // (ends with a barrier, or has none to wait for)
+    const Select sel = evict_select(p, bh, e.want, pass);
     __syncthreads();
     const uint32_t himask = pass == 0 ? 0u : 0xffffffffu << (digit_shift(pass) + digit_bits(pass));
     const uint32_t dmask = (1u << digit_bits(pass)) - 1;
-    const float* wt = p.w_in + (int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs;
-#pragma unroll 8
-    for (int i = 0; i < LV_EVICT_CHUNK / 256; ++i) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
         const int j = c0 + 256 * i + tid;
-        if (j >= e.lo && j < c1) {
-            const uint32_t key = order_key(wt[j]);
-            if ((key & himask) == sel.prefix) atomicAdd(&hist[tid & (COPIES - 1)][(key >> digit_shift(pass)) & dmask], 1u);
-        }
+        const uint32_t key = order_key(x[i]);
+        if (j >= e.lo && j < c1 && (key & himask) == sel.prefix) atomicAdd(&hist[tid & (COPIES - 1)][(key >> digit_shift(pass)) & dmask], 1u);
     }
     __syncthreads();
     uint32_t* out = p.hist + ((int64_t)pass * p.batch * p.hkv + bh) * 2048;
@@ -247,13 +252,19 @@ __global__ __launch_bounds__(256) void lv_evict_count_kernel(EvictParams p) {
     const int bh = blockIdx.y, s = bh / p.hkv, kvh = bh % p.hkv, tid = threadIdx.x;
     const EvictRange e = evict_range(p, s);
     if (!e.cut) return;
-    const Select sel = evict_select(p, bh, e.want, e.want > 0 ? 3 : 0);
+    constexpr int PER = LV_EVICT_CHUNK / 256;
     const float* wt = p.w_in + (int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs;
-    uint32_t n0 = 0, n1 = 0;
-#pragma unroll 8
-    for (int i = 0; i < LV_EVICT_CHUNK / 256; ++i) {
+    float x[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
         const int j = blockIdx.x * LV_EVICT_CHUNK + 256 * i + tid;
-        const int c = evict_class(e, sel, j, j < e.len ? wt[j] : 0.f);
+        x[i] = j < e.len ? wt[j] : 0.f;
+    }
+    const Select sel = evict_select(p, bh, e.want, e.want > 0 ? 3 : 0);
+    uint32_t n0 = 0, n1 = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int c = evict_class(e, sel, blockIdx.x * LV_EVICT_CHUNK + 256 * i + tid, x[i]);
         n0 += __popcll(__ballot(c == 0));
         n1 += __popcll(__ballot(c == 1));
     }
@@ -268,10 +279,10 @@ __global__ __launch_bounds__(256) void lv_evict_count_kernel(EvictParams p) {
     }
 }
 
-// the kept rows' numbers: a thread owns 32 consecutive rows of the chunk
+// the kept rows' numbers: a thread owns 8 consecutive rows of the chunk
 __global__ __launch_bounds__(256) void lv_evict_index_kernel(EvictParams p) {
     constexpr int PER = LV_EVICT_CHUNK / 256;
-    __shared__ float tile[LV_EVICT_CHUNK + LV_EVICT_CHUNK / 32];
+    __shared__ float tile[LV_EVICT_CHUNK + LV_EVICT_CHUNK / 32];      // (one word in 33 unused: a thread's rows are 8 apart)
     __shared__ uint32_t sum0[4], sum1[4];
     const int bh = blockIdx.y, s = bh / p.hkv, kvh = bh % p.hkv, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const EvictRange e = evict_range(p, s);
@@ -395,7 +406,8 @@ extern "C" int lv_evict_index(const float* weight, const int32_t* cache_lens, in
     p.batch = batch; p.rows = rows; p.hkv = hkv; p.keep = keep; p.sink = sink; p.recent = recent; p.wi_bs = w_bs; p.wi_hs = w_hs;
     hipStream_t st = (hipStream_t)stream;
     if (rows <= LV_EVICT_SMALL) {
-        hipLaunchKernelGGL(lv_evict_small_kernel, dim3((unsigned)(batch * hkv)), dim3(1024), 0, st, p);
+        if (rows <= 4096) hipLaunchKernelGGL(lv_evict_small_kernel<4>, dim3((unsigned)(batch * hkv)), dim3(1024), 0, st, p);
+        else hipLaunchKernelGGL(lv_evict_small_kernel<LV_EVICT_SMALL / 1024>, dim3((unsigned)(batch * hkv)), dim3(1024), 0, st, p);
     } else {
         p.chunks = evict_chunks(rows);
         p.hist = (uint32_t*)workspace;
