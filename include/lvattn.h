@@ -202,15 +202,23 @@ int lvattn_combine_sum(const float* ws, void* out, const int32_t* comb_dev, int 
  *       rows.  piece > 0 (multiple of 64 forward, 32 backward): sweeps cut every `piece` elements, results in workspace rows,
  *       combine entries in comb_host as for lv_build_fwd_blocks_split.  desc_host == NULL only counts.  Returns the count.
  *   lv_plan_score_split    host: the piece length for a launch of these sweeps, 0 = leave them whole.
- *   lvattn_fwd_score / lvattn_bwd_score  as lvattn_fwd / lvattn_bwd on such tables; delta from lvattn_bwd_delta. */
+ *   lvattn_fwd_score / lvattn_bwd_score  as lvattn_fwd / lvattn_bwd on such tables.  out_lo (or NULL) [rows, hq, d] uint8 receives
+ *       the eight mantissa bits that the rounding of out to bf16 cut off; out_f32 != 0: out is fp32, contiguous (the partial results
+ *       of cut sweeps), out_lo NULL.
+ *   lvattn_score_delta      delta[h, row] = sum_d dout * (out with its cut-off byte), fp32 [hq, lse_stride].
+ *   lvattn_score_combine    out / out_lo / lse <- log-sum-exp merge of the pieces' fp32 out [ws_rows, hq, d] and lse, as lvattn_combine_lse. */
 int lv_build_score_blocks(const int32_t* cu_seqlens_host, int n_seg, int causal, int band, const int32_t* prefix_host, int backward, int piece,
                           int32_t* desc_host, int max_blocks, int32_t* comb_host, int max_comb, int* n_comb, int* ws_rows);
 int lv_plan_score_split(const int32_t* cu_seqlens_host, int n_seg, int causal, int band, const int32_t* prefix_host, int backward, int hq, int hkv,
                         int n_cu);
-int lvattn_fwd_score(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* desc_dev, int n_blocks,
+int lvattn_fwd_score(const void* q, const void* k, const void* v, void* out, uint8_t* out_lo, int out_f32, float* lse, const int32_t* desc_dev, int n_blocks,
                      int q_rows_total, int k_rows_total, int hq, int hkv, int d, int64_t q_row_stride, int64_t q_head_stride,
                      int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride, int64_t o_row_stride,
                      int64_t o_head_stride, int64_t lse_stride, float softmax_scale, float softcap, const float* slopes, void* stream);
+int lvattn_score_delta(const void* out, const uint8_t* out_lo, const void* dout, float* delta, int rows, int hq, int d, int64_t o_row_stride,
+                       int64_t o_head_stride, int64_t do_row_stride, int64_t do_head_stride, int64_t lse_stride, void* stream);
+int lvattn_score_combine(const float* ws_out, const float* ws_lse, void* out, uint8_t* out_lo, float* lse, const int32_t* comb_dev, int n_comb,
+                         int hq, int d, int64_t ws_lse_stride, int64_t o_row_stride, int64_t o_head_stride, int64_t lse_stride, void* stream);
 int lvattn_bwd_score(const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dq, void* dk,
                      void* dv, const int32_t* qdesc_dev, int n_qblocks, const int32_t* kdesc_dev, int n_kblocks, int q_rows_total,
                      int k_rows_total, int hq, int hkv, int d, int64_t q_row_stride, int64_t q_head_stride, int64_t k_row_stride,

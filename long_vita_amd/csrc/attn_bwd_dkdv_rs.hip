@@ -302,7 +302,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
             for (int g = 0; g < 4; ++g) {
                 f32x4 t4 = *(LDS_PTR(f32x4, ld_ptr + sbx + 32 * g));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) cst[u][g][e] = t4[e] * cmul;
+                for (int e = 0; e < 4; ++e) cst[u][g][e] = MOD != 0 ? __builtin_fmaf(t4[e], cmul, is_k ? 0.f : 15.f) : t4[e] * cmul;
             }
         };
 #pragma unroll
@@ -368,17 +368,30 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
                     }
 #pragma unroll
                     for (int i = 0; i < 16; ++i) y[u][i >> 3][i & 7] = (__bf16)pv[i];
-                    if constexpr ((MOD & LV_SCORE_CAP) != 0) {   // the partner forms dS = P (1 - tanh^2) (dP - delta): it gets the first two factors
-                        bf16x8 z[2];
+                    if constexpr (MOD != 0) {
+                        // P travels to the partner as 2^15 P in fp16 (P <= 1: up to 2^15, and down to 2^-29 with the full 11 bits),
+                        // so that dS = P (1 - tanh^2) (dP - delta) is rounded to bf16 once and not twice; with a cap the first two
+                        // factors are multiplied here.  Rounded towards zero, the form that packs two: within 2^-10.
+                        u32x4 z[2];
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) z[i >> 3][i & 7] = (__bf16)(pv[i] * x[u][i]);
-                        *(LDS_PTR(bf16x8, p_ptr + u * PBUF)) = z[0];
-                        *(LDS_PTR(bf16x8, p_ptr + u * PBUF + 1024)) = z[1];
+                        for (int i = 0; i < 16; i += 2) {
+                            const float a = (MOD & LV_SCORE_CAP) != 0 ? pv[i] * x[u][i] : pv[i], b = (MOD & LV_SCORE_CAP) != 0 ? pv[i + 1] * x[u][i + 1] : pv[i + 1];
+                            z[i >> 3][(i & 7) >> 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+                        }
+                        *(LDS_PTR(u32x4, p_ptr + u * PBUF)) = z[0];
+                        *(LDS_PTR(u32x4, p_ptr + u * PBUF + 1024)) = z[1];
                     } else {
                     *(LDS_PTR(bf16x8, p_ptr + u * PBUF)) = y[u][0];
                     *(LDS_PTR(bf16x8, p_ptr + u * PBUF + 1024)) = y[u][1];
                     }
                 } else {
+                    if constexpr (MOD != 0) {
+                        f16x8 pf[2];
+                        pf[0] = *(LDS_PTR(f16x8, p_ptr + u * PBUF));
+                        pf[1] = *(LDS_PTR(f16x8, p_ptr + u * PBUF + 1024));
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) y[u][i >> 3][i & 7] = (__bf16)((float)pf[i >> 3][i & 7] * (x[u][i] + cst[u][i >> 2][i & 3]));
+                    } else {
                     bf16x8 pf[2];
                     pf[0] = *(LDS_PTR(bf16x8, p_ptr + u * PBUF));
                     pf[1] = *(LDS_PTR(bf16x8, p_ptr + u * PBUF + 1024));
@@ -389,6 +402,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
 #else
                         y[u][i >> 3][i & 7] = (__bf16)((float)pf[i >> 3][i & 7] * (x[u][i] + cst[u][i >> 2][i & 3]));  // (bf16 -> f32 is exact)
 #endif
+                    }
                 }
                 asm volatile("" : "+v"(y[u][0]), "+v"(y[u][1]));  // Y is formed here, not next to its first use
             }
@@ -481,7 +495,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
     // ---- epilogue: accumulators (key on the lane) -> rows of dv (V-wave) or dk (K-wave, times scale)
     if (kj < k_rows) {
         const int64_t grow = k_row0 + dsc.out_delta + kj;
-        const float f = is_k ? p.scale : 1.f;
+        const float f = (is_k ? p.scale : 1.f) * (MOD != 0 ? 0x1p-15f : 1.f);
         void* const gbase = is_k ? p.dk : p.dv;
         const int64_t g_rs = is_k ? p.dk_rs : p.dv_rs, g_hs = is_k ? p.dk_hs : p.dv_hs;
 #pragma unroll

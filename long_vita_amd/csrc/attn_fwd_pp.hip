@@ -403,7 +403,27 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
     const float l_tot = pair32_sum(l_run);
     const bool live = (qi < q_rows);
     const float inv = (l_tot > 0.f) ? 1.f / l_tot : 0.f;
+    if constexpr (MOD != 0) {
+        if (live && (p.o_f32 || p.o_lo)) {
+            const int64_t at = ((int64_t)(q_row0 + dsc.out_delta + qi) * p.hq + head) * D + 4 * h;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int g4 = 0; g4 < 4; ++g4) {
+                    f32x4 v4;
+                    uint32_t lo = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        v4[e] = oacc[mt][4 * g4 + e] * inv;
+                        lo |= lv_low_byte(v4[e]) << (8 * e);
+                    }
+                    if (p.o_f32) *reinterpret_cast<f32x4*>(p.o_f32 + at + 32 * mt + 8 * g4) = v4;
+                    else *reinterpret_cast<uint32_t*>(p.o_lo + at + 32 * mt + 8 * g4) = lo;
+                }
+        }
+    }
     if (live) {
+        if (MOD == 0 || !p.o_f32) {
         __bf16* optr = p.o + (int64_t)(q_row0 + dsc.out_delta + qi) * p.o_rs + (int64_t)head * p.o_hs;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -414,6 +434,7 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
                 for (int e = 0; e < 4; ++e) ov[e] = (__bf16)(oacc[mt][4 * g4 + e] * inv);
                 *reinterpret_cast<bf16x4*>(optr + 32 * mt + 8 * g4 + 4 * h) = ov;
             }
+        }
         if (h == 0) {
             const float unit = MOD != 0 ? 0.6931471805599453f : p.scale;
             float lse = (l_tot > 0.f) ? (m_run * unit + __logf(l_tot)) : -INFINITY;

@@ -154,19 +154,116 @@ extern "C" int lv_plan_score_split(const int32_t* cu, int n_seg, int causal, int
     }
 }
 
-extern "C" int lvattn_fwd_score(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* desc_dev, int n_blocks,
+// delta = rowsum dO O with O to 16 bits of mantissa (out + its cut-off byte): dS = P (dP - delta) takes the difference of two
+// numbers that a rounding of O to bf16 alone would move by more than dS's own rounding.  D / 8 threads per (row, head).
+template <int D>
+__global__ __launch_bounds__(256) void lv_score_delta_kernel(const __bf16* __restrict__ o, const uint8_t* __restrict__ o_lo, const __bf16* __restrict__ dout,
+                                                             float* __restrict__ delta, int64_t total, int hq, int64_t o_rs, int64_t o_hs,
+                                                             int64_t do_rs, int64_t do_hs, int64_t lse_stride) {
+    constexpr int CPR = D / 8;
+    const int64_t idx = blockIdx.x * 256ll + threadIdx.x, at = idx < total ? idx : total - 1;
+    const int ch = (int)(at % CPR);
+    const int64_t rh = at / CPR, row = rh / hq;
+    const int head = (int)(rh % hq);
+    const u32x4 a = *reinterpret_cast<const u32x4*>(o + row * o_rs + (int64_t)head * o_hs + ch * 8);
+    const u32x2 lo = *reinterpret_cast<const u32x2*>(o_lo + at * 8);
+    const bf16x8 b = *reinterpret_cast<const bf16x8*>(dout + row * do_rs + (int64_t)head * do_hs + ch * 8);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        s += lv_join_low((a[i >> 1] >> (16 * (i & 1))) & 0xffffu, (lo[i >> 2] >> (8 * (i & 3))) & 0xffu) * (float)b[i];
+#pragma unroll
+    for (int off = CPR / 2; off > 0; off >>= 1) s += __shfl_xor(s, off);
+    if (ch == 0 && idx < total) delta[(int64_t)head * lse_stride + row] = s;
+}
+
+// out / lse / cut-off bytes of a row = the log-sum-exp merge of its block's pieces, first piece first, from fp32 partials
+template <int D>
+__global__ __launch_bounds__(256) void lv_score_combine_kernel(const float* __restrict__ ws_out, const float* __restrict__ ws_lse, __bf16* __restrict__ out,
+                                                               uint8_t* __restrict__ out_lo, float* __restrict__ lse, const int32_t* __restrict__ comb,
+                                                               int hq, int64_t ws_lse_stride, int64_t o_rs, int64_t o_hs, int64_t lse_stride) {
+    constexpr int ROWS = 32, CPR = D / 8;
+    const int e = blockIdx.x / (kFwdRows / ROWS), head = blockIdx.y;
+    const int out_row0 = comb[4 * e], rows = comb[4 * e + 1], ws_row0 = comb[4 * e + 2], np = comb[4 * e + 3];
+    const int r0 = blockIdx.x % (kFwdRows / ROWS) * ROWS, r1 = min(rows, r0 + ROWS);
+    for (int idx = threadIdx.x; idx < (r1 - r0) * CPR; idx += 256) {
+        const int row = r0 + idx / CPR, ch = idx % CPR;
+        const float* lp = ws_lse + (int64_t)head * ws_lse_stride + ws_row0 + row;
+        float m = -INFINITY;
+        for (int p = 0; p < np; ++p) m = fmaxf(m, lp[(int64_t)p * kFwdRows]);
+        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, tot = 0.f;
+        if (m > -INFINITY)
+            for (int p = 0; p < np; ++p) {
+                const float w = __expf(lp[(int64_t)p * kFwdRows] - m);
+                const float* src = ws_out + ((ws_row0 + (int64_t)p * kFwdRows + row) * hq + head) * D + ch * 8;
+                const f32x4 a = *reinterpret_cast<const f32x4*>(src), b = *reinterpret_cast<const f32x4*>(src + 4);
+                tot += w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { acc[i] += w * a[i]; acc[4 + i] += w * b[i]; }
+            }
+        const float inv = tot > 0.f ? 1.f / tot : 0.f;
+        bf16x8 o;
+        u32x2 lo = {0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = acc[i] * inv;
+            o[i] = (__bf16)x;
+            lo[i >> 2] |= lv_low_byte(x) << (8 * (i & 3));
+        }
+        *reinterpret_cast<bf16x8*>(out + (int64_t)(out_row0 + row) * o_rs + (int64_t)head * o_hs + ch * 8) = o;
+        if (out_lo) *reinterpret_cast<u32x2*>(out_lo + ((int64_t)(out_row0 + row) * hq + head) * D + ch * 8) = lo;
+        if (ch == 0) lse[(int64_t)head * lse_stride + out_row0 + row] = tot > 0.f ? m + __logf(tot) : -INFINITY;
+    }
+}
+
+extern "C" int lvattn_score_delta(const void* out, const uint8_t* out_lo, const void* dout, float* delta, int rows, int hq, int d, int64_t o_rs, int64_t o_hs,
+                                  int64_t do_rs, int64_t do_hs, int64_t lse_stride, void* stream) {
+    if (!out || !out_lo || !dout || !delta) return lv_fail(LV_EINVAL, "lvattn_score_delta: null pointer");
+    if (d != 64 && d != 128) return lv_fail(LV_EINVAL, "head dim %d not supported (64 or 128)", d);
+    if ((((uintptr_t)out | (uintptr_t)dout) & 15) || ((uintptr_t)out_lo & 7)) return lv_fail(LV_EINVAL, "lvattn_score_delta: out / dout must be 16-byte, out_lo 8-byte aligned");
+    if ((o_rs | o_hs | do_rs | do_hs) & 7) return lv_fail(LV_EINVAL, "strides must be multiples of 8 elements");
+    if (rows < 0 || hq <= 0 || lse_stride < rows) return lv_fail(LV_EINVAL, "bad sizes");
+    if (rows == 0) return LV_OK;
+    const int64_t total = (int64_t)rows * hq * (d / 8), grid = (total + 255) / 256;
+    if (grid > 0x7fffffffLL) return lv_fail(LV_EINVAL, "grid too large");
+    if (d == 128) hipLaunchKernelGGL(lv_score_delta_kernel<128>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, (const __bf16*)out, out_lo, (const __bf16*)dout,
+                                     delta, total, hq, o_rs, o_hs, do_rs, do_hs, lse_stride);
+    else hipLaunchKernelGGL(lv_score_delta_kernel<64>, dim3((unsigned)grid), dim3(256), 0, (hipStream_t)stream, (const __bf16*)out, out_lo, (const __bf16*)dout,
+                            delta, total, hq, o_rs, o_hs, do_rs, do_hs, lse_stride);
+    return hipGetLastError() == hipSuccess ? LV_OK : lv_fail(LV_ELAUNCH, "delta launch failed");
+}
+
+extern "C" int lvattn_score_combine(const float* ws_out, const float* ws_lse, void* out, uint8_t* out_lo, float* lse, const int32_t* comb_dev, int n_comb,
+                                    int hq, int d, int64_t ws_lse_stride, int64_t o_rs, int64_t o_hs, int64_t lse_stride, void* stream) {
+    if (!ws_out || !ws_lse || !out || !lse || !comb_dev) return lv_fail(LV_EINVAL, "lvattn_score_combine: null pointer");
+    if (n_comb < 0 || hq <= 0 || hq > 65535 || (d != 64 && d != 128) || ((o_rs | o_hs) & 7) || (((uintptr_t)ws_out | (uintptr_t)out) & 15) || ((uintptr_t)out_lo & 7))
+        return lv_fail(LV_EINVAL, "lvattn_score_combine: sizes, strides or alignment");
+    if ((int64_t)n_comb * 8 > 0x7fffffffLL) return lv_fail(LV_EINVAL, "grid too large");
+    if (n_comb == 0) return LV_OK;
+    const dim3 grid((unsigned)(n_comb * (kFwdRows / 32)), (unsigned)hq);
+    if (d == 128) hipLaunchKernelGGL(lv_score_combine_kernel<128>, grid, dim3(256), 0, (hipStream_t)stream, ws_out, ws_lse, (__bf16*)out, out_lo, lse, comb_dev, hq,
+                                     ws_lse_stride, o_rs, o_hs, lse_stride);
+    else hipLaunchKernelGGL(lv_score_combine_kernel<64>, grid, dim3(256), 0, (hipStream_t)stream, ws_out, ws_lse, (__bf16*)out, out_lo, lse, comb_dev, hq, ws_lse_stride,
+                            o_rs, o_hs, lse_stride);
+    return hipGetLastError() == hipSuccess ? LV_OK : lv_fail(LV_ELAUNCH, "combine launch failed");
+}
+
+extern "C" int lvattn_fwd_score(const void* q, const void* k, const void* v, void* out, uint8_t* out_lo, int out_f32, float* lse, const int32_t* desc_dev, int n_blocks,
                                 int q_rows_total, int k_rows_total, int hq, int hkv, int d, int64_t q_rs, int64_t q_hs, int64_t k_rs, int64_t k_hs,
                                 int64_t v_rs, int64_t v_hs, int64_t o_rs, int64_t o_hs, int64_t lse_stride, float softmax_scale, float softcap,
                                 const float* slopes, void* stream) {
     if (int e = lv_check_qkv(q, k, v, hq, hkv, d, q_rs, q_hs, k_rs, k_hs, v_rs, v_hs)) return e;
     if (int e = check_rule(d, hq, hkv, softmax_scale, softcap, slopes)) return e;
     if (!out || !lse || !desc_dev) return lv_fail(LV_EINVAL, "null out/lse/desc pointer");
-    if (((uintptr_t)out & 7) || (o_rs & 3) || (o_hs & 3)) return lv_fail(LV_EINVAL, "out must be 8-byte aligned with strides %% 4 == 0");
+    if (((uintptr_t)out & (out_f32 ? 15 : 7)) || (o_rs & 3) || (o_hs & 3)) return lv_fail(LV_EINVAL, "out must be 8-byte (fp32: 16-byte) aligned with strides %% 4 == 0");
+    if (out_f32 && (out_lo || o_hs != d || o_rs != (int64_t)hq * d)) return lv_fail(LV_EINVAL, "fp32 results are contiguous and have no cut-off bytes");
+    if ((uintptr_t)out_lo & 3) return lv_fail(LV_EINVAL, "out_lo must be 4-byte aligned");
     if (n_blocks < 0 || q_rows_total <= 0 || k_rows_total <= 0) return lv_fail(LV_EINVAL, "bad sizes");
     if (n_blocks == 0) return LV_OK;
     if ((int64_t)n_blocks * hq > 0x7fffffffLL) return lv_fail(LV_EINVAL, "grid too large");
     FwdParams p{};
     p.q = (const __bf16*)q; p.k = (const __bf16*)k; p.v = (const __bf16*)v; p.o = (__bf16*)out; p.lse = lse;
+    p.o_f32 = out_f32 ? (float*)out : nullptr; p.o_lo = out_lo;
     p.desc = (const AttnDesc*)desc_dev;
     p.n_blocks = n_blocks; p.hq = hq; p.hkv = hkv; p.group = hq / hkv;
     p.q_rows_total = q_rows_total; p.k_rows_total = k_rows_total;

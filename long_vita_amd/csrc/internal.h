@@ -54,8 +54,21 @@ struct FwdParams {
     int rope_tab_div;
     __bf16* q_rot;
     int64_t qr_rs, qr_hs;
-    ScoreRule score;    // read by the MOD != 0 kernels only
+    ScoreRule score;    // read by the MOD != 0 kernels only, as are the two below
+    float* o_f32;       // not null: results go here, unrounded, [rows][hq][d] contiguous, instead of o
+    uint8_t* o_lo;      // not null: what the rounding of o cut off, [rows][hq][d] contiguous (lv_low_byte)
 };
+// An fp32 number as its bf16 rounding plus one byte: the eight bits below the bf16 mantissa, before the rounding.  The tie that
+// rounds down would read like one that rounds up; it is stored a step lower.  lv_join_low gives back 16 bits of mantissa.
+#ifdef __HIPCC__
+__device__ __forceinline__ uint32_t lv_low_byte(float x) {
+    const uint32_t u = __float_as_uint(x), b = (u >> 8) & 0xffu;
+    return b - ((u & 0x1ffffu) == 0x8000u ? 1u : 0u);
+}
+__device__ __forceinline__ float lv_join_low(uint32_t bf16_bits, uint32_t b) {
+    return __uint_as_float(((bf16_bits - (b >> 7)) << 16) | (b << 8) | 0x80u);
+}
+#endif
 // Workgroup i of a launch runs on XCD i % 8, and every XCD has its own L2.  When ALL the work items of one KV head
 // (query blocks x the group's query heads) fit on an XCD's 32 CUs at once, they are given consecutive slots of one XCD:
 // the head's K / V then come into that L2 once instead of once per XCD that hosts one of its items (the vision

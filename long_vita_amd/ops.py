@@ -881,12 +881,12 @@ class _ScoreRule:
         return _blocks.get(("score", self.key, bool(backward), int(piece), str(device)), build)
 
 
-def _score_fwd_launch(q, k, v, tables, rule, slopes, scale, out, lse):
+def _score_fwd_launch(q, k, v, tables, rule, slopes, scale, out, lse, out_lo=None):
     rq, hq, d = q.shape
     check(_lib.lib().lvattn_fwd_score(
-        _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(tables.desc), tables.desc.shape[0], rq, k.shape[0], hq, k.shape[1], d,
-        q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1), out.stride(0), out.stride(1), lse.stride(0),
-        float(scale), float(rule.softcap), _ptr(slopes), _stream()), "lvattn_fwd_score")
+        _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(out_lo), int(out.dtype == torch.float32), _ptr(lse), _ptr(tables.desc), tables.desc.shape[0],
+        rq, k.shape[0], hq, k.shape[1], d, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+        out.stride(0), out.stride(1), lse.stride(0), float(scale), float(rule.softcap), _ptr(slopes), _stream()), "lvattn_fwd_score")
 
 
 def _score_bwd_launch(q, k, v, dout, lse, delta, tq, tk, rule, slopes, scale, dq, dk, dv, accum_f32):
@@ -918,16 +918,19 @@ class _ScoreAttention(torch.autograd.Function):
         lse = torch.empty((hq, total), dtype=torch.float32, device=dev)
         if not covered:
             lse.fill_(float("-inf"))
+        # for the backward pass: the byte of every output's mantissa that its rounding cut off (lvattn_score_delta)
+        out_lo = (torch.empty if covered else torch.zeros)((total, hq, d), dtype=torch.uint8, device=dev) if any(ctx.needs_input_grad) else None
         if rule.cu[-1] > rule.cu[0]:
             t = rule.tables(False, pieces[0], dev)
             if pieces[0]:
-                ws_out = torch.empty((t.ws_rows, hq, d), dtype=torch.bfloat16, device=dev)
-                ws_lse = torch.empty((hq, t.ws_rows), dtype=torch.float32, device=dev)
+                ws_out = _workspace((t.ws_rows, hq, d), dev)
+                ws_lse = _workspace((hq, t.ws_rows), dev)
                 _score_fwd_launch(q, k, v, t, rule, slopes, scale, ws_out, ws_lse)
-                combine_lse_launch(ws_out, ws_lse, out, lse, t)
+                check(_lib.lib().lvattn_score_combine(_ptr(ws_out), _ptr(ws_lse), _ptr(out), _ptr(out_lo), _ptr(lse), _ptr(t.comb), t.comb.shape[0], hq, d,
+                                                      ws_lse.stride(0), out.stride(0), out.stride(1), lse.stride(0), _stream()), "lvattn_score_combine")
             else:
-                _score_fwd_launch(q, k, v, t, rule, slopes, scale, out, lse)
-        ctx.save_for_backward(q, k, v, out, lse, slopes)
+                _score_fwd_launch(q, k, v, t, rule, slopes, scale, out, lse, out_lo)
+        ctx.save_for_backward(q, k, v, out, lse, slopes, out_lo)
         ctx.rule, ctx.scale, ctx.pieces, ctx.covered = rule, scale, pieces, covered
         ctx.mark_non_differentiable(lse)
         return out, lse
@@ -935,7 +938,7 @@ class _ScoreAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _dlse):
-        q, k, v, out, lse, slopes = ctx.saved_tensors
+        q, k, v, out, lse, slopes, out_lo = ctx.saved_tensors
         _require_gpu(q, dout)
         rule = ctx.rule
         rq, hq, d = q.shape
@@ -945,8 +948,8 @@ class _ScoreAttention(torch.autograd.Function):
             return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), None, None, None
         dout = _rows(dout)
         delta = torch.empty((hq, rq), dtype=torch.float32, device=dev)
-        check(_lib.lib().lvattn_bwd_delta(_ptr(out), _ptr(dout), _ptr(delta), rq, hq, d, out.stride(0), out.stride(1),
-                                          dout.stride(0), dout.stride(1), delta.stride(0), _stream()), "lvattn_bwd_delta")
+        check(_lib.lib().lvattn_score_delta(_ptr(out), _ptr(out_lo), _ptr(dout), _ptr(delta), rq, hq, d, out.stride(0), out.stride(1),
+                                            dout.stride(0), dout.stride(1), delta.stride(0), _stream()), "lvattn_score_delta")
         make = torch.empty if ctx.covered else torch.zeros       # rows no segment covers get a zero gradient
         dq = make((rq, hq, d), dtype=torch.bfloat16, device=dev)
         dk, dv = (make((rq, hkv, d), dtype=torch.bfloat16, device=dev) for _ in range(2))

@@ -110,7 +110,7 @@ def test_plan_cuts_few_long_sweeps_only():
 def test_entry_points_refuse_bad_rules():
     L = _lib.lib()
     ones = [16] * 3
-    common = [16, 16, 16, 1, 8, 8, 4, 2, 64] + [256, 64] * 4 + [8]
+    common = [16, None, 0, 16, 16, 1, 8, 8, 4, 2, 64] + [256, 64] * 4 + [8]
     assert L.lvattn_fwd_score(*ones, *common, 1.0, -1.0, None, None) == -1 and b"softcap" in L.lvattn_last_error()
     assert L.lvattn_fwd_score(*ones, *common, 1.0, float("nan"), None, None) == -1
     assert L.lvattn_fwd_score(*ones, *common, float("inf"), 0.0, None, None) == -1 and b"softmax_scale" in L.lvattn_last_error()
