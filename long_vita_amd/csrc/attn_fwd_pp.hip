@@ -176,16 +176,21 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
         voff_full[j] = row * (int)(x_rs * 2) + ch16;
         voff_part[j] = min(row, rows_last - 1) * (int)(x_rs * 2) + ch16;  // rows past the end repeat the last valid one
     }
-    int ld_t = 0;  // next tile to request
+    // A slope makes near keys the likely ones: the tiles are walked from the last to the first, so that the running maximum is found
+    // at once and the optimistic pass below holds from the second tile on (in rising order the maximum grows with every tile).
+    constexpr bool REV = (MOD & LV_SCORE_BIAS) != 0;
+    int ld_t = 0;  // next tile to request, counted from the walk's start
     // slot of K tile t: t % NS; of V tile t: (t + 1) % NS (its V half)
     uint32_t ld_dst = lds_base + (grp_b ? SLOTB + TILEB : 0) + PPW * wg * 1024;
     const uint32_t ld_wrap = lds_base + NS * SLOTB;
     auto issue_tile = [&]() __attribute__((always_inline)) {
-        int rows = rows_avail - ld_t * BN;
+        const int lt = REV ? __builtin_amdgcn_readfirstlane(max(nkt - 1 - ld_t, 0)) : ld_t;
+        int rows = REV && ld_t >= nkt ? 0 : rows_avail - lt * BN;
+        if constexpr (REV) rows = __builtin_amdgcn_readfirstlane(rows);
         rows = rows < 0 ? 0 : (rows > BN ? BN : rows);
         // tiles past the end of the key range: zero records, every lane out of range, nothing fetched
         const uint32_t rec = rows ? (uint32_t)((rows - 1) * x_rs * 2 + ROWB) : 0u;
-        auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(xbase + ld_t * x_tile_bytes), 0, rec, 0x00020000);
+        auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(xbase + lt * x_tile_bytes), 0, rec, 0x00020000);
         const bool partial = rows < BN;
 #pragma unroll
         for (int j = 0; j < PPW; ++j) pp_dma16(rs, partial ? voff_part[j] : voff_full[j], ld_dst + j * 1024);
@@ -212,10 +217,24 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
         for (int i = 0; i < 16; ++i) oacc[mt][i] = 0.f;
     float m_run = -1e30f, l_run = 0.f;
     const float c = MOD != 0 ? 1.f : p.scale_log2e;   // (MOD: the scores become t, in log2 units, before the softmax sees them)
+    // MOD: t = x * t_mul + t_add per sub-tile, with x what the matrix product left (a cap alone: the rational part of its tanh).
+    // A slope without a cap: on the tiles before the row (distance fq - key >= 0) the bias is linear in the key, so its part inside
+    // the tile, the same in every tile and sub-tile, is the value that the accumulators start from, and the rest is t_add: no
+    // instruction per score.  With the order of tiles below: 2430 -> 1690 us for 12288 causal rows of 40 / 8 heads, 920 TFLOP/s.
+    constexpr bool SLOPE_INIT = (MOD & LV_SCORE_BIAS) != 0 && (MOD & LV_SCORE_CAP) == 0;
     float nslope2 = 0.f;
+    f32x16 bias0;
     if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
         nslope2 = -1.4426950408889634f * p.score.slopes[head];
         asm volatile("" : "+v"(nslope2));
+        if constexpr (SLOPE_INIT) {
+            const float raw = -nslope2 / p.scale_log2e;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                bias0[i] = raw * (float)((i & 3) + 8 * (i >> 2));
+                asm volatile("" : "+v"(bias0[i]));
+            }
+        }
     }
     f32x16 s[2];
     bf16x8 pf[2][2];
@@ -228,7 +247,7 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[st][i] = 0.f;
+            for (int i = 0; i < 16; ++i) s[st][i] = SLOPE_INIT ? bias0[i] : 0.f;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 bf16x8 kf = *(LDS_PTR(bf16x8, k_ptr[ks] + sb + st * 32 * ROWB));
@@ -247,16 +266,34 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
         if (grp_b) asm volatile("s_barrier" ::: "memory");
         for (int t = 0; t < nkt; ++t) {
             // ================= VALU(t): softmax of S_t -> P_t =================
-            if (t < my_nkt) {
-                const int kb0 = t * BN;
+            const int tt = REV ? nkt - 1 - t : t;
+            if (tt < my_nkt) {
+                const int kb0 = tt * BN;
                 const bool need_mask = (kb0 + BN - 1 > (MOD != 0 ? max(32 * w + shift, dsc.prefix - 1) : 32 * w + shift)) || (kb0 + BN > k_len) || (kb0 < 32 * w + 31 + band_low);
+                float t_mul = 1.f, t_add[2] = {0.f, 0.f};
                 if constexpr (MOD != 0) {
                     const float fq = (float)(qi + shift - kb0 - 4 * h);   // distance of the row to the lane's first key of the tile
+                    if constexpr (MOD == LV_SCORE_RULE) {
+                        t_mul = p.scale_log2e;
+                    } else if constexpr ((MOD & LV_SCORE_BIAS) == 0) {
 #pragma unroll
-                    for (int st = 0; st < 2; ++st)
+                        for (int st = 0; st < 2; ++st)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            s[st][i] = lv_score<MOD>(s[st][i], p.scale_log2e, p.score, nslope2, fq - (float)(32 * st + (i & 3) + 8 * (i >> 2)));
+                            for (int i = 0; i < 16; ++i) s[st][i] = __builtin_amdgcn_rcpf(fast_exp2(s[st][i] * p.score.cap_in) + 1.f);
+                        t_mul = -2.f * p.score.cap_out;
+                        t_add[0] = t_add[1] = p.score.cap_out;
+                    } else if (SLOPE_INIT && kb0 + BN - 1 <= 32 * w + shift) {
+                        t_mul = p.scale_log2e;
+                        t_add[0] = nslope2 * fq;
+                        t_add[1] = nslope2 * (fq - 32.f);
+                    } else {
+#pragma unroll
+                        for (int st = 0; st < 2; ++st)
+#pragma unroll
+                            for (int i = 0; i < 16; ++i)
+                                s[st][i] = lv_score<MOD>(SLOPE_INIT ? s[st][i] - bias0[i] : s[st][i], p.scale_log2e, p.score, nslope2,
+                                                         fq - (float)(32 * st + (i & 3) + 8 * (i >> 2)));
+                    }
                 }
                 // Optimistic pass: once every row of the wave has a finite running maximum, P is formed
                 // against it WITHOUT looking for the tile's maximum first (a third of the softmax's
@@ -270,7 +307,7 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
                     for (int st = 0; st < 2; ++st)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            float pv = fast_exp2(__builtin_fmaf(s[st][i], c, -mc));
+                            float pv = fast_exp2(MOD != 0 ? __builtin_fmaf(s[st][i], t_mul, t_add[st] - mc) : __builtin_fmaf(s[st][i], c, -mc));
                             rs += pv;
                             pf[st][i >> 3][i & 7] = (__bf16)pv;
                         }
@@ -278,6 +315,12 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
                     else l_run += rs;
                 }
                 if (exact) {
+                if constexpr (MOD != 0) {
+#pragma unroll
+                    for (int st = 0; st < 2; ++st)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) s[st][i] = __builtin_fmaf(s[st][i], t_mul, t_add[st]);
+                }
                 if (need_mask) {
 #pragma unroll
                     for (int st = 0; st < 2; ++st)
@@ -365,7 +408,7 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
                 if (g < 3) load_group(g + 1, set ^ 1);
                 if (s2 == 0) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s[st][i] = 0.f;
+                    for (int i = 0; i < 16; ++i) s[st][i] = SLOPE_INIT ? bias0[i] : 0.f;
                 }
 #pragma unroll
                 for (int i = 0; i < MPG; ++i) {
