@@ -18,6 +18,7 @@
 #include "cache_list.h"
 #include "../../include/lvattn.h"
 
+#include <algorithm>
 #include <type_traits>
 
 // [slots of K / V tiles][cum][lens][par][depth][anc][stat]
@@ -31,6 +32,9 @@ struct TreeShape {
     static constexpr int TILE = 32 * WK * SUB;    // keys per tile: 128
     static_assert(TILE == 128, "tree_plan counts tiles of 128 keys");
     static constexpr int THREADS = 64 * WR * WK;
+    // tiles that taking up another sequence costs (list_scan); 0 / 3 / 5 / 8 measured: 77 / 65 / 63 / 62 us for 25 tokens of 8
+    // sequences of 0 to 16K keys, 111 / 107 / 108 / 112 us for 8 tokens of 16 sequences of 40 to 30K
+    static constexpr int LEAD = WR == 4 ? 5 : 3;
     template <int D> static constexpr int slot_bytes() { return TILE * 2 * D * 2; }       // a tile of K and V
     template <int D> static constexpr int slots() { return WR == 4 ? 2 : (LV_TREE_RING / slot_bytes<D>() > 4 ? 4 : LV_TREE_RING / slot_bytes<D>()); }
     template <int D> static constexpr int lds_bytes() { return slots<D>() * slot_bytes<D>() + LV_TREE_LDS_FIXED; }
@@ -84,7 +88,8 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
     if (unit >= p.hkv * p.shares) return;
     const int kvh = unit % p.hkv, g = unit / p.hkv;
 
-    list_scan<BN>(p.cache_lens, p.batch, p.rows, p.n, cum, lens);
+    constexpr int LEAD = TreeShape<WR>::LEAD;
+    list_scan<BN, LEAD>(p.cache_lens, p.batch, p.rows, p.n, cum, lens);
     const ListDeal deal(p.shares, __builtin_amdgcn_readfirstlane(cum[p.batch - 1]));
     if (g >= (int)deal.G) return;
     int tile = __builtin_amdgcn_readfirstlane(deal.first(g));
@@ -161,8 +166,10 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
     while (tile < tile_end) {
         // ---------------- one sequence of this share ----------------
         const int len = __builtin_amdgcn_readfirstlane(lens[s]), keys = len + p.n;
-        const int list0 = s ? __builtin_amdgcn_readfirstlane(cum[s - 1]) : 0;
+        const int list0 = (s ? __builtin_amdgcn_readfirstlane(cum[s - 1]) : 0) + list_lead<LEAD>(s);
+        tile = max(tile, list0);
         const int t0 = tile - list0, t1 = min(tile_end, __builtin_amdgcn_readfirstlane(cum[s])) - list0;
+        if (t1 <= t0) break;              // the share ends ahead of the sequence's first tile
         const bool sees_tree = t1 * BN > len;
 
         // WR = 1 asks for tile t + NS when its own slot is free, WR = 2 for tile t + NS - 1 behind the barrier of tile t, the
@@ -443,7 +450,15 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
         }
 
         // ---------------- join the key waves; this share's result for the sequence -> partial slot g + s ----------------
+        // (a sequence that is the share's alone is finished here, and the second kernel passes its rows by; WR = 4 has no
+        // registers left for it: a 64-token tree over 131K keys took 231 instead of 226 us)
+        const bool whole = WR < 4 && p.direct && t0 == 0 && list0 + t1 == __builtin_amdgcn_readfirstlane(cum[s]);
         const int64_t part = ((int64_t)(kvh * p.n_rb + rb) * p.slots + g + s) * (32 * WR) + 32 * wr;
+        int row_o = lane & 31;            // (derived anew: not kept in registers through the loop)
+        asm volatile("" : "+v"(row_o));
+        row_o += 32 * (WR * rb + wr);
+        const int rowc_o = min(row_o, n_rows - 1), token_o = rowc_o / p.group, head_o = kvh * p.group + rowc_o % p.group;
+        __bf16* const orow = p.o + (int64_t)s * p.o_bs + (int64_t)token_o * p.o_ns + (int64_t)head_o * p.o_hs;
         const float unit2 = MOD != 0 ? 0.6931471805599453f : p.scale;
         const float l_w = pair32_sum(l_run);
         if (h == 0) {
@@ -461,7 +476,11 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
         for (int i = 0; i < WK; ++i) l_tot += stat[256 + (i * WR + wr) * 32 + r] * fast_exp2((stat[(i * WR + wr) * 32 + r] - m_tot) * c);
         const float sc = fast_exp2((m_run - m_tot) * c);
         const float inv = (l_tot > 0.f && live) ? 1.f / l_tot : 0.f;
-        if (wk == 0 && h == 0) p.part_lse[part + r] = (l_tot > 0.f && live) ? m_tot * unit2 + __logf(l_tot) : -INFINITY;
+        if (wk == 0 && h == 0) {
+            const float x = (l_tot > 0.f && live) ? m_tot * unit2 + __logf(l_tot) : -INFINITY;
+            if (!whole) p.part_lse[part + r] = x;
+            else if (p.lse && row_o < n_rows) p.lse[((int64_t)s * p.n + token_o) * p.hq + head_o] = x;
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -476,7 +495,10 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
                 f32x4 acc = obuf[((wr * MT + mt) * 4 + g4) * 64 + lane];
 #pragma unroll
                 for (int i = 1; i < WK; ++i) acc += obuf[(((i * WR + wr) * MT + mt) * 4 + g4) * 64 + lane];
-                *reinterpret_cast<f32x4*>(p.part_o + (part + r) * D + 32 * mt + 8 * g4 + 4 * h) = inv > 0.f ? acc * inv : f32x4{0.f, 0.f, 0.f, 0.f};
+                acc = inv > 0.f ? acc * inv : f32x4{0.f, 0.f, 0.f, 0.f};
+                const int col = 32 * mt + 8 * g4 + 4 * h;
+                if (!whole) *reinterpret_cast<f32x4*>(p.part_o + (part + r) * D + col) = acc;
+                else if (row_o < n_rows) *reinterpret_cast<bf16x4*>(orow + col) = bf16x4{(__bf16)acc[0], (__bf16)acc[1], (__bf16)acc[2], (__bf16)acc[3]};
             }
         __syncthreads();                  // the next sequence's requests go where obuf is
         ++s;
@@ -495,16 +517,17 @@ __global__ __launch_bounds__(256) void lv_tree_join_kernel(TreeParams p) {
     __shared__ float red[8];
     __shared__ f32x4 osum[GR][TPR];
     const int tid = threadIdx.x, gr = tid / TPR, col = tid % TPR * 4;
-    list_scan<TreeShape<WR>::TILE>(p.cache_lens, p.batch, p.rows, p.n, cum, nullptr);
+    list_scan<TreeShape<WR>::TILE, TreeShape<WR>::LEAD>(p.cache_lens, p.batch, p.rows, p.n, cum, nullptr);
     const ListDeal deal(p.shares, cum[p.batch - 1]);
     const int n_rows = p.n * p.group;
-    const int64_t idx = ONE_ROW ? blockIdx.x : (int64_t)blockIdx.x * GR + gr;     // (sequence, KV head, row)
-    if (idx >= (int64_t)p.batch * p.hkv * n_rows) return;
+    const int64_t total = (int64_t)p.batch * p.hkv * n_rows;
+    for (int64_t idx = ONE_ROW ? blockIdx.x : (int64_t)blockIdx.x * GR + gr; idx < total; idx += ONE_ROW ? total : (int64_t)gridDim.x * GR) {   // (sequence, KV head, row)
     const int row = (int)((uint32_t)idx % n_rows), unit = (int)((uint32_t)idx / n_rows), kvh = unit % p.hkv, s = unit / p.hkv;
-    const int g0 = deal.share_of(s ? cum[s - 1] : 0), g1 = deal.share_of(cum[s] - 1);
+    const int g0 = deal.share_of(s ? cum[s - 1] + list_lead<TreeShape<WR>::LEAD>(s) : 0), g1 = deal.share_of(cum[s] - 1);
     const int rb = row / rows_pb;
     const int64_t part = ((int64_t)(kvh * p.n_rb + rb) * p.slots + g0 + s) * rows_pb + row % rows_pb;
     const int np = g1 - g0 + 1;               // at most shares
+    if (np == 1 && p.direct) continue;        // the share that had the sequence to itself wrote the result (uniform where barriers follow)
     const float* lp = p.part_lse + part;
     const float* po = p.part_o + part * D + col;
     float m = -INFINITY, tot = 0.f;
@@ -554,6 +577,7 @@ __global__ __launch_bounds__(256) void lv_tree_join_kernel(TreeParams p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) op[e] = (__bf16)(acc[e] * inv);
     if (p.lse && col == 0) p.lse[((int64_t)s * p.n + token) * p.hq + head] = tot > 0.f ? m + __logf(tot) : -INFINITY;
+    }
 }
 
 struct TreePlan { int wr, n_rb, shares, slots; int64_t part_rows; };
@@ -587,9 +611,10 @@ static void launch_tree(const TreeParams& p, int mod, unsigned blocks, int64_t o
     }
     if (hipPeekAtLastError() != hipSuccess) return;   // (reported by the caller)
     // a workgroup per row takes the slots side by side; with more rows than the chip holds at once (eight workgroups to a compute
-    // unit) a group of threads walks its row's slots instead, eight or sixteen rows to a workgroup
+    // unit) a group of threads walks its row's slots instead, eight or sixteen rows to a workgroup at a time, and the workgroups
+    // that the chip holds go round the rows (122,880 rows of 256 sequences: the list's lengths are summed 2048 times, not 15,360)
     if (out_rows <= 2048) hipLaunchKernelGGL((lv_tree_join_kernel<D, WR, true>), dim3((unsigned)out_rows), dim3(256), 0, stream, p);
-    else hipLaunchKernelGGL((lv_tree_join_kernel<D, WR, false>), dim3((unsigned)((out_rows * (D / 4) + 255) / 256)), dim3(256), 0, stream, p);
+    else hipLaunchKernelGGL((lv_tree_join_kernel<D, WR, false>), dim3((unsigned)std::min<int64_t>((out_rows * (D / 4) + 255) / 256, 2048)), dim3(256), 0, stream, p);
 }
 
 extern "C" int64_t lvattn_tree_workspace_bytes(int batch, int n, int rows, int hq, int hkv, int d) {
@@ -617,7 +642,7 @@ extern "C" int lvattn_tree(const void* q, const void* k, const void* v, void* ou
     if (workspace_bytes < need) return lv_fail(LV_ESIZE, "lvattn_tree: %lld bytes of workspace needed, room for %lld", (long long)need, (long long)workspace_bytes);
     const int64_t units = (int64_t)hkv * t.shares, blocks = (units + 7) / 8 * 8 * t.n_rb;
     const int64_t join = (int64_t)batch * hkv * n * (hq / hkv);
-    if (blocks > 0x7fffffffLL || join > 0x7fffffffLL || (int64_t)batch * (rows / 128 + 1) > 0x7fffffffLL)
+    if (blocks > 0x7fffffffLL || join > 0x7fffffffLL || (int64_t)batch * (rows / 128 + 16) > 0x7fffffffLL)
         return lv_fail(LV_EINVAL, "lvattn_tree: grid too large");
     TreeParams p{};
     p.q = (const __bf16*)q; p.k = (const __bf16*)k; p.v = (const __bf16*)v; p.o = (__bf16*)out; p.lse = lse;
@@ -625,6 +650,7 @@ extern "C" int lvattn_tree(const void* q, const void* k, const void* v, void* ou
     p.part_o = (float*)workspace; p.part_lse = p.part_o + t.part_rows * d;
     p.batch = batch; p.n = n; p.rows = rows; p.hq = hq; p.hkv = hkv; p.group = hq / hkv;
     p.n_rb = t.n_rb; p.shares = t.shares; p.slots = t.slots;
+    p.direct = t.wr < 4 && !(((uintptr_t)out & 7) || ((o_bs | o_ns | o_hs) & 3));       // results can be stored four columns at a time
     p.q_bs = q_bs; p.q_ns = q_ns; p.q_hs = q_hs; p.k_bs = k_bs; p.k_rs = k_rs; p.k_hs = k_hs; p.v_bs = v_bs; p.v_rs = v_rs; p.v_hs = v_hs;
     p.o_bs = o_bs; p.o_ns = o_ns; p.o_hs = o_hs;
     p.scale = softmax_scale; p.scale_log2e = softmax_scale * 1.4426950408889634f;

@@ -16,15 +16,19 @@ __device__ __forceinline__ int list_lds_off(int row, int chunk) {
 // cached keys of sequence s: never outside the cache, whatever the caller's array says
 __device__ __forceinline__ int list_len(const int32_t* cache_lens, int s, int rows, int n) { return min(max(cache_lens[s], 0), rows - n); }
 
-// cum[s] = tiles of sequences 0 .. s, lens[s] (one wave); returns after a barrier of the whole workgroup
-template <int BN>
+// cum[s] = tiles of sequences 0 .. s, lens[s] (one wave); returns after a barrier of the whole workgroup.  Taking up a sequence
+// costs a workgroup about as much as LEAD tiles (drain, first loads, join); so that no share gets its fair part of the tiles and
+// the restarts on top, every sequence but the first counts LEAD tiles more, ahead of its own: list_lead(s) of them hold no keys.
+template <int LEAD>
+__device__ __forceinline__ int list_lead(int s) { return s ? LEAD : 0; }
+template <int BN, int LEAD>
 __device__ __forceinline__ void list_scan(const int32_t* cache_lens, int batch, int rows, int n, int* cum, int* lens) {
     if (threadIdx.x < 64) {
         const int lane = threadIdx.x;
         int carry = 0;
         for (int s0 = 0; s0 < batch; s0 += 64) {
             const int len = s0 + lane < batch ? list_len(cache_lens, s0 + lane, rows, n) : 0;
-            int x = s0 + lane < batch ? (len + n + BN - 1) / BN : 0;
+            int x = s0 + lane < batch ? (len + n + BN - 1) / BN + list_lead<LEAD>(s0 + lane) : 0;
 #pragma unroll
             for (int off = 1; off < 64; off <<= 1) {
                 const int y = __shfl_up(x, off);

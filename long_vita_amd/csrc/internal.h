@@ -133,7 +133,7 @@ struct TreeParams {
     int64_t parents_bs;
     float* part_o;               // [hkv][n_rb][slots][32 * WR][d]
     float* part_lse;             // the same without d
-    int batch, n, rows, hq, hkv, group, n_rb, shares, slots;
+    int batch, n, rows, hq, hkv, group, n_rb, shares, slots, direct;
     int64_t q_bs, q_ns, q_hs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, o_bs, o_ns, o_hs;
     float scale, scale_log2e;
     ScoreRule score;
