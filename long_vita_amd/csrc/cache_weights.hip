@@ -7,15 +7,16 @@
 // S = Q K^T, with the KEY on the lane (32x32x16 MFMA, A = query rows, B = keys): a key's sum over 32 query rows is a sum over
 // its lane's 16 accumulators.  Nothing is ever summed by atomics.  Two kernels:
 //
-// - up to 64 query rows per KV head (a decode step, a small tree): bound by K's bytes.  The query fragments and the rows'
-//   constants stay in registers, eight waves per workgroup stream K, each its own 32-key slices through its own LDS slots by
+// - up to 128 query rows per KV head (a decode step, a tree): bound by K's bytes.  The query fragments and, with up to 64 rows,
+//   the rows' constants stay in registers, eight waves per workgroup stream K, each its own 32-key slices through its own LDS slots by
 //   direct global -> LDS loads, without a barrier; tiles of all sequences are dealt evenly (cache_list.h).  The old weight of a
 //   key travels with its slice, so w_out is written on the spot.
 // - more rows (a large tree, a prompt): a workgroup holds the fragments of 128 keys in registers and the query rows stream
 //   through an LDS ring of 64-row tiles shared by its four waves, two on each half of the keys, on alternate 32 rows.  A
 //   first small kernel prepares the rows' constants.  When there are fewer key blocks than the chip has room for, the rows
 //   are cut into pieces whose sums are added in order by a last kernel.  8 MFMAs (256 cycles) stand against 16 exponentials,
-//   multiply-adds and adds per 32 x 32 scores, so the vector work bounds it.
+//   multiply-adds and adds per 32 x 32 scores, so the vector work bounds it.  Short sweeps pay for every 128 keys' loads: 125
+//   rows of 16 ragged caches of 107K keys, 8 KV heads, took 192 us this way and take 68 us streamed.
 #include "cache_list.h"
 #include "../../include/lvattn.h"
 
@@ -48,10 +49,11 @@ __global__ __launch_bounds__(256) void lv_weight_copy_kernel(WeightParams p) {
 // up to 32 RT query rows
 // ---------------------------------------------------------------------------
 #define LV_WEIGHT_TILE 256                    // keys per tile: 32 for each of eight waves
+#define LV_WEIGHT_STREAM_ROWS 128
 template <int D> constexpr int weight_slots() { return D == 128 ? 2 : 4; }
 template <int D> constexpr int weight_slot_bytes() { return 32 * D * 2 + 256; }        // a slice of K, the 32 old weights
 template <int D> constexpr int weight_lds_bytes() {
-    return 8 * weight_slots<D>() * weight_slot_bytes<D>() + LV_TREE_MAX_BATCH * 8 + LV_TREE_MAX_TOKENS * 8 + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4 + 4 * 64 * 4;
+    return 8 * weight_slots<D>() * weight_slot_bytes<D>() + LV_TREE_MAX_BATCH * 8 + LV_TREE_MAX_TOKENS * 8 + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4 + 4 * LV_WEIGHT_STREAM_ROWS * 4;
 }
 
 template <int D, int RT, int MOD>
@@ -73,8 +75,9 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
     int* const par = lens + LV_TREE_MAX_BATCH;                          // [LV_TREE_MAX_TOKENS]
     int* const depth = par + LV_TREE_MAX_TOKENS;
     uint32_t* const anc = reinterpret_cast<uint32_t*>(depth + LV_TREE_MAX_TOKENS);
-    float* const rc = reinterpret_cast<float*>(anc + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32));   // [3][64]: constant, position, slope
-    int* const rtok = reinterpret_cast<int*>(rc + 3 * 64);              // [64]: token of a row
+    float* const rc = reinterpret_cast<float*>(anc + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32));   // [3][SR]: constant, position, slope
+    constexpr int SR = LV_WEIGHT_STREAM_ROWS;
+    int* const rtok = reinterpret_cast<int*>(rc + 3 * SR);              // [SR]: token of a row
 
     const int tid = threadIdx.x;
     const int lane = tid & 63;
@@ -138,12 +141,12 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
 
         // query fragments (lane r: row 32 b + r), and the rows' constants in LDS
         __syncthreads();                  // the previous sequence's constants are no longer read
-        if (tid < 64) {
+        if (tid < SR) {
             const int tc = min(tid, n_rows - 1), token = tc / p.group, head = kvh * p.group + tc % p.group;
             rc[tid] = (tid < n_rows && !(p.parents && par[token] == LV_TREE_UNUSED)) ? row_constant(p, s, token, head) : -INFINITY;
             if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
-                rc[64 + tid] = (float)(len + (p.parents ? depth[token] : token));
-                rc[128 + tid] = -1.4426950408889634f * p.score.slopes[head];
+                rc[SR + tid] = (float)(len + (p.parents ? depth[token] : token));
+                rc[2 * SR + tid] = -1.4426950408889634f * p.score.slopes[head];
             }
             rtok[tid] = token;
         }
@@ -175,17 +178,23 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
             // make the wait a little longer than it has to be)
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NS - 1) * (NP + 1)) : "memory");
             if (kb0 < keys) {
-                f32x16 x[RT];
+                // two row tiles' products side by side; four row tiles, whose fragments fill the registers, go one after the other and
+                // read the slice four times
+                constexpr int XT = RT <= 2 ? RT : 1;
+                f32x16 x[XT];
+                auto products = [&](int b0) __attribute__((always_inline)) {
 #pragma unroll
-                for (int b = 0; b < RT; ++b)
+                    for (int b = 0; b < XT; ++b)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) x[b][i] = 0.f;
+                        for (int i = 0; i < 16; ++i) x[b][i] = 0.f;
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    const bf16x8 kf = *(LDS_PTR(bf16x8, kb + k_off[ks]));
+                    for (int ks = 0; ks < KS; ++ks) {
+                        const bf16x8 kf = *(LDS_PTR(bf16x8, kb + k_off[ks]));
 #pragma unroll
-                    for (int b = 0; b < RT; ++b) x[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[b][ks], kf, x[b], 0, 0, 0);
-                }
+                        for (int b = 0; b < XT; ++b) x[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qf[b0 + b][ks], kf, x[b], 0, 0, 0);
+                    }
+                };
+                products(0);
                 const float old = *(LDS_PTR(float, kb + 32 * ROWB + 4 * r));
                 const bool masked = kb0 + 32 > len;
                 const int jt = key - len;
@@ -193,24 +202,31 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
                 if constexpr ((MOD & LV_SCORE_BIAS) != 0)
                     if (p.parents && jt >= 0 && jt < p.n) kpos = (float)(len + depth[jt]);
                 float sum = 0.f;
+                int row_of = 4 * h;       // (with four row tiles the constants are read from LDS every time: the registers are full)
+                if constexpr (RT > 2) asm volatile("" : "+v"(row_of));
 #pragma unroll
                 for (int b = 0; b < RT; ++b) {
+                    if (XT == 1 && b > 0) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        products(b);
+                    }
+                    const f32x16& xb = x[XT == 1 ? 0 : b];
                     float pv[16];
 #pragma unroll
                     for (int q4 = 0; q4 < 4; ++q4) {
-                        const int ar = 32 * b + 8 * q4 + 4 * h;      // rows of accumulators 4 q4 .. + 3
+                        const int ar = 32 * b + 8 * q4 + row_of;     // rows of accumulators 4 q4 .. + 3
                         const f32x4 cc = *reinterpret_cast<const f32x4*>(rc + ar);
                         f32x4 pos = {}, slope = {};
                         if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
-                            pos = *reinterpret_cast<const f32x4*>(rc + 64 + ar);
-                            slope = *reinterpret_cast<const f32x4*>(rc + 128 + ar);
+                            pos = *reinterpret_cast<const f32x4*>(rc + SR + ar);
+                            slope = *reinterpret_cast<const f32x4*>(rc + 2 * SR + ar);
                         }
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const int i = 4 * q4 + e;
                             float t2;
-                            if constexpr (MOD != 0) t2 = lv_score<MOD>(x[b][i], p.scale_log2e, p.score, slope[e], pos[e] - kpos) + cc[e];
-                            else t2 = __builtin_fmaf(x[b][i], p.scale_log2e, cc[e]);
+                            if constexpr (MOD != 0) t2 = lv_score<MOD>(xb[i], p.scale_log2e, p.score, slope[e], pos[e] - kpos) + cc[e];
+                            else t2 = __builtin_fmaf(xb[i], p.scale_log2e, cc[e]);
                             pv[i] = fast_exp2(t2);
                         }
                     }
@@ -218,9 +234,11 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
                         // a chain: row R (token R / group) sees drafted key jt from row jt * group on; a tree's keys are looked up
                         const int first_row = key >= keys ? 0x7fffffff : max(jt, 0) * p.group;
                         const bool look = p.parents && key < keys && jt >= 0;
+                        int row_m = 4 * h;
+                        asm volatile("" : "+v"(row_m));          // (the rows' tokens are looked up here, not kept)
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const int ar = 32 * b + (i & 3) + 8 * (i >> 2) + 4 * h;
+                            const int ar = 32 * b + (i & 3) + 8 * (i >> 2) + row_m;
                             bool vis = ar >= first_row;
                             if (look) vis = (anc[rtok[ar] * words + (jt >> 5)] >> (jt & 31)) & 1;
                             pv[i] = vis ? pv[i] : 0.f;
@@ -542,7 +560,7 @@ struct WeightPlan { bool stream; int shares, pieces, key_blocks, rows_pad; int64
 static WeightPlan weight_plan(int batch, int n, int rows, int hq, int hkv) {
     WeightPlan t{};
     const int n_rows = n * (hq / hkv);
-    t.stream = n_rows <= 64 && n <= LV_TREE_MAX_TOKENS && batch <= LV_TREE_MAX_BATCH;
+    t.stream = n_rows <= LV_WEIGHT_STREAM_ROWS && n <= LV_TREE_MAX_TOKENS && batch <= LV_TREE_MAX_BATCH;
     if (t.stream) {
         const int64_t tiles = (int64_t)batch * ((rows + LV_WEIGHT_TILE - 1) / LV_WEIGHT_TILE);
         int64_t g = 256 / hkv;                // a workgroup's slots fill a compute unit's LDS
@@ -568,7 +586,8 @@ template <int D>
 static void launch_stream(const WeightParams& p, int mod, int rt, unsigned blocks, hipStream_t stream) {
 #define LV_W(M) do { \
         if (rt == 1) hipLaunchKernelGGL((lv_weight_stream_kernel<D, 1, M>), dim3(blocks), dim3(512), weight_lds_bytes<D>(), stream, p); \
-        else hipLaunchKernelGGL((lv_weight_stream_kernel<D, 2, M>), dim3(blocks), dim3(512), weight_lds_bytes<D>(), stream, p); } while (0)
+        else if (rt == 2) hipLaunchKernelGGL((lv_weight_stream_kernel<D, 2, M>), dim3(blocks), dim3(512), weight_lds_bytes<D>(), stream, p); \
+        else hipLaunchKernelGGL((lv_weight_stream_kernel<D, 4, M>), dim3(blocks), dim3(512), weight_lds_bytes<D>(), stream, p); } while (0)
     static_assert(weight_lds_bytes<D>() <= 160 * 1024, "one workgroup per compute unit");
     switch (mod) {
         case 0: LV_W(0); break;
@@ -637,7 +656,7 @@ extern "C" int lv_key_weights(const void* q, const void* k, const float* lse, co
     const int mod = lv_score_mod(softcap, slopes) & (LV_SCORE_CAP | LV_SCORE_BIAS);
     hipStream_t st = (hipStream_t)stream;
     if (t.stream) {
-        const int rt = n * p.group <= 32 ? 1 : 2;
+        const int rt = n * p.group <= 32 ? 1 : (n * p.group <= 64 ? 2 : 4);
         if (w_in != w_out)
             hipLaunchKernelGGL(lv_weight_copy_kernel, dim3((unsigned)((rows + 4095) / 4096), (unsigned)(batch * hkv)), dim3(256), 0, st, p);
         const unsigned blocks = (unsigned)(hkv * t.shares);

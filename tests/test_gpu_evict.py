@@ -59,6 +59,11 @@ W_CASES = [
     ("prompt_cap", [0], 260, 4, 4, 64, False, 0, 25.0, False, False),
     ("prompt_tail", [700, 100], 64, 5, 1, 128, False, 0, None, True, True),
     ("group_40", [150], 3, 40, 1, 64, False, 0, None, False, False),
+    ("rows_128", [600, 33, 256], 32, 4, 1, 128, True, 3, None, False, True),
+    ("rows_128_rule", [300, 70], 25, 5, 1, 128, True, 0, 25.0, True, False),
+    ("rows_129", [255, 128], 43, 3, 1, 128, True, 2, None, False, True),
+    ("tree_long_rows", [400, 90], 100, 5, 1, 64, True, 9, 30.0, True, True),
+    ("batch_60", [(41 * i) % 310 for i in range(60)], 5, 8, 2, 64, True, 0, None, False, False),
 ]
 
 

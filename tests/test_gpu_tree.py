@@ -102,6 +102,9 @@ CASES = [
     ("tree_unused_d128", [500, 127], 20, 5, 1, 128, True, 7, 20.0, True),
     ("tree_edge", [127, 128, 96, 97], 32, 8, 8, 64, True, 0, None, False),
     ("batch_70", [(37 * i) % 300 for i in range(70)], 3, 4, 2, 64, True, 0, None, False),
+    ("batch_50_wide", [(53 * i) % 290 for i in range(50)], 14, 20, 4, 128, True, 2, None, True),
+    ("batch_40_rows_100", [(97 * i) % 400 for i in range(40)], 20, 20, 4, 128, True, 2, 30.0, False),
+    ("batch_one_long", [3, 5000, 0, 40, 7, 2500, 11], 9, 16, 8, 128, True, 0, None, False),
 ]
 
 
@@ -187,6 +190,30 @@ def test_strides_out_workspace_and_views():
     odd = torch.empty(q.numel() + 1, dtype=torch.bfloat16, device="cuda")[1:].view(q.shape)
     odd.copy_(q)
     assert torch.equal(ops.tree_attention(odd, k.cuda(), v.cuda(), L), want)
+
+
+@pytest.mark.parametrize("n,hq,hkv", [(1, 8, 4), (9, 16, 4), (20, 16, 4)])
+def test_many_sequences_one_by_one(n, hq, hkv):
+    """A sequence's result does not depend on the batch around it beyond the order in which its keys are joined, nor on where
+    it is stored: buffers whose rows start at odd elements get the same numbers."""
+    from long_vita_amd import ops
+    lens = [(61 * i) % 500 for i in range(64)]
+    rows, d = max(lens) + n + 3, 128
+    q, k, v = (t.cuda() for t in make(64, n, rows, hq, hkv, d, 5, lens))
+    L = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    out, lse = ops.tree_attention(q, k, v, L, return_lse=True)
+    buf = torch.full((64, n, hq + 1, d + 3), -7.0, dtype=torch.bfloat16, device="cuda")
+    odd = buf[:, :, 1:, 1:d + 1]
+    assert ops.tree_attention(q, k, v, L, out=odd) is odd
+    # rounded once from fp32 in either case; the joins' order of adding moves a sum by a few 2^-24
+    assert torch.allclose(odd.float(), out.float(), rtol=2 ** -7, atol=2 ** -16)
+    buf[:, :, 1:, 1:d + 1] = -7.0
+    assert bool((buf == -7.0).all())
+    for s in range(0, 64, 7):
+        one, one_lse = ops.tree_attention(q[s:s + 1], k[s:s + 1], v[s:s + 1], L[s:s + 1], return_lse=True)
+        # P is rounded to bf16 against running maxima that may differ by the split: 2^-9 of every term, |v| up to ~4
+        assert float((one.float() - out[s:s + 1].float()).abs().max()) <= 2 ** -5
+        assert torch.allclose(one_lse, lse[s:s + 1], rtol=0, atol=1e-5)
 
 
 def test_cache_past_32_bit_offsets():
