@@ -7,6 +7,7 @@ actual_seq_qlen/kvlen) and :454-467 (generic SBH / BNSD / TND).  This function t
 the same arguments and returns a tuple whose element 0 is the attention output in
 the input layout; elements 1 and 2 are (softmax_max, softmax_sum) in the
 decomposition max = log-sum-exp, sum = 1 (lse = max + ln(sum) as in the NPU op).
+``sparse_mode`` 6 with ``prefix`` (one length per sequence) runs ``ops.score_attention``.
 
 ``npu_incre_flash_attention`` / ``npu_prompt_flash_attention`` stand in for the two ops of the
 ``--use-kv-cache`` branch (:428-451): one new token against the cache, and the prompt pass.
@@ -24,6 +25,8 @@ def _is_causal(atten_mask, sparse_mode, pre_tockens, next_tockens):
         if sparse_mode == 0:
             return False
         raise ValueError(f"sparse_mode={sparse_mode} needs an atten_mask")
+    if sparse_mode == 6:      # causal, and the first prefix[i] keys of sequence i visible to all of its rows
+        return True
     if sparse_mode in (2, 3, 4):
         # 2 = left-up causal, 3 = right-down causal (identical when q and kv lengths agree),
         # 4 = band with pre/next tokens; the reference only uses the causal band (next_tockens = 0).
@@ -55,14 +58,26 @@ def _band(causal, sparse_mode, pre_tockens, longest):
     return None
 
 
+def _attend(q, k, v, cu, scale, causal, band, prefix):
+    if prefix is None:
+        return ops.varlen_attention(q, k, v, cu, scale, causal, band)
+    if len(prefix) != len(cu) - 1:
+        raise ValueError(f"{len(prefix)} prefix lengths for {len(cu) - 1} sequences")
+    return ops.score_attention(q, k, v, cu, scale=scale, causal=causal, prefix_lens=prefix)
+
+
 def npu_fusion_attention(query, key, value, head_num, input_layout, pse=None, padding_mask=None, atten_mask=None,
                          scale=1.0, keep_prob=1.0, pre_tockens=2147483647, next_tockens=2147483647, inner_precise=0,
                          prefix=None, actual_seq_qlen=None, actual_seq_kvlen=None, sparse_mode=0, gen_mask_parallel=True,
                          sync=False):
     if pse is not None:
         raise NotImplementedError("pse (alibi) is not supported")
-    if padding_mask is not None or prefix is not None:
-        raise NotImplementedError("padding_mask / prefix are not supported")
+    if padding_mask is not None:
+        raise NotImplementedError("padding_mask is not supported")
+    if (prefix is not None) != (sparse_mode == 6):
+        raise NotImplementedError("prefix comes with sparse_mode 6, the compressed causal template with a prefix, and that mode with it")
+    if prefix is not None:
+        prefix = [int(x) for x in prefix]
     if keep_prob != 1.0:
         raise NotImplementedError("attention dropout is not supported (the shipped scripts use 0)")
     causal = _is_causal(atten_mask, sparse_mode, pre_tockens, next_tockens)
@@ -74,7 +89,7 @@ def npu_fusion_attention(query, key, value, head_num, input_layout, pse=None, pa
             raise NotImplementedError("different q / kv segmentations are not supported")
         cu = ops.cu_seqlens_from_actual_seq_len(actual_seq_qlen)
         band = _band(causal, sparse_mode, pre_tockens, max((b - a for a, b in zip(cu[:-1], cu[1:])), default=0))
-        out, lse = ops.varlen_attention(query, key, value, cu, scale, causal, band)
+        out, lse = _attend(query, key, value, cu, scale, causal, band, prefix)
         return out, lse, torch.ones_like(lse)
 
     if input_layout == "SBH":
@@ -87,7 +102,14 @@ def npu_fusion_attention(query, key, value, head_num, input_layout, pse=None, pa
         v3 = value.reshape(value.shape[0], b * hkv, d)
         if k3.shape[0] != s:
             raise NotImplementedError("q and kv lengths differ")
-        out, lse = ops.varlen_attention(q3, k3, v3, [0, s], scale, causal, _band(causal, sparse_mode, pre_tockens, s))
+        if prefix is not None and len(set(prefix)) > 1:       # folded heads share one prefix: sequences that do not are packed
+            rows = [x.unflatten(1, (b, -1)).transpose(0, 1).reshape(b * s, -1, d) for x in (q3, k3, v3)]
+            out, lse = _attend(*rows, [i * s for i in range(b + 1)], scale, causal, None, prefix)
+            lse = lse.unflatten(1, (b, s)).transpose(0, 1).reshape(b * head_num, s)
+            return out.reshape(b, s, hd).transpose(0, 1), lse, torch.ones_like(lse)
+        if prefix is not None and len(prefix) != b:
+            raise ValueError(f"{len(prefix)} prefix lengths for {b} sequences")
+        out, lse = _attend(q3, k3, v3, [0, s], scale, causal, _band(causal, sparse_mode, pre_tockens, s), prefix and prefix[:1])
         return out.reshape(s, b, hd), lse, torch.ones_like(lse)
 
     if input_layout in ("BSH", "BSND", "BNSD"):
@@ -102,7 +124,7 @@ def npu_fusion_attention(query, key, value, head_num, input_layout, pse=None, pa
             d = hd // head_num
             to_t = lambda x: x.reshape(b * s, x.shape[2] // d, d)
         cu = [i * s for i in range(b + 1)]
-        out, lse = ops.varlen_attention(to_t(query), to_t(key), to_t(value), cu, scale, causal, _band(causal, sparse_mode, pre_tockens, s))
+        out, lse = _attend(to_t(query), to_t(key), to_t(value), cu, scale, causal, _band(causal, sparse_mode, pre_tockens, s), prefix)
         if input_layout == "BNSD":
             out = out.reshape(b, s, -1, d).permute(0, 2, 1, 3)
         elif input_layout == "BSND":

@@ -284,6 +284,36 @@ def test_refusals(name, call):
         ops.score_attention(*args, **kw)
 
 
+@pytest.mark.parametrize("layout", ["TND", "SBH", "BSH", "BNSD"])
+@pytest.mark.parametrize("prefix", [[70, 3], [33, 33]])
+def test_fused_op_with_a_prefix(layout, prefix):
+    """The fused op's prefix mode in its layouts is score_attention on the packed rows, forward and backward, bit for bit."""
+    from long_vita_amd import ops
+    from long_vita_amd.fusion_attention import npu_fusion_attention
+    b, s, hq, hkv, d = 2, 150, 4, 2, 64
+    q, k, v, _do = (t.cuda() for t in make(b * s, hq, hkv, d, 3))
+    do = torch.randn(b * s, hq, d, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    want, want_lse = ops.score_attention(*leaves, [0, s, 2 * s], scale=0.1, prefix_lens=prefix)
+    want.backward(do)
+    mine = [t.clone().requires_grad_(True) for t in (q, k, v)]
+    put = {"TND": lambda x: x, "SBH": lambda x: x.reshape(b, s, -1).transpose(0, 1), "BSH": lambda x: x.reshape(b, s, -1),
+           "BNSD": lambda x: x.reshape(b, s, -1, d).permute(0, 2, 1, 3)}[layout]
+    back = {"TND": lambda x: x, "SBH": lambda x: x.transpose(0, 1).reshape(b * s, hq, d), "BSH": lambda x: x.reshape(b * s, hq, d),
+            "BNSD": lambda x: x.permute(0, 2, 1, 3).reshape(b * s, hq, d)}[layout]
+    kw = dict(actual_seq_qlen=[s, 2 * s], actual_seq_kvlen=[s, 2 * s]) if layout == "TND" else {}
+    out, lse, _one = npu_fusion_attention(*(put(x) for x in mine), hq, layout, atten_mask=True, scale=0.1, sparse_mode=6, prefix=prefix, **kw)
+    assert torch.equal(back(out), want)
+    back(out).backward(do)
+    for x, y in zip(mine, leaves):
+        assert torch.equal(x.grad, y.grad)
+    if layout == "SBH":
+        assert torch.equal(lse.reshape(b, hq, s).transpose(0, 1).reshape(hq, b * s), want_lse)
+    for bad in (dict(sparse_mode=6), dict(sparse_mode=2, prefix=prefix), dict(sparse_mode=6, prefix=[1, 2, 3])):
+        with pytest.raises((NotImplementedError, ValueError)):
+            npu_fusion_attention(*(put(x) for x in mine), hq, layout, atten_mask=True, scale=0.1, **bad, **kw)
+
+
 def test_empty_batches():
     from long_vita_amd import ops
     q, k, v, _ = (t.cuda() for t in make(8, 4, 2, 64, 1))
