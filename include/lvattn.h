@@ -274,7 +274,8 @@ int lvattn_decode_noalloc(const void* q, const void* k, const void* v, void* out
  * parents int32 live in device memory.  Sequence b holds cache_lens[b] keys that all its tokens see (a value outside
  * [0, rows - n] is moved to the nearest end), the n drafted tokens' keys are the rows behind them.  parents[b][i] (batch stride
  * 0: one tree for all) is the number of token i's parent: below i, -1 for a token that continues the cache, -2 for a slot
- * that holds no token (its output is 0, its lse -inf, its K / V rows are not looked at); a parent at or past i counts as -1.
+ * that holds no token (its output is 0, its lse -inf, its K / V rows are not looked at); a parent at or past i, or one that holds no token,
+ * counts as -1.  softmax_scale > 0.
  * parents == NULL: a chain (token i sees drafted tokens 0 .. i); n == 1 is the ordinary decode step.  The score rule is
  * lvattn_fwd_score's, with token i at position cache_lens[b] + its depth and cached key j at position j.
  * n <= 256, batch <= 512.  workspace: lvattn_tree_workspace_bytes(...) bytes, contents undefined afterwards, not shared by calls

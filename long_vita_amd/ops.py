@@ -330,7 +330,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_lens
 
     ``parents`` (int32 [n] or [b, n] on the device): token i's parent in the draft tree, -1 where it continues the cache,
     ``TREE_UNUSED`` (-2) for a slot that holds no token (output 0, lse -inf); a token sees itself and its ancestors.  Parents come
-    before their children (an entry that does not counts as -1).  None: a chain, and with n = 1 the ordinary decode step over
+    before their children (an entry that does not, or that names an unused slot, counts as -1).  None: a chain, and with n = 1 the ordinary decode step over
     caches of different lengths.  ``softcap`` / ``alibi_slopes`` as in ``score_attention``, token i standing at position
     ``cache_lens[s]`` + its depth and cached row j at position j (of an evicted cache that is no longer so).
 

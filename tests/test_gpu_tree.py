@@ -153,6 +153,18 @@ def test_one_tree_for_all_and_chain_as_tree():
     assert torch.equal(ops.tree_attention(q, k, v, L, parents=bad), ops.tree_attention(q, k, v, L, parents=good))
 
 
+def test_parents_that_are_none():
+    """A parent behind its child, the token itself, a number past the tree or an unused slot: the token continues the cache."""
+    from long_vita_amd import ops
+    q, k, v = (t.cuda() for t in make(1, 8, 60, 4, 2, 64, 9, [50]))
+    L = _lens("cuda", 50)
+    t = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    sl = slopes_of(4).cuda()
+    want = ops.tree_attention(q, k, v, L, parents=t(-1, -2, -1, 2, -1, -1, -1, 6), alibi_slopes=sl, return_lse=True)
+    got = ops.tree_attention(q, k, v, L, parents=t(-9 + 8, -2, 1, 2, 4, 7, 2 ** 31 - 1, 6), alibi_slopes=sl, return_lse=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_matches_decode_attention():
     from long_vita_amd import ops
     q, k, v = (t.cuda() for t in make(2, 1, 1000, 40, 8, 128, 9, [999, 999]))
