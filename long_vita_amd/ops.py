@@ -10,6 +10,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 from collections import OrderedDict
+from functools import lru_cache
 from typing import Sequence
 
 import numpy as np
@@ -371,9 +372,14 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_lens
     return (out, lse) if return_lse else out
 
 
+@lru_cache(maxsize=256)
+def _workspace_bytes(fn: str, *sizes) -> int:
+    return int(getattr(_lib.lib(), fn)(*sizes))
+
+
 def tree_workspace_bytes(b: int, n: int, rows: int, hq: int, hkv: int, d: int) -> int:
     """Bytes of workspace ``tree_attention`` needs for these sizes."""
-    return int(_lib.lib().lvattn_tree_workspace_bytes(b, n, rows, hq, hkv, d))
+    return _workspace_bytes("lvattn_tree_workspace_bytes", b, n, rows, hq, hkv, d)
 
 
 def tree_accept(k: torch.Tensor, v: torch.Tensor, cache_lens: torch.Tensor, path: torch.Tensor, n_accept: torch.Tensor,
@@ -448,7 +454,7 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: tor
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise LvAttnError(f"{who}: scale {scale} is not finite")
-    need = int(_lib.lib().lv_key_weights_workspace_bytes(b, n, rows, hq, hkv))
+    need = _workspace_bytes("lv_key_weights_workspace_bytes", b, n, rows, hq, hkv)
     ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
     check(_lib.lib().lv_key_weights(_ptr(q), _ptr(k), _ptr(lse), _ptr(row_weight), _ptr(weight), _ptr(out), _ptr(cache_lens), _ptr(parents), p_bs,
                                     _ptr(ws), need, b, n, rows, hq, hkv, d, *q.stride()[:3], *k.stride()[:3], *weight.stride()[:2],
@@ -513,7 +519,7 @@ def evict_cache(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, cache_le
             raise LvAttnError(f"{who}: the out buffers must not overlap the caches they are filled from")
     index = torch.empty((b, hkv, keep), dtype=torch.int32, device=dev)
     lens = torch.empty((b,), dtype=torch.int32, device=dev)
-    need = int(_lib.lib().lv_evict_workspace_bytes(b, rows, hkv))
+    need = _workspace_bytes("lv_evict_workspace_bytes", b, rows, hkv)
     ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
     check(_lib.lib().lv_evict_index(_ptr(weight), _ptr(cache_lens.contiguous()), _ptr(index), _ptr(lens), _ptr(ws), need, b, rows, hkv, keep, sink, recent,
                                     *weight.stride()[:2], _stream()), "lv_evict_index")
@@ -911,30 +917,37 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
+def _score_forward(q, k, v, slopes, rule, scale, with_grad):
+    """(out, lse, out_lo, pieces, covered); q, k, v as ``_rows`` returns them."""
+    total, hq, d = q.shape
+    dev = q.device
+    covered = rule.cu[0] == 0 and rule.cu[-1] == total
+    pieces = rule.pieces(hq, k.shape[1], dev)
+    make = torch.empty if covered else torch.zeros
+    out = make((total, hq, d), dtype=torch.bfloat16, device=dev)
+    lse = torch.empty((hq, total), dtype=torch.float32, device=dev)
+    if not covered:
+        lse.fill_(float("-inf"))
+    # for the backward pass: the byte of every output's mantissa that its rounding cut off (lvattn_score_delta)
+    out_lo = make((total, hq, d), dtype=torch.uint8, device=dev) if with_grad else None
+    if rule.cu[-1] > rule.cu[0]:
+        t = rule.tables(False, pieces[0], dev)
+        if pieces[0]:
+            ws_out = _workspace((t.ws_rows, hq, d), dev)
+            ws_lse = _workspace((hq, t.ws_rows), dev)
+            _score_fwd_launch(q, k, v, t, rule, slopes, scale, ws_out, ws_lse)
+            check(_lib.lib().lvattn_score_combine(_ptr(ws_out), _ptr(ws_lse), _ptr(out), _ptr(out_lo), _ptr(lse), _ptr(t.comb), t.comb.shape[0], hq, d,
+                                                  ws_lse.stride(0), out.stride(0), out.stride(1), lse.stride(0), _stream()), "lvattn_score_combine")
+        else:
+            _score_fwd_launch(q, k, v, t, rule, slopes, scale, out, lse, out_lo)
+    return out, lse, out_lo, pieces, covered
+
+
 class _ScoreAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, slopes, rule, scale):
         q, k, v = _rows(q), _rows(k), _rows(v)
-        total, hq, d = q.shape
-        dev = q.device
-        covered = rule.cu[0] == 0 and rule.cu[-1] == total
-        pieces = rule.pieces(hq, k.shape[1], dev)
-        out = (torch.empty if covered else torch.zeros)((total, hq, d), dtype=torch.bfloat16, device=dev)
-        lse = torch.empty((hq, total), dtype=torch.float32, device=dev)
-        if not covered:
-            lse.fill_(float("-inf"))
-        # for the backward pass: the byte of every output's mantissa that its rounding cut off (lvattn_score_delta)
-        out_lo = (torch.empty if covered else torch.zeros)((total, hq, d), dtype=torch.uint8, device=dev) if any(ctx.needs_input_grad) else None
-        if rule.cu[-1] > rule.cu[0]:
-            t = rule.tables(False, pieces[0], dev)
-            if pieces[0]:
-                ws_out = _workspace((t.ws_rows, hq, d), dev)
-                ws_lse = _workspace((hq, t.ws_rows), dev)
-                _score_fwd_launch(q, k, v, t, rule, slopes, scale, ws_out, ws_lse)
-                check(_lib.lib().lvattn_score_combine(_ptr(ws_out), _ptr(ws_lse), _ptr(out), _ptr(out_lo), _ptr(lse), _ptr(t.comb), t.comb.shape[0], hq, d,
-                                                      ws_lse.stride(0), out.stride(0), out.stride(1), lse.stride(0), _stream()), "lvattn_score_combine")
-            else:
-                _score_fwd_launch(q, k, v, t, rule, slopes, scale, out, lse, out_lo)
+        out, lse, out_lo, pieces, covered = _score_forward(q, k, v, slopes, rule, scale, any(ctx.needs_input_grad))
         ctx.save_for_backward(q, k, v, out, lse, slopes, out_lo)
         ctx.rule, ctx.scale, ctx.pieces, ctx.covered = rule, scale, pieces, covered
         ctx.mark_non_differentiable(lse)
@@ -1029,7 +1042,10 @@ def score_attention(q, k, v, cu_seqlens: Sequence[int], scale: float | None = No
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise LvAttnError(f"score_attention: scale {scale} is not finite")
-    return _ScoreAttention.apply(q, k, v, slopes, _ScoreRule(cu, causal, band, prefix, cap), scale)
+    rule = _ScoreRule(cu, causal, band, prefix, cap)
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        return _score_forward(_rows(q), _rows(k), _rows(v), slopes, rule, scale, False)[:2]
+    return _ScoreAttention.apply(q, k, v, slopes, rule, scale)
 
 
 # ---------------------------------------------------------------------------
