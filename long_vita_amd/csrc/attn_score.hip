@@ -270,7 +270,7 @@ extern "C" int lvattn_fwd_score(const void* q, const void* k, const void* v, voi
     p.q_rs = q_rs; p.q_hs = q_hs; p.k_rs = k_rs; p.k_hs = k_hs; p.v_rs = v_rs; p.v_hs = v_hs;
     p.o_rs = o_rs; p.o_hs = o_hs; p.lse_stride = lse_stride;
     p.scale = softmax_scale; p.scale_log2e = softmax_scale * 1.4426950408889634f;
-    if (!(fabsf(p.scale_log2e) >= 1e-30f)) p.scale_log2e = 1e-30f;   // the kernel divides slopes by it; scores this small are 0 beside them
+    if (!(fabsf(p.scale_log2e) >= 1e-20f)) p.scale_log2e = 1e-20f;   // the kernel divides slopes by it; scores this small are 0 beside them
     p.score = lv_score_rule(softmax_scale, softcap, slopes);
     if (lv_launch_fwd_pp_score(p, d, lv_score_mod(softcap, slopes), (hipStream_t)stream))
         return lv_fail(LV_ELAUNCH, "forward launch failed: %s", hipGetErrorString(hipGetLastError()));

@@ -333,9 +333,10 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_lens
     ``TREE_UNUSED`` (-2) for a slot that holds no token (output 0, lse -inf); a token sees itself and its ancestors.  Parents come
     before their children (an entry that does not, or that names an unused slot, counts as -1).  None: a chain, and with n = 1 the ordinary decode step over
     caches of different lengths.  ``softcap`` / ``alibi_slopes`` as in ``score_attention``, token i standing at position
-    ``cache_lens[s]`` + its depth and cached row j at position j (of an evicted cache that is no longer so).
+    ``cache_lens[s]`` + its depth and cached row j at position j (of an evicted cache that is no longer so).  The rows of tokens
+    that are there must be finite (unused slots and rows behind the tokens may hold anything).
 
-    At most 256 tokens per sequence and 512 sequences.  ``workspace`` (uint8, at least ``tree_workspace_bytes(...)``) lets a
+    At most 256 tokens per sequence and 512 sequences.  ``out`` must not overlap q, k or v.  ``workspace`` (uint8, at least ``tree_workspace_bytes(...)``) lets a
     program keep its own; calls that may overlap need one each.  No gradient."""
     who = "tree_attention"
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -357,6 +358,10 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_lens
         out = torch.empty((b, n, hq, d), dtype=torch.bfloat16, device=q.device)
     elif out.shape != (b, n, hq, d) or out.dtype != torch.bfloat16 or out.device != q.device or out.stride(3) != 1:
         raise LvAttnError(f"{who}: out must be bf16 [b, n, hq, d] on q's device with a contiguous last dimension")
+    elif 0 in out.stride() and any(s == 0 and m > 1 for s, m in zip(out.stride(), out.shape)):
+        raise LvAttnError(f"{who}: an expanded tensor cannot be written")
+    elif out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+        raise LvAttnError(f"{who}: out must not overlap q, k or v")
     if lse is None:
         lse = torch.empty((b, n, hq), dtype=torch.float32, device=q.device) if return_lse else None
     elif lse.shape != (b, n, hq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
@@ -387,6 +392,7 @@ def tree_accept(k: torch.Tensor, v: torch.Tensor, cache_lens: torch.Tensor, path
     """The accepted path of a draft tree becomes the caches' next rows, in place: row ``cache_lens[s] + path[s, i]`` moves to row
     ``cache_lens[s] + i`` for i < ``n_accept[s]``, in k, v [b, rows, hkv, d] and ``weight`` [b, hkv, rows] when given.  ``path``
     int32 [b, n] holds ascending token numbers (a parent stands before its child); entries past n_accept are not looked at.
+    ``cache_lens`` is at most rows - n and ``n_accept`` 0 to n, as they were for the attention (rows outside are never touched).
     Returns the new lengths, cache_lens + n_accept."""
     who = "tree_accept"
     _require_gpu(k, v, cache_lens, path, n_accept, weight)
@@ -515,8 +521,8 @@ def evict_cache(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, cache_le
             raise LvAttnError(f"{who}: out weight must be fp32 [{b}, {hkv}, {keep} or more] with contiguous rows")
         if any(s == 0 and m > 1 for t in out for s, m in zip(t.stride(), t.shape)):
             raise LvAttnError(f"{who}: an expanded tensor cannot be written")
-        if any(_overlap(o, i) for o in out for i in (k, v, weight)):
-            raise LvAttnError(f"{who}: the out buffers must not overlap the caches they are filled from")
+        if any(_overlap(o, i) for o in out for i in (k, v, weight)) or k_out.data_ptr() == v_out.data_ptr():
+            raise LvAttnError(f"{who}: the out buffers must not overlap each other or the caches they are filled from")
     index = torch.empty((b, hkv, keep), dtype=torch.int32, device=dev)
     lens = torch.empty((b,), dtype=torch.int32, device=dev)
     need = _workspace_bytes("lv_evict_workspace_bytes", b, rows, hkv)
@@ -1014,7 +1020,8 @@ def score_attention(q, k, v, cu_seqlens: Sequence[int], scale: float | None = No
     j <= i (all of them when ``causal`` is false).  ``prefix_lens`` (one per segment, causal only): the segment's first keys are
     visible to all of its rows, as the tokens of an image that opens a sample are; a length past the segment means the whole
     segment.  ``band`` (causal only, not with prefix_lens): a query sees itself and the ``band`` keys before it.
-    Rows outside every segment come back as zeros with lse -inf.  ``alibi_slopes`` (fp32 [Hq] on q's device) are constants."""
+    Rows outside every segment come back as zeros with lse -inf.  ``alibi_slopes`` (fp32 [Hq] on q's device) are constants.  As in
+    ``varlen_attention`` a segment's k and v must be finite: a key that a row does not see has weight 0, and 0 * NaN is NaN."""
     for t in (q, k, v):
         if not isinstance(t, torch.Tensor):
             raise LvAttnError("score_attention: q, k, v must be tensors")

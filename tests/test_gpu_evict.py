@@ -305,7 +305,7 @@ def test_refusals():
         ((k.float(), v, w, L, 8), {}), ((k, v, w.cpu(), L, 8), {}), ((k, v, w, L, 8), dict(out=(k, fine[1], fine[2]))),
         ((k, v, w, L, 9), dict(out=tuple(fine))), ((k, v, w, L, 8), dict(out=(fine[0], fine[1], fine[2].half()))),
         ((k, v, w, L, 8), dict(out=(fine[0][:1].expand(2, 8, 2, 64), fine[1], fine[2]))),
-        ((k, v, w.clone().requires_grad_(True), L, 8), {}),
+        ((k, v, w.clone().requires_grad_(True), L, 8), {}), ((k, v, w, L, 8), dict(out=(fine[0], fine[0], fine[2]))),
     ]
     for args, kw in evicts:
         with pytest.raises(_lib.LvAttnError):

@@ -333,6 +333,9 @@ REFUSED = [
     ("scale_zero", lambda q, k, v, L: ((q, k, v, L, 0.0), {})),
     ("grad", lambda q, k, v, L: ((q.clone().requires_grad_(True), k, v, L), {})),
     ("out", lambda q, k, v, L: ((q, k, v, L), dict(out=torch.empty(1, device=q.device)))),
+    ("out_is_q", lambda q, k, v, L: ((q, k, v, L), dict(out=q))),
+    ("out_in_cache", lambda q, k, v, L: ((q, (kk := torch.zeros(2, 20, 4, 64, dtype=torch.bfloat16, device=q.device))[:, :, :2], v, L), dict(out=kk[:, :3]))),
+    ("out_expanded", lambda q, k, v, L: ((q, k, v, L), dict(out=torch.empty_like(q[:1]).expand(2, -1, -1, -1)))),
     ("lse", lambda q, k, v, L: ((q, k, v, L), dict(lse=torch.empty(1, device=q.device)))),
     ("workspace", lambda q, k, v, L: ((q, k, v, L), dict(workspace=torch.empty(8, dtype=torch.uint8, device=q.device)))),
     ("cache_strides", lambda q, k, v, L: ((q, k.transpose(2, 3).contiguous().transpose(2, 3), v, L), {})),
