@@ -217,6 +217,61 @@ def test_saturated_cap_and_large_bias():
     assert float((lse.double().cpu() - want[1]).abs().max()) <= 8 * 2.0 ** -12
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.11, 1e-25, 1e-6])
+@pytest.mark.parametrize("cap,alibi", [(None, True), (20.0, False), (20.0, True)])
+def test_scales(scale, cap, alibi):
+    """A scale of 0, below 0 or next to nothing is a scale like any other."""
+    from long_vita_amd import ops
+    q, k, v, do = make(330, 4, 2, 64, 51)
+    cu, slopes = [0, 70, 330], slopes_of(4) if alibi else None
+    want = ref(q, k, v, cu, scale, True, cap, slopes, do=do)
+    leaves = [t.cuda().requires_grad_(True) for t in (q, k, v)]
+    out, lse = ops.score_attention(*leaves, cu, scale, softcap=cap, alibi_slopes=None if slopes is None else slopes.cuda())
+    out.backward(do.cuda())
+    assert rel(out, want[0]) <= REL_TOL and float((lse.double().cpu() - want[1]).abs().max()) <= LSE_TOL
+    for t, w in zip(leaves, want[2:]):
+        # (a scale of 1e-25 leaves gradients of 1e-25: still a part of the largest one)
+        assert rel(t.grad, w) <= GRAD_TOL if float(w.abs().max()) > 0 else not t.grad.any()
+
+
+def test_broadcast_inputs():
+    """Heads and rows that are one tensor seen several times: their gradients add up."""
+    from long_vita_amd import ops
+    T, hq, hkv, d = 140, 4, 2, 64
+    q, k, v, do = make(T, hq, hkv, d, 61)
+    q[:], k[:, 1] = q[:1], k[:, 0]
+    want = ref(q, k, v, [0, T], 0.2, True, 15.0, do=do)
+    q1, k1, v1 = (t.cuda().requires_grad_(True) for t in (q[:1], k[:, :1], v))
+    out, _ = ops.score_attention(q1.expand(T, hq, d), k1.expand(T, hkv, d), v1, [0, T], 0.2, softcap=15.0)
+    out.backward(do.cuda())
+    assert rel(out, want[0]) <= REL_TOL and rel(v1.grad, want[4]) <= GRAD_TOL
+    # a sum over rows (heads) of gradients that were each rounded: random signs, a few standard deviations against the largest
+    assert float((q1.grad.double().cpu() - want[2].sum(0, keepdim=True)).abs().max()) <= GRAD_TOL * float(want[2].abs().max()) * math.sqrt(T)
+    assert float((k1.grad.double().cpu() - want[3].sum(1, keepdim=True)).abs().max()) <= GRAD_TOL * float(want[3].abs().max()) * math.sqrt(hkv)
+
+
+@pytest.mark.parametrize("piece", [0, 256])
+def test_cut_off_bytes(piece):
+    """Out and its cut-off byte are the result to 16 bits of mantissa.  With equal scores P is 1, exact in bf16, so the result
+    is a mean of v in fp32 (row lengths up to 600: 600 * 2^-24 of |v| <= 5)."""
+    from long_vita_amd import ops
+    T, hq, hkv, d = 600, 2, 1, 128
+    _q, k, v, do = (t.cuda() for t in make(T, hq, hkv, d, 71))
+    rule = ops._ScoreRule((0, T), True, None, None, 0.0)
+    ops.set_split_override(piece, piece)
+    try:
+        out, lse, lo, pieces, covered = ops._score_forward(torch.zeros(T, hq, d, dtype=torch.bfloat16, device="cuda"), k, v, None, rule, 0.1, True)
+    finally:
+        ops.set_split_override(None, None)
+    assert covered and pieces[0] == piece
+    want = (v.double().cumsum(0) / torch.arange(1, T + 1, device="cuda", dtype=torch.float64)[:, None, None]).expand(T, hq, d)
+    b = lo.to(torch.int32)
+    bits = ((out.contiguous().view(torch.int16).to(torch.int32) & 0xffff) - (b >> 7)) * 65536 + b * 256 + 128
+    full = bits.view(torch.float32).double()
+    assert float((full - want).abs().max()) <= 2.0 ** -16 * float(want.abs().max()) + 600 * 2.0 ** -24 * 5
+    assert float((full - out.double()).abs().max()) <= 2.0 ** -8 * float(want.abs().max())
+
+
 def test_other_stream_and_graph():
     from long_vita_amd import ops
     q, k, v, do = (t.cuda() for t in make(700, 5, 1, 128, 41))
