@@ -302,7 +302,10 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
             for (int g = 0; g < 4; ++g) {
                 f32x4 t4 = *(LDS_PTR(f32x4, ld_ptr + sbx + 32 * g));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) cst[u][g][e] = MOD != 0 ? __builtin_fmaf(t4[e], cmul, is_k ? 0.f : 15.f) : t4[e] * cmul;
+                for (int e = 0; e < 4; ++e) {
+                    if constexpr (MOD != 0) cst[u][g][e] = __builtin_fmaf(t4[e], cmul, is_k ? 0.f : 15.f + lv_score_plus0<MOD>(p.score));
+                    else cst[u][g][e] = t4[e] * cmul;
+                }
             }
         };
 #pragma unroll
@@ -344,9 +347,8 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
                         const float fk = (float)(i0 + shift - kj + 4 * h);   // distance of the lane's first row of the unit to its key
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            float g;
-                            const float t = lv_score<MOD>(x[u][i], c, p.score, nslope2, fk + (float)((i & 3) + 8 * (i >> 2)), &g);
-                            pv[i] = fast_exp2(t + cst[u][i >> 2][i & 3]);
+                            float g = 0.f;
+                            pv[i] = fast_exp2(lv_score_plus<MOD>(x[u][i], c, p.score, nslope2, fk + (float)((i & 3) + 8 * (i >> 2)), cst[u][i >> 2][i & 3], &g));
                             if constexpr ((MOD & LV_SCORE_CAP) != 0) x[u][i] = g;
                         }
                     } else {
@@ -371,7 +373,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
                     if constexpr (MOD != 0) {
                         // P travels to the partner as 2^15 P in fp16 (P <= 1: up to 2^15, and down to 2^-29 with the full 11 bits),
                         // so that dS = P (1 - tanh^2) (dP - delta) is rounded to bf16 once and not twice; with a cap the first two
-                        // factors are multiplied here.  Rounded towards zero, the form that packs two: within 2^-10.
+                        // factors are multiplied here (a fourth of them).  Rounded towards zero, the form that packs two: within 2^-10.
                         u32x4 z[2];
 #pragma unroll
                         for (int i = 0; i < 16; i += 2) {
@@ -495,7 +497,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
     // ---- epilogue: accumulators (key on the lane) -> rows of dv (V-wave) or dk (K-wave, times scale)
     if (kj < k_rows) {
         const int64_t grow = k_row0 + dsc.out_delta + kj;
-        const float f = (is_k ? p.scale : 1.f) * (MOD != 0 ? 0x1p-15f : 1.f);
+        const float f = MOD == 0 ? (is_k ? p.scale : 1.f) : 0x1p-15f * (is_k ? ((MOD & LV_SCORE_CAP) != 0 ? 4.f : 1.f) * p.scale : 1.f);
         void* const gbase = is_k ? p.dk : p.dv;
         const int64_t g_rs = is_k ? p.dk_rs : p.dv_rs, g_hs = is_k ? p.dk_hs : p.dv_hs;
 #pragma unroll

@@ -217,12 +217,12 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
                 // dependent pair would stall on the first one's latency sixteen times over
                 float pv[16];
                 if constexpr (MOD != 0) {
-                    const float fq = (float)(qi + shift - kb0 - 4 * h);
+                    const float fq = (float)(qi + shift - kb0 - 4 * h), plus = lv_score_plus0<MOD>(p.score) - lse2;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        float g;
-                        pv[i] = lv_score<MOD>(s[i], c, p.score, nslope2, fq - (float)((i & 3) + 8 * (i >> 2)), &g) - lse2;
-                        if constexpr ((MOD & LV_SCORE_CAP) != 0) s[i] = g;   // the score's own derivative, for dS below
+                        float g = 0.f;
+                        pv[i] = lv_score_plus<MOD>(s[i], c, p.score, nslope2, fq - (float)((i & 3) + 8 * (i >> 2)), plus, &g);
+                        if constexpr ((MOD & LV_SCORE_CAP) != 0) s[i] = g;   // a fourth of the score's own derivative, for dS below
                     }
                 } else {
 #pragma unroll
@@ -314,6 +314,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
     // ---- epilogue: dQ^T accumulators (query on the lane) -> rows of dq
     if (qi < q_rows) {
         const int64_t grow = q_row0 + dsc.out_delta + qi;
+        const float f = p.scale * ((MOD & LV_SCORE_CAP) != 0 ? 4.f : 1.f);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -323,13 +324,13 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
                     float* dqp = reinterpret_cast<float*>(p.dq) + grow * p.dq_rs + (int64_t)head * p.dq_hs + dcol;
                     f32x4 a = p.f32_store ? f32x4{0.f, 0.f, 0.f, 0.f} : *reinterpret_cast<f32x4*>(dqp);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) a[e] += dq[mt][4 * g4 + e] * p.scale;
+                    for (int e = 0; e < 4; ++e) a[e] += dq[mt][4 * g4 + e] * f;
                     *reinterpret_cast<f32x4*>(dqp) = a;
                 } else {
                     __bf16* dqp = reinterpret_cast<__bf16*>(p.dq) + grow * p.dq_rs + (int64_t)head * p.dq_hs + dcol;
                     bf16x4 a;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) a[e] = (__bf16)(dq[mt][4 * g4 + e] * p.scale);
+                    for (int e = 0; e < 4; ++e) a[e] = (__bf16)(dq[mt][4 * g4 + e] * f);
                     *reinterpret_cast<bf16x4*>(dqp) = a;
                 }
             }

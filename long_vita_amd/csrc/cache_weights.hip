@@ -25,12 +25,13 @@ __device__ __forceinline__ void weight_dma4(const float* g, uint32_t lds_dst) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_dst) : "memory");
 }
 
-// log2(rho) - lse log2(e) of a row: what its scores' exponents start from; -inf for a row that counts for nothing
+// log2(rho) - lse log2(e) of a row, plus cap_out (0 without a cap) as lv_score_plus wants it: what its scores' exponents start
+// from; -inf for a row that counts for nothing
 __device__ __forceinline__ float row_constant(const WeightParams& p, int s, int token, int head) {
     const float rho = p.row_weight ? p.row_weight[(int64_t)s * p.n + token] : 1.f;
     const float l = p.lse[((int64_t)s * p.n + token) * p.hq + head];
     if (!(rho > 0.f) || !(l > -INFINITY)) return -INFINITY;
-    return (p.row_weight ? __builtin_amdgcn_logf(rho) : 0.f) - l * 1.4426950408889634f;
+    return (p.row_weight ? __builtin_amdgcn_logf(rho) : 0.f) + (p.score.cap_out - l * 1.4426950408889634f);
 }
 
 // rows that hold no key keep their weights (launched when w_out is not w_in); 4096 rows of one (sequence, KV head) per workgroup
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
                         for (int e = 0; e < 4; ++e) {
                             const int i = 4 * q4 + e;
                             float t2;
-                            if constexpr (MOD != 0) t2 = lv_score<MOD>(xb[i], p.scale_log2e, p.score, slope[e], pos[e] - kpos) + cc[e];
+                            if constexpr (MOD != 0) t2 = lv_score_plus<MOD>(xb[i], p.scale_log2e, p.score, slope[e], pos[e] - kpos, cc[e]);
                             else t2 = __builtin_fmaf(xb[i], p.scale_log2e, cc[e]);
                             pv[i] = fast_exp2(t2);
                         }
@@ -470,7 +471,7 @@ __global__ __launch_bounds__(256, (MOD & LV_SCORE_BIAS) || GUARD ? 2 : 3) void l
                     if constexpr (MOD != 0) {
                         float dist = 0.f, sl2 = 0.f;
                         if constexpr ((MOD & LV_SCORE_BIAS) != 0) { dist = pv4[i >> 2][i & 3] - kpos[g]; sl2 = sv4[i >> 2][i & 3]; }
-                        e = lv_score<MOD>(x[g][i], p.scale_log2e, p.score, sl2, dist) + cc;
+                        e = lv_score_plus<MOD>(x[g][i], p.scale_log2e, p.score, sl2, dist, cc);
                     } else {
                         e = __builtin_fmaf(x[g][i], p.scale_log2e, cc);
                     }
