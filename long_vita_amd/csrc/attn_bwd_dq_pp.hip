@@ -170,6 +170,17 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
         nslope2 = -1.4426950408889634f * p.score.slopes[head];
         asm volatile("" : "+v"(nslope2));
     }
+    // With a cap the vector phase is the longer one: dP's accumulators start from -delta, one subtraction per score less
+    // (577 -> 536 us for 8192 packed rows of 40 / 8 heads)
+    constexpr bool DP_INIT = (MOD & LV_SCORE_CAP) != 0;
+    f32x16 dp0;
+    if constexpr (DP_INIT) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            dp0[i] = -delta;
+            asm volatile("" : "+v"(dp0[i]));
+        }
+    }
 
     // fragments of one MFMA group: SPG K rows, SPG V rows (slot sb_new), QPG K columns (slot sb_old)
     bf16x8 kfr[2][SPG], vfr[2][SPG], tfr[2][QPG];
@@ -198,7 +209,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
         issue_tile();
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 #pragma unroll
-        for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+        for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = DP_INIT ? dp0[i] : 0.f; }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             bf16x8 kf = *(LDS_PTR(bf16x8, k_ptr[ks]));
@@ -242,7 +253,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    float ds = pv[i] * (dp[i] - delta);
+                    float ds = DP_INIT ? pv[i] * dp[i] : pv[i] * (dp[i] - delta);
                     if constexpr ((MOD & LV_SCORE_CAP) != 0) ds *= s[i];
                     dsf[i >> 3][i & 7] = (__bf16)ds;
                 }
@@ -263,7 +274,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
             // ================= MFMA(t+1): S_{t+1}, dP_{t+1}, dQ += K_t^T dS_t =================
             __builtin_amdgcn_s_setprio(LV_PP_PRIO);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = 0.f; }
+            for (int i = 0; i < 16; ++i) { s[i] = 0.f; dp[i] = DP_INIT ? dp0[i] : 0.f; }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const int set = g & 1;
