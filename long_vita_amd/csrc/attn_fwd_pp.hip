@@ -451,19 +451,25 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
         if (live && (p.o_f32 || p.o_lo)) {
             const int64_t at = ((int64_t)(q_row0 + dsc.out_delta + qi) * p.hq + head) * D + 4 * h;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt) {
+                uint32_t lo[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int g4 = 0; g4 < 4; ++g4) {
                     f32x4 v4;
-                    uint32_t lo = 0;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         v4[e] = oacc[mt][4 * g4 + e] * inv;
-                        lo |= lv_low_byte(v4[e]) << (8 * e);
+                        lo[g4] |= lv_low_byte(v4[e]) << (8 * e);
                     }
                     if (p.o_f32) *reinterpret_cast<f32x4*>(p.o_f32 + at + 32 * mt + 8 * g4) = v4;
-                    else *reinterpret_cast<uint32_t*>(p.o_lo + at + 32 * mt + 8 * g4) = lo;
                 }
+                if (!p.o_f32) {
+                    // the two lanes of a row hold four bytes in turn: exchanged, so that each stores 16 neighbours
+                    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(lo[0]), "+v"(lo[2]));
+                    asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(lo[1]), "+v"(lo[3]));
+                    *reinterpret_cast<u32x4*>(p.o_lo + at + 32 * mt + 12 * h) = u32x4{lo[0], lo[2], lo[1], lo[3]};
+                }
+            }
         }
     }
     if (live) {

@@ -259,7 +259,7 @@ extern "C" int lvattn_fwd_score(const void* q, const void* k, const void* v, voi
     if (!out || !lse || !desc_dev) return lv_fail(LV_EINVAL, "null out/lse/desc pointer");
     if (((uintptr_t)out & (out_f32 ? 15 : 7)) || (o_rs & 3) || (o_hs & 3)) return lv_fail(LV_EINVAL, "out must be 8-byte (fp32: 16-byte) aligned with strides %% 4 == 0");
     if (out_f32 && (out_lo || o_hs != d || o_rs != (int64_t)hq * d)) return lv_fail(LV_EINVAL, "fp32 results are contiguous and have no cut-off bytes");
-    if ((uintptr_t)out_lo & 3) return lv_fail(LV_EINVAL, "out_lo must be 4-byte aligned");
+    if ((uintptr_t)out_lo & 15) return lv_fail(LV_EINVAL, "out_lo must be 16-byte aligned");
     if (n_blocks < 0 || q_rows_total <= 0 || k_rows_total <= 0) return lv_fail(LV_EINVAL, "bad sizes");
     if (n_blocks == 0) return LV_OK;
     if ((int64_t)n_blocks * hq > 0x7fffffffLL) return lv_fail(LV_EINVAL, "grid too large");
