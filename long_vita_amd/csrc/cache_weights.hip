@@ -7,7 +7,7 @@
 // S = Q K^T, with the KEY on the lane (32x32x16 MFMA, A = query rows, B = keys): a key's sum over 32 query rows is a sum over
 // its lane's 16 accumulators.  Nothing is ever summed by atomics.  Two kernels:
 //
-// - up to 128 query rows per KV head (a decode step, a tree): bound by K's bytes.  The query fragments and, with up to 64 rows,
+// - up to 128 query rows per KV head (a decode step, a tree), twice that in two passes: bound by K's bytes.  The query fragments and, with up to 64 rows,
 //   the rows' constants stay in registers, eight waves per workgroup stream K, each its own 32-key slices through its own LDS slots by
 //   direct global -> LDS loads, without a barrier; tiles of all sequences are dealt evenly (cache_list.h).  The old weight of a
 //   key travels with its slice, so w_out is written on the spot.
@@ -15,8 +15,8 @@
 //   through an LDS ring of 64-row tiles shared by its four waves, two on each half of the keys, on alternate 32 rows.  A
 //   first small kernel prepares the rows' constants.  When there are fewer key blocks than the chip has room for, the rows
 //   are cut into pieces whose sums are added in order by a last kernel.  8 MFMAs (256 cycles) stand against 16 exponentials,
-//   multiply-adds and adds per 32 x 32 scores, so the vector work bounds it.  Short sweeps pay for every 128 keys' loads: 125
-//   rows of 16 ragged caches of 107K keys, 8 KV heads, took 192 us this way and take 68 us streamed.
+//   multiply-adds and adds per 32 x 32 scores, so the vector work bounds it; few rows pay for every 128 keys' loads (125 rows
+//   of the 16 ragged caches below: 192 us, streamed 68 us).
 //
 // Measured, 40 / 8 heads of 128: one token over 4 caches of 7,777 to 65,536 keys 65 us (47 us streaming, 5.8 TB/s; 6 us copying
 // the unused rows); a prompt of 8,191 tokens 386 us (890 TFLOP/s).
@@ -59,7 +59,11 @@ __global__ __launch_bounds__(256) void lv_weight_copy_kernel(WeightParams p) {
 // up to 32 RT query rows
 // ---------------------------------------------------------------------------
 #define LV_WEIGHT_TILE 256                    // keys per tile: 32 for each of eight waves
-#define LV_WEIGHT_STREAM_ROWS 128
+#define LV_WEIGHT_STREAM_ROWS 128             // query rows of a pass over the keys
+// Two passes at most, then the other kernel (160 / 255 rows, two passes against it: 152 / 168 against 267 / 310 us for 16 ragged caches
+// of 107K keys, whose longest sets its grid, 133 / 141 against 164 / 196 us for one of 131K, 143 / 151 against 112 / 138 us for 64
+// short ones; with three passes it is 210 against 209 us for the long one).
+#define LV_WEIGHT_PASSES 2
 template <int D> constexpr int weight_slots() { return D == 128 ? 2 : 4; }
 template <int D> constexpr int weight_slot_bytes() { return 32 * D * 2 + 256; }        // a slice of K, the 32 old weights
 template <int D> constexpr int weight_lds_bytes() {
@@ -152,8 +156,8 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
         // query fragments (lane r: row 32 b + r), and the rows' constants in LDS
         __syncthreads();                  // the previous sequence's constants are no longer read
         if (tid < SR) {
-            const int tc = min(tid, n_rows - 1), token = tc / p.group, head = kvh * p.group + tc % p.group;
-            rc[tid] = (tid < n_rows && !(p.parents && par[token] == LV_TREE_UNUSED)) ? row_constant(p, s, token, head) : -INFINITY;
+            const int tc = min(p.row0 + tid, n_rows - 1), token = tc / p.group, head = kvh * p.group + tc % p.group;
+            rc[tid] = (p.row0 + tid < n_rows && !(p.parents && par[token] == LV_TREE_UNUSED)) ? row_constant(p, s, token, head) : -INFINITY;
             if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
                 rc[SR + tid] = (float)(len + (p.parents ? depth[token] : token));
                 rc[2 * SR + tid] = -1.4426950408889634f * p.score.slopes[head];
@@ -163,7 +167,7 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
         bf16x8 qf[RT][KS];
 #pragma unroll
         for (int b = 0; b < RT; ++b) {
-            const int row = 32 * b + r, rowc = min(row, n_rows - 1), token = rowc / p.group;
+            const int row = p.row0 + 32 * b + r, rowc = min(row, n_rows - 1), token = rowc / p.group;
             const bool on = row < n_rows && (!p.row_weight || p.row_weight[(int64_t)s * p.n + token] > 0.f) && !(p.parents && par[token] == LV_TREE_UNUSED);
             const __bf16* qp = p.q + (int64_t)s * p.q_bs + (int64_t)token * p.q_ns + (int64_t)(kvh * p.group + rowc % p.group) * p.q_hs + 8 * h;
 #pragma unroll
@@ -249,7 +253,7 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int ar = 32 * b + (i & 3) + 8 * (i >> 2) + row_m;
-                            bool vis = ar >= first_row;
+                            bool vis = p.row0 + ar >= first_row;
                             if (look) vis = (anc[rtok[ar] * words + (jt >> 5)] >> (jt & 31)) & 1;
                             pv[i] = vis ? pv[i] : 0.f;
                             asm volatile("" : "+v"(pv[i]));      // keeps this a branch
@@ -341,7 +345,7 @@ __global__ __launch_bounds__(256, (MOD & LV_SCORE_BIAS) || GUARD ? 2 : 3) void l
     }
     const int n_rows = p.n * p.group;
     const int words = (p.n + 31) >> 5;
-    if (p.parents) list_tree(p.parents + (int64_t)s * p.parents_bs, p.n, words, k0 + LV_WEIGHT_KEYS > len, par, depth, anc, tid, 256);
+    if (p.parents && k0 + LV_WEIGHT_KEYS > len) list_tree(p.parents + (int64_t)s * p.parents_bs, p.n, words, true, par, depth, anc, tid, 256);
 
     // ---- this wave's keys: two groups of 32, fragments for the whole kernel
     bf16x8 kf[2][KS];
@@ -570,7 +574,7 @@ struct WeightPlan { bool stream; int shares, pieces, key_blocks, rows_pad; int64
 static WeightPlan weight_plan(int batch, int n, int rows, int hq, int hkv) {
     WeightPlan t{};
     const int n_rows = n * (hq / hkv);
-    t.stream = n_rows <= LV_WEIGHT_STREAM_ROWS && n <= LV_TREE_MAX_TOKENS && batch <= LV_TREE_MAX_BATCH;
+    t.stream = n_rows <= LV_WEIGHT_PASSES * LV_WEIGHT_STREAM_ROWS && n <= LV_TREE_MAX_TOKENS && batch <= LV_TREE_MAX_BATCH;
     if (t.stream) {
         const int64_t tiles = (int64_t)batch * ((rows + LV_WEIGHT_TILE - 1) / LV_WEIGHT_TILE);
         int64_t g = 256 / hkv;                // a workgroup's slots fill a compute unit's LDS
@@ -666,12 +670,15 @@ extern "C" int lv_key_weights(const void* q, const void* k, const float* lse, co
     const int mod = lv_score_mod(softcap, slopes) & (LV_SCORE_CAP | LV_SCORE_BIAS);
     hipStream_t st = (hipStream_t)stream;
     if (t.stream) {
-        const int rt = n * p.group <= 32 ? 1 : (n * p.group <= 64 ? 2 : 4);
+        const int n_rows = n * p.group, rt = n_rows <= 32 ? 1 : (n_rows <= 64 ? 2 : 4);
         if (w_in != w_out)
             hipLaunchKernelGGL(lv_weight_copy_kernel, dim3((unsigned)((rows + LV_WEIGHT_COPY - 1) / LV_WEIGHT_COPY), (unsigned)(batch * hkv)), dim3(256), 0, st, p);
         const unsigned blocks = (unsigned)(hkv * t.shares);
-        if (d == 128) launch_stream<128>(p, mod, rt, blocks, st);
-        else launch_stream<64>(p, mod, rt, blocks, st);
+        for (p.row0 = 0; p.row0 < n_rows; p.row0 += LV_WEIGHT_STREAM_ROWS) {
+            if (d == 128) launch_stream<128>(p, mod, rt, blocks, st);
+            else launch_stream<64>(p, mod, rt, blocks, st);
+            p.w_in = w_out; p.wi_bs = wo_bs; p.wi_hs = wo_hs;      // the next pass adds to what this one left
+        }
     } else {
         const int64_t blocks = (int64_t)batch * hkv * t.key_blocks * t.pieces;
         if (blocks > 0x7fffffffLL) return lv_fail(LV_EINVAL, "lv_key_weights: grid too large");
