@@ -206,6 +206,7 @@ int lvattn_combine_sum(const float* ws, void* out, const int32_t* comb_dev, int 
  *       the eight mantissa bits that the rounding of out to bf16 cut off; out_f32 != 0: out is fp32, contiguous (the partial results
  *       of cut sweeps), out_lo NULL.
  *   lvattn_score_delta      delta[h, row] = sum_d dout * (out with its cut-off byte), fp32 [hq, lse_stride].
+ *   lvattn_score_combine_grads  dq, dk, dv <- sums of their pieces [ws_rows, heads, d] fp32 (lvattn_combine_sum, three in one launch).
  *   lvattn_score_combine    out / out_lo / lse <- log-sum-exp merge of the pieces' fp32 out [ws_rows, hq, d] and lse, as lvattn_combine_lse. */
 int lv_build_score_blocks(const int32_t* cu_seqlens_host, int n_seg, int causal, int band, const int32_t* prefix_host, int backward, int piece,
                           int32_t* desc_host, int max_blocks, int32_t* comb_host, int max_comb, int* n_comb, int* ws_rows);
@@ -219,6 +220,10 @@ int lvattn_score_delta(const void* out, const uint8_t* out_lo, const void* dout,
                        int64_t o_head_stride, int64_t do_row_stride, int64_t do_head_stride, int64_t lse_stride, void* stream);
 int lvattn_score_combine(const float* ws_out, const float* ws_lse, void* out, uint8_t* out_lo, float* lse, const int32_t* comb_dev, int n_comb,
                          int hq, int d, int64_t ws_lse_stride, int64_t o_row_stride, int64_t o_head_stride, int64_t lse_stride, void* stream);
+int lvattn_score_combine_grads(const float* dq_ws, const float* dk_ws, const float* dv_ws, void* dq, void* dk, void* dv, const int32_t* qcomb_dev,
+                               int n_qcomb, const int32_t* kcomb_dev, int n_kcomb, int hq, int hkv, int d, int64_t dq_row_stride,
+                               int64_t dq_head_stride, int64_t dk_row_stride, int64_t dk_head_stride, int64_t dv_row_stride,
+                               int64_t dv_head_stride, void* stream);
 int lvattn_bwd_score(const void* q, const void* k, const void* v, const void* dout, const float* lse, const float* delta, void* dq, void* dk,
                      void* dv, const int32_t* qdesc_dev, int n_qblocks, const int32_t* kdesc_dev, int n_kblocks, int q_rows_total,
                      int k_rows_total, int hq, int hkv, int d, int64_t q_row_stride, int64_t q_head_stride, int64_t k_row_stride,

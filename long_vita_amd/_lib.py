@@ -52,6 +52,7 @@ _SIGNATURES = {
     "lv_build_score_blocks": (_int, [_i32p, _int, _int, _int, _i32p, _int, _int, _i32p, _int, _i32p, _int, C.POINTER(C.c_int), C.POINTER(C.c_int)]),
     "lv_plan_score_split": (_int, [_i32p, _int, _int, _int, _i32p, _int, _int, _int, _int]),
     "lvattn_score_delta": (_int, [_vp] * 4 + [_int] * 3 + [_i64] * 5 + [_vp]),
+    "lvattn_score_combine_grads": (_int, [_vp] * 7 + [_int, _vp] + [_int] * 4 + [_i64] * 6 + [_vp]),
     "lvattn_score_combine": (_int, [_vp] * 6 + [_int] * 3 + [_i64] * 4 + [_vp]),
     "lvattn_fwd_score": (_int, [_vp] * 5 + [_int, _vp, _vp] + [_int] * 6 + [_i64] * 9 + [_f, _f, _vp, _vp]),
     "lvattn_bwd_score": (_int, [_vp] * 10 + [_int, _vp] + [_int] * 6 + [_i64] * 15 + [_f, _f, _vp, _int, _vp]),

@@ -984,9 +984,9 @@ class _ScoreAttention(torch.autograd.Function):
             dq_ws = _workspace((tq.ws_rows, hq, d), dev)
             dk_ws, dv_ws = (_workspace((tk.ws_rows, hkv, d), dev) for _ in range(2))
             _score_bwd_launch(q, k, v, dout, lse, delta, tq, tk, rule, slopes, ctx.scale, dq_ws, dk_ws, dv_ws, 2)
-            combine_sum_launch(dq_ws, dq, tq)
-            combine_sum_launch(dk_ws, dk, tk)
-            combine_sum_launch(dv_ws, dv, tk)
+            check(_lib.lib().lvattn_score_combine_grads(_ptr(dq_ws), _ptr(dk_ws), _ptr(dv_ws), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(tq.comb), tq.comb.shape[0],
+                                                        _ptr(tk.comb), tk.comb.shape[0], hq, hkv, d, dq.stride(0), dq.stride(1), dk.stride(0), dk.stride(1),
+                                                        dv.stride(0), dv.stride(1), _stream()), "lvattn_score_combine_grads")
         else:
             _score_bwd_launch(q, k, v, dout, lse, delta, rule.tables(False, 0, dev), rule.tables(True, 0, dev), rule, slopes, ctx.scale,
                               dq, dk, dv, 0)
