@@ -853,6 +853,9 @@ def varlen_attention(q, k, v, cu_seqlens: Sequence[int], scale: float | None = N
 # ---------------------------------------------------------------------------
 # autograd: packed attention whose scores follow a rule (tanh cap, distance bias, prefix)
 # ---------------------------------------------------------------------------
+_captured_tables: dict = {}
+
+
 class _ScoreRule:
     """What a launch needs to know besides q, k, v: the segments, who sees whom, and how a score is changed.  ``slopes`` (fp32
     [hq] on the device, or None) stays out of the table keys: tables do not depend on it."""
@@ -894,7 +897,15 @@ class _ScoreRule:
             call(desc.ctypes.data_as(_I32P), desc.shape[0], comb.ctypes.data_as(_I32P), comb.shape[0])
             return SplitTables(_to_device(desc[:n], device), torch.from_numpy(comb[:n_comb.value]).to(device) if piece else None,
                                int(ws_rows.value) if piece else 0, LV_BWD_BLOCK_N if backward else 256, int(piece))
-        return _blocks.get(("score", self.key, bool(backward), int(piece), str(device)), build)
+        key = ("score", self.key, bool(backward), int(piece), str(device))
+        capturing = key[-1] != "cpu" and torch.cuda.is_current_stream_capturing()
+        if capturing and key not in _blocks.store:
+            raise LvAttnError("score_attention: the first call with these segments copies their work-item tables to the device, which a "
+                              "stream capture does not allow: call it once, forward and backward, before the capture")
+        t = _blocks.get(key, build)
+        if capturing:
+            _captured_tables[key] = t       # a graph reads the table at every replay: it outlives its turn in the cache
+        return t
 
 
 def _score_fwd_launch(q, k, v, tables, rule, slopes, scale, out, lse, out_lo=None):

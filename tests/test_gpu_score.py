@@ -304,6 +304,45 @@ def test_other_stream_and_graph():
         assert all(torch.equal(a, b) for a, b in zip(captured, want))
 
 
+def test_graph_outlives_the_table_cache():
+    """A captured call keeps its work-item tables when other packings have pushed them out of the cache."""
+    from long_vita_amd import ops
+    q, k, v, do = (t.cuda() for t in make(500, 4, 2, 64, 43))
+    leaves = [t.clone().requires_grad_(True) for t in (q, k, v)]
+
+    def step():
+        out, lse = ops.score_attention(*leaves, [0, 123, 500], softcap=30.0, prefix_lens=[50, 60])
+        return (out, lse, *torch.autograd.grad(out, leaves, do))
+    want = [t.detach().clone() for t in step()]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    store = dict(ops._blocks.store)
+    mine = [key for key in store if key[0] == "score" and key[1][0] == (0, 123, 500)]
+    assert mine and all(any(store[key] is t for t in ops._captured_tables.values()) for key in mine)
+    for n in range(ops._blocks.capacity + 1):
+        ops._blocks.get(("other", n), lambda: None)
+    del store
+    junk = [torch.full((64,), -1, dtype=torch.int32, device="cuda") for _ in range(2000)]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, want))
+    del junk
+    fresh = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(fresh):
+        with pytest.raises(_lib.LvAttnError, match="before the capture"):
+            ops.score_attention(q, k, v, [0, 77, 500])
+        after = q + 1
+    fresh.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(after, q + 1)
+
+
 REFUSED = [
     ("rank", lambda q, k, v: ((q[0], k, v, [0, 8]), {})),
     ("dtype", lambda q, k, v: ((q.float(), k, v, [0, 8]), {})),
