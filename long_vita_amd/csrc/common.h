@@ -43,6 +43,13 @@ __device__ __forceinline__ void pair32(float x, float& a, float& b) {
 __device__ __forceinline__ float pair32_max(float x) { float a, b; pair32(x, a, b); return fmaxf(a, b); }
 __device__ __forceinline__ float pair32_sum(float x) { float a, b; pair32(x, a, b); return a + b; }
 
+// acc + the sum of eight bf16 values, in fp32 (two to an instruction)
+__device__ __forceinline__ float add_bf16x8(bf16x8 v, float acc) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 2) acc = __builtin_amdgcn_fdot2_f32_bf16(bf16x2{v[i], v[i + 1]}, bf16x2{(__bf16)1.f, (__bf16)1.f}, acc, false);
+    return acc;
+}
+
 // ---- bf16 rounding helpers of the rotary embedding (shared by rope.hip and the attention prologue) ----
 // Round to the nearest bf16 (ties to even) and return it as f32.  Done on the bit pattern: written as a
 // float -> __bf16 -> float cast pair the compiler may keep the unrounded value ("excess precision") and
