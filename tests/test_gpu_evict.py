@@ -251,6 +251,64 @@ def test_run_together():
     assert float((o.double().cpu() - wo).abs().max()) <= 2.0 ** -7 * float(wo.abs().max())
 
 
+@pytest.mark.parametrize("n", [1, 70])
+def test_long_cache_past_32_bit_offsets(n):
+    """A cache of more than 2^32 bytes and 2^31 elements: weights and eviction at both of its ends."""
+    from long_vita_amd import ops
+    rows, hq, hkv, d = (1 << 21) + 5000, 8, 8, 128
+    length = rows - n
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k = torch.randn(1, rows, hkv, d, generator=g, device="cuda", dtype=torch.bfloat16)
+    q = torch.randn(1, n, hq, d, generator=g, device="cuda", dtype=torch.bfloat16)
+    assert k.numel() > 2 ** 31
+    L = torch.tensor([length], dtype=torch.int32, device="cuda")
+    lse = torch.full((1, n, hq), 15.0, device="cuda")
+    wide = 5 if n == 70 else 1             # heads of one KV head side by side: 70 tokens x 5 heads take the kernel for many rows
+    qw = q.repeat_interleave(wide, 2)
+    w0 = torch.zeros(1, hkv, rows, device="cuda")
+    w = ops.key_weights(qw, k, lse.repeat_interleave(wide, 2), w0, L)
+    for j in (0, 127, 1 << 20, length - 1, length, rows - 1):
+        x = (q[0].double() * k[0, j].double()).sum(-1) * d ** -0.5                         # [n, heads]
+        see = torch.arange(n, device="cuda")[:, None] >= j - length
+        want = wide * (torch.exp(x - 15.0) * see).sum(0)
+        assert float((w[0, :, j].double() - want).abs().max()) <= W_TOL * float(want.max())
+    # the heaviest are planted, two of them behind the offsets
+    top = torch.tensor([5, 1 << 20, length - 3], device="cuda")
+    w[0, :, top] = w.max() * 2 + 1
+    k2, v2, w2, L2, idx = ops.evict_cache(k, k, w, L, 40, sink=2, recent=1)
+    keep = idx[0].long()
+    assert int(L2[0]) == 40 and all(bool((keep == t).any(1).all()) for t in top.tolist()) and bool((keep[:, -1] == length - 1).all())
+    for h in range(hkv):
+        assert torch.equal(k2[0, :, h], k[0, keep[h], h]) and torch.equal(v2[0, :, h], k2[0, :, h]) and torch.equal(w2[0, h], w[0, h, keep[h]])
+
+
+def test_two_streams_at_once():
+    """Calls of different batches on two streams, interleaved without a wait, give what each gives alone."""
+    from long_vita_amd import ops
+    sets = []
+    for seed, lens, n in ((1, [700, 20000, 90], 5), (2, [3000, 40, 18000, 256], 30)):
+        b, rows = len(lens), max(lens) + n
+        q, k, v = (t.cuda() for t in make(b, n, rows, 10, 2, 128, seed, lens))
+        par = random_parents(b, n, seed, 0).cuda()
+        sets.append((q, k, v, torch.tensor(lens, dtype=torch.int32, device="cuda"), par, torch.rand(b, 2, rows, device="cuda")))
+
+    def step(q, k, v, L, par, w):
+        out, lse = ops.tree_attention(q, k, v, L, parents=par, return_lse=True)
+        w2 = ops.key_weights(q, k, lse, w, L, parents=par)
+        return (out, lse, w2, *ops.evict_cache(k, v, w2, L, 500, sink=4, recent=50))
+    alone = [[t.clone() for t in step(*x)] for x in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = []
+    for _ in range(4):
+        for st, x in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(step(*x))
+    torch.cuda.synchronize()
+    for i, res in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(res, alone[i % 2]))
+
+
 def test_graph_replay():
     from long_vita_amd import ops
     b, rows, hkv, d = 2, 20000, 2, 64
