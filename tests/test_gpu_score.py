@@ -272,6 +272,31 @@ def test_cut_off_bytes(piece):
     assert float((full - out.double()).abs().max()) <= 2.0 ** -8 * float(want.abs().max())
 
 
+@pytest.mark.parametrize("piece", [0, 128])
+def test_rows_past_32_bit_offsets(piece):
+    """A segment whose rows lie behind 2^31 elements (and 2^32 bytes) gives what it gives at the front, bit for bit."""
+    from long_vita_amd import ops
+    n, T, hq, hkv, d = 300, 430000, 40, 8, 128
+    q, k, v, do = (t.cuda() for t in make(n, hq, hkv, d, 81))
+    big = [torch.zeros(T, t.shape[1], d, dtype=torch.bfloat16, device="cuda") for t in (q, k, v, do)]
+    for b, t in zip(big, (q, k, v, do)):
+        b[-n:] = t
+    assert big[0].numel() > 2 ** 31
+    ops.set_split_override(piece, piece)
+    try:
+        res = []
+        for (x, y, z, w), cu in (((q, k, v, do), [0, n]), (big, [T - n, T])):
+            leaves = [t.requires_grad_(True) for t in (x, y, z)]
+            out, lse = ops.score_attention(*leaves, cu, softcap=30.0)
+            res.append((out, lse, torch.autograd.grad(out, leaves, w)))
+    finally:
+        ops.set_split_override(None, None)
+    (o1, l1, g1), (o2, l2, g2) = res
+    assert torch.equal(o2[-n:], o1) and torch.equal(l2[:, -n:], l1)
+    for a, b in zip(g1, g2):
+        assert torch.equal(b[-n:], a) and not b[:1000].any()
+
+
 def test_other_stream_and_graph():
     from long_vita_amd import ops
     q, k, v, do = (t.cuda() for t in make(700, 5, 1, 128, 41))
