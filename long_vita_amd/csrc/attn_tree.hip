@@ -26,7 +26,7 @@
 #include <type_traits>
 
 // [slots of K / V tiles][cum][lens][par][depth][anc][stat]
-#define LV_TREE_LDS_FIXED (LV_TREE_MAX_BATCH * 8 + LV_TREE_MAX_TOKENS * 8 + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4 + 2048)
+#define LV_TREE_LDS_FIXED (LV_TREE_MAX_BATCH * 8 + LV_TREE_MAX_TOKENS * 8 + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32) * 4 + 3072)
 #define LV_TREE_RING (128 * 1024)
 
 template <int WR>
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
     int* const par = lens + LV_TREE_MAX_BATCH;                          // [LV_TREE_MAX_TOKENS]
     int* const depth = par + LV_TREE_MAX_TOKENS;                        // [LV_TREE_MAX_TOKENS]
     uint32_t* const anc = reinterpret_cast<uint32_t*>(depth + LV_TREE_MAX_TOKENS);   // [tokens][words]: a token and its ancestors
-    float* const stat = reinterpret_cast<float*>(anc + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32));   // [2][8 waves][32]
+    float* const stat = reinterpret_cast<float*>(anc + LV_TREE_MAX_TOKENS * (LV_TREE_MAX_TOKENS / 32));   // [3][8 waves][32]
     f32x4* const obuf = reinterpret_cast<f32x4*>(smem);                 // the join's buffer is the ring: [wave][MT][4][lane]
     static_assert(NS * SLOTB >= NW * MT * 4096, "the join fits the ring");
 
@@ -207,6 +207,10 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
 
         f32x16 oacc[MT];
         float m_run = -1e30f, l_run = 0.f;
+        // the sum of P as it was rounded divides O, so that the rounding of a row's largest P cancels (out's error against 64 bits
+        // 0.0023 -> 0.0020; not with WR = 4, whose vector phase it would lengthen by 6 %)
+        constexpr bool PV_SUM = WR < 4;
+        float l_pv = 0.f;
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -262,7 +266,12 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
                 if (__any(!(sum <= OPTIMISTIC_MAX))) exact = true;      // (also catches inf / nan)
                 else l_run += sum;
             }
-            if (!exact) return;
+            auto add_pv = [&]() __attribute__((always_inline)) {
+                if constexpr (PV_SUM)
+#pragma unroll
+                    for (int u = 0; u < SUB; ++u) l_pv = add_bf16x8(pf[u][1], add_bf16x8(pf[u][0], l_pv));
+            };
+            if (!exact) { add_pv(); return; }
             if (masked) {
 #pragma unroll
                 for (int u = 0; u < SUB; ++u) {
@@ -298,12 +307,14 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
                 const float alpha = fast_exp2((m_run - m_new) * c);
                 m_run = m_new;
                 l_run *= alpha;
+                l_pv *= alpha;
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) oacc[mt][i] *= alpha;
             }
             l_run += weigh();
+            add_pv();
         };
         // rows of unused slots hold whatever was there: zero, so that not even a NaN gets through P = 0 (every wave that shares
         // the slice writes the same zeros before it reads)
@@ -469,6 +480,10 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
             stat[w * 32 + r] = m_run;
             stat[256 + w * 32 + r] = l_w;
         }
+        if constexpr (PV_SUM) {
+            const float l_x = pair32_sum(l_pv);
+            if (h == 0) stat[512 + w * 32 + r] = l_x;
+        }
         // (what was asked for past the share's last tile of the sequence brings nothing, but has to be over before the ring is
         // written by hand)
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -479,7 +494,13 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
 #pragma unroll
         for (int i = 0; i < WK; ++i) l_tot += stat[256 + (i * WR + wr) * 32 + r] * fast_exp2((stat[(i * WR + wr) * 32 + r] - m_tot) * c);
         const float sc = fast_exp2((m_run - m_tot) * c);
-        const float inv = (l_tot > 0.f && live) ? 1.f / l_tot : 0.f;
+        float l_o = l_tot;
+        if constexpr (PV_SUM) {
+            l_o = 0.f;
+#pragma unroll
+            for (int i = 0; i < WK; ++i) l_o += stat[512 + (i * WR + wr) * 32 + r] * fast_exp2((stat[(i * WR + wr) * 32 + r] - m_tot) * c);
+        }
+        const float inv = (l_tot > 0.f && live) ? 1.f / l_o : 0.f;
         if (wk == 0 && h == 0) {
             const float x = (l_tot > 0.f && live) ? m_tot * unit2 + __logf(l_tot) : -INFINITY;
             if (!whole) p.part_lse[part + r] = x;
