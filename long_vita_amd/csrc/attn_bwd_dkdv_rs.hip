@@ -224,7 +224,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dkdv_rs_kernel(BwdParams p) {
     const float c = p.scale_log2e;
     float slope_v = 0.f;   // lane g: -log2(e) times the slope of head g of the group (at most 64)
     if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
-        if (lane < p.group) slope_v = -1.4426950408889634f * p.score.slopes[kvh * p.group + lane];
+        if (lane < p.group) slope_v = lv_slope2<MOD>(p.score, kvh * p.group + lane);
         asm volatile("" : "+v"(slope_v));
     }
     const int pre = MOD != 0 ? dsc.prefix : 0;   // keys of the block below this are visible to every row
@@ -556,11 +556,12 @@ static void launch_rs_score(const BwdParams& p, int accum, hipStream_t stream) {
 
 int lv_launch_bwd_dkdv_rs_score(const BwdParams& p, int d, int accum, int mod, hipStream_t stream) {
     if (p.n_blocks <= 0) return 0;
-    switch (mod & (LV_SCORE_CAP | LV_SCORE_BIAS)) {
+    switch (LV_SCORE_BITS(mod)) {
         case 0: d == 128 ? launch_rs_score<128, 4>(p, accum, stream) : launch_rs_score<64, 4>(p, accum, stream); break;
         case LV_SCORE_CAP: d == 128 ? launch_rs_score<128, 5>(p, accum, stream) : launch_rs_score<64, 5>(p, accum, stream); break;
         case LV_SCORE_BIAS: d == 128 ? launch_rs_score<128, 6>(p, accum, stream) : launch_rs_score<64, 6>(p, accum, stream); break;
-        default: d == 128 ? launch_rs_score<128, 7>(p, accum, stream) : launch_rs_score<64, 7>(p, accum, stream);
+        case LV_SCORE_CAP | LV_SCORE_BIAS: d == 128 ? launch_rs_score<128, 7>(p, accum, stream) : launch_rs_score<64, 7>(p, accum, stream); break;
+        default: d == 128 ? launch_rs_score<128, 15>(p, accum, stream) : launch_rs_score<64, 15>(p, accum, stream);
     }
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }

@@ -167,7 +167,7 @@ __global__ __launch_bounds__(512) void lv_bwd_dq_pp_kernel(BwdParams p) {
     asm volatile("" : "+v"(lse2), "+v"(delta));
     float nslope2 = 0.f;
     if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
-        nslope2 = -1.4426950408889634f * p.score.slopes[head];
+        nslope2 = lv_slope2<MOD>(p.score, head);
         asm volatile("" : "+v"(nslope2));
     }
     // With a cap the vector phase is the longer one: dP's accumulators start from -delta, one subtraction per score less
@@ -371,11 +371,12 @@ static void launch_dq_pp_score(const BwdParams& p, int accum, hipStream_t stream
 
 int lv_launch_bwd_dq_pp_score(const BwdParams& p, int d, int accum, int mod, hipStream_t stream) {
     if (p.n_qblocks <= 0) return 0;
-    switch (mod & (LV_SCORE_CAP | LV_SCORE_BIAS)) {
+    switch (LV_SCORE_BITS(mod)) {
         case 0: d == 128 ? launch_dq_pp_score<128, 4>(p, accum, stream) : launch_dq_pp_score<64, 4>(p, accum, stream); break;
         case LV_SCORE_CAP: d == 128 ? launch_dq_pp_score<128, 5>(p, accum, stream) : launch_dq_pp_score<64, 5>(p, accum, stream); break;
         case LV_SCORE_BIAS: d == 128 ? launch_dq_pp_score<128, 6>(p, accum, stream) : launch_dq_pp_score<64, 6>(p, accum, stream); break;
-        default: d == 128 ? launch_dq_pp_score<128, 7>(p, accum, stream) : launch_dq_pp_score<64, 7>(p, accum, stream);
+        case LV_SCORE_CAP | LV_SCORE_BIAS: d == 128 ? launch_dq_pp_score<128, 7>(p, accum, stream) : launch_dq_pp_score<64, 7>(p, accum, stream); break;
+        default: d == 128 ? launch_dq_pp_score<128, 15>(p, accum, stream) : launch_dq_pp_score<64, 15>(p, accum, stream);
     }
     return hipGetLastError() == hipSuccess ? 0 : -2;
 }

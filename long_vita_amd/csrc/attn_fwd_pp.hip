@@ -230,7 +230,7 @@ __global__ __launch_bounds__(512) void lv_fwd_pp_kernel(FwdParams p) {
     float nslope2 = 0.f;
     f32x16 bias0;
     if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
-        nslope2 = -1.4426950408889634f * p.score.slopes[head];
+        nslope2 = lv_slope2<MOD>(p.score, head);
         asm volatile("" : "+v"(nslope2));
         if constexpr (SLOPE_INIT) {
             const float raw = -nslope2 / p.scale_log2e;
@@ -532,11 +532,12 @@ static void launch_pp_score(const FwdParams& p0, int mod, hipStream_t stream) {
     const dim3 grid(p.head_per_xcd ? (unsigned)(((p.hkv + 7) / 8) * 8 * p.n_blocks * p.group)
                                    : (unsigned)((((int64_t)p.n_blocks * p.hkv + 7) / 8) * 8 * p.group)), block(512);
     const size_t lds = (size_t)LV_PP_NS * 2 * 64 * D * 2;
-    switch (mod & (LV_SCORE_CAP | LV_SCORE_BIAS)) {
+    switch (LV_SCORE_BITS(mod)) {
         case 0: hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true, false, LV_SCORE_RULE>), grid, block, lds, stream, p); break;
         case LV_SCORE_CAP: hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true, false, LV_SCORE_RULE | LV_SCORE_CAP>), grid, block, lds, stream, p); break;
         case LV_SCORE_BIAS: hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true, false, LV_SCORE_RULE | LV_SCORE_BIAS>), grid, block, lds, stream, p); break;
-        default: hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true, false, LV_SCORE_RULE | LV_SCORE_CAP | LV_SCORE_BIAS>), grid, block, lds, stream, p);
+        case LV_SCORE_CAP | LV_SCORE_BIAS: hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true, false, LV_SCORE_RULE | LV_SCORE_CAP | LV_SCORE_BIAS>), grid, block, lds, stream, p); break;
+        default: hipLaunchKernelGGL((lv_fwd_pp_kernel<D, true, false, LV_SCORE_RULE | LV_SCORE_CAP | LV_SCORE_BIAS | LV_SCORE_WIDE>), grid, block, lds, stream, p);
     }
 }
 

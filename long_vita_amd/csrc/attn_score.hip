@@ -118,10 +118,12 @@ ScoreRule lv_score_rule(float scale, float softcap, const float* slopes) {
     ScoreRule r;
     r.cap_in = softcap > 0.f ? (float)(2.0 * 1.4426950408889634 * (double)scale / (double)softcap) : 0.f;
     r.cap_out = softcap * 1.4426950408889634f;
+    r.plus0 = softcap > LV_SCORE_WIDE_CAP ? 0.f : r.cap_out;
     r.slopes = slopes;
     return r;
 }
 int lv_score_mod(float softcap, const float* slopes) {
+    if (softcap > LV_SCORE_WIDE_CAP) return LV_SCORE_RULE | LV_SCORE_CAP | LV_SCORE_BIAS | LV_SCORE_WIDE;
     return LV_SCORE_RULE | (softcap > 0.f ? LV_SCORE_CAP : 0) | (slopes ? LV_SCORE_BIAS : 0);
 }
 

@@ -164,7 +164,7 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
     const int rowc = min(row, n_rows - 1);
     const int token = rowc / p.group, head = kvh * p.group + rowc % p.group;
     float nslope2 = 0.f;
-    if constexpr ((MOD & LV_SCORE_BIAS) != 0) nslope2 = -1.4426950408889634f * p.score.slopes[head];
+    if constexpr ((MOD & LV_SCORE_BIAS) != 0) nslope2 = lv_slope2<MOD>(p.score, head);
     const float c = MOD != 0 ? 1.f : p.scale_log2e;
 
     while (tile < tile_end) {
@@ -632,7 +632,8 @@ static void launch_tree(const TreeParams& p, int mod, unsigned blocks, int64_t o
         case 0: hipLaunchKernelGGL((lv_tree_kernel<D, WR, 0>), grid, block, lds, stream, p); break;
         case LV_SCORE_CAP: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_CAP>), grid, block, lds, stream, p); break;
         case LV_SCORE_BIAS: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_BIAS>), grid, block, lds, stream, p); break;
-        default: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_CAP | LV_SCORE_BIAS>), grid, block, lds, stream, p);
+        case LV_SCORE_CAP | LV_SCORE_BIAS: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_CAP | LV_SCORE_BIAS>), grid, block, lds, stream, p); break;
+        default: hipLaunchKernelGGL((lv_tree_kernel<D, WR, LV_SCORE_CAP | LV_SCORE_BIAS | LV_SCORE_WIDE>), grid, block, lds, stream, p);
     }
     if (hipPeekAtLastError() != hipSuccess) return;   // (reported by the caller)
     // a workgroup per row takes the slots side by side; with more rows than the chip holds at once (eight workgroups to a compute
@@ -680,7 +681,7 @@ extern "C" int lvattn_tree(const void* q, const void* k, const void* v, void* ou
     p.o_bs = o_bs; p.o_ns = o_ns; p.o_hs = o_hs;
     p.scale = softmax_scale; p.scale_log2e = softmax_scale * 1.4426950408889634f;
     p.score = lv_score_rule(softmax_scale, softcap, slopes);
-    const int mod = lv_score_mod(softcap, slopes) & (LV_SCORE_CAP | LV_SCORE_BIAS);
+    const int mod = LV_SCORE_BITS(lv_score_mod(softcap, slopes));
     hipStream_t st = (hipStream_t)stream;
     if (d == 128) {
         if (t.wr == 1) launch_tree<128, 1>(p, mod, (unsigned)blocks, join, st);

@@ -28,13 +28,12 @@ __device__ __forceinline__ void weight_dma4(const float* g, uint32_t lds_dst) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "s"(lds_dst) : "memory");
 }
 
-// log2(rho) - lse log2(e) of a row, plus cap_out (0 without a cap) as lv_score_plus wants it: what its scores' exponents start
-// from; -inf for a row that counts for nothing
+// log2(rho) - lse log2(e) of a row, plus what lv_score_plus wants on top: what its scores' exponents start from; -inf for a row that counts for nothing
 __device__ __forceinline__ float row_constant(const WeightParams& p, int s, int token, int head) {
     const float rho = p.row_weight ? p.row_weight[(int64_t)s * p.n + token] : 1.f;
     const float l = p.lse[((int64_t)s * p.n + token) * p.hq + head];
     if (!(rho > 0.f) || !(l > -INFINITY)) return -INFINITY;
-    return (p.row_weight ? __builtin_amdgcn_logf(rho) : 0.f) + (p.score.cap_out - l * 1.4426950408889634f);
+    return (p.row_weight ? __builtin_amdgcn_logf(rho) : 0.f) + (p.score.plus0 - l * 1.4426950408889634f);
 }
 
 // rows that hold no key keep their weights (launched when w_out is not w_in); 1024 rows of one (sequence, KV head) per workgroup,
@@ -160,7 +159,7 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
             rc[tid] = (p.row0 + tid < n_rows && !(p.parents && par[token] == LV_TREE_UNUSED)) ? row_constant(p, s, token, head) : -INFINITY;
             if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
                 rc[SR + tid] = (float)(len + (p.parents ? depth[token] : token));
-                rc[2 * SR + tid] = -1.4426950408889634f * p.score.slopes[head];
+                rc[2 * SR + tid] = lv_slope2<MOD>(p.score, head);
             }
             rtok[tid] = token;
         }
@@ -607,7 +606,8 @@ static void launch_stream(const WeightParams& p, int mod, int rt, unsigned block
         case 0: LV_W(0); break;
         case LV_SCORE_CAP: LV_W(LV_SCORE_CAP); break;
         case LV_SCORE_BIAS: LV_W(LV_SCORE_BIAS); break;
-        default: LV_W((LV_SCORE_CAP | LV_SCORE_BIAS));
+        case LV_SCORE_CAP | LV_SCORE_BIAS: LV_W((LV_SCORE_CAP | LV_SCORE_BIAS)); break;
+        default: LV_W((LV_SCORE_CAP | LV_SCORE_BIAS | LV_SCORE_WIDE));
     }
 #undef LV_W
 }
@@ -625,7 +625,8 @@ static void launch_block(const WeightParams& p, int mod, bool guard, unsigned bl
         case 0: LV_W(0); break;
         case LV_SCORE_CAP: LV_W(LV_SCORE_CAP); break;
         case LV_SCORE_BIAS: LV_W(LV_SCORE_BIAS); break;
-        default: LV_W((LV_SCORE_CAP | LV_SCORE_BIAS));
+        case LV_SCORE_CAP | LV_SCORE_BIAS: LV_W((LV_SCORE_CAP | LV_SCORE_BIAS)); break;
+        default: LV_W((LV_SCORE_CAP | LV_SCORE_BIAS | LV_SCORE_WIDE));
     }
 #undef LV_W
 }
@@ -667,7 +668,7 @@ extern "C" int lv_key_weights(const void* q, const void* k, const float* lse, co
     p.wi_bs = wi_bs; p.wi_hs = wi_hs; p.wo_bs = wo_bs; p.wo_hs = wo_hs;
     p.scale_log2e = softmax_scale * 1.4426950408889634f;
     p.score = lv_score_rule(softmax_scale, softcap, slopes);
-    const int mod = lv_score_mod(softcap, slopes) & (LV_SCORE_CAP | LV_SCORE_BIAS);
+    const int mod = LV_SCORE_BITS(lv_score_mod(softcap, slopes));
     hipStream_t st = (hipStream_t)stream;
     if (t.stream) {
         const int n_rows = n * p.group, rt = n_rows <= 32 ? 1 : (n_rows <= 64 ? 2 : 4);

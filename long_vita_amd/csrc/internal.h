@@ -5,37 +5,68 @@
 // Rules that change a score before the softmax.  A kernel instantiated with MOD != 0 works on t = log2(e) * score, where
 //   score = cap * tanh(scale * q.k / cap)   (LV_SCORE_CAP; else scale * q.k)
 //           - slope[head] * |query position - key position|   (LV_SCORE_BIAS)
-// and always honours the descriptor's prefix (word 7).  tanh(y) = 1 - 2 / (2^(2 y log2 e) + 1): one exponential and one
-// reciprocal, exact limits on both sides (2^x = inf gives 1, 0 gives -1), absolute error of a few 2^-24.
+// and always honours the descriptor's prefix (word 7).  With x = 2 log2(e) scale q.k / cap,
+//   cap tanh = cap (1 - 2 / (2^x + 1)):  one exponential and one reciprocal, exact limits on both sides (2^x = inf gives cap,
+// 0 gives -cap).  The two terms nearly cancel where the score is small beside the cap: the absolute error is about 1.4e-7 cap,
+// 9e-6 at a cap of 64, 1e-3 at 1e4.  Caps above LV_SCORE_WIDE_CAP (LV_SCORE_WIDE) therefore take, for |x| < log2(e) (scores under
+// half the cap),
+//   cap tanh = score (1 + x^2 (a1 + x^2 (a2 + x^2 (a3 + x^2 a4)))),
+// a polynomial fitted to tanh(y) / y for |y| <= 1/2 (least squares, weights moved until the error is level: 1.4e-8); with either
+// form the error is then below 4e-7 of the score itself, whatever the cap.  That costs about ten vector instructions per score,
+// so caps that models train with (20 to 50) do not take it: 8,192 packed rows, 40 / 8 heads, cap 50 / 65, forward 351 / 640 us, training
+// 1,403 / 2,138 us.  The wide kernels always hold the bias (slopes may be null: 0), so that one more variant serves both.
 #define LV_SCORE_CAP 1
 #define LV_SCORE_BIAS 2
 #define LV_SCORE_RULE 4        // set in every MOD: prefix rows, no other rule needed
+#define LV_SCORE_WIDE 8        // with CAP and BIAS
+#define LV_SCORE_WIDE_CAP 64.f
+#define LV_SCORE_BITS(mod) ((mod) & (LV_SCORE_CAP | LV_SCORE_BIAS | LV_SCORE_WIDE))
 struct ScoreRule {
     float cap_in;              // 2 log2(e) scale / cap: the exponent of the tanh from the raw product q.k
     float cap_out;             // cap log2(e)
+    float plus0;               // lv_score_plus: cap_out with a cap up to LV_SCORE_WIDE_CAP, else 0
     const float* slopes;       // [hq], device
 };
 #ifdef __HIPCC__
+// -log2(e) slope of a head (MOD has LV_SCORE_BIAS)
+template <int MOD>
+__device__ __forceinline__ float lv_slope2(const ScoreRule& u, int head) {
+    if constexpr (MOD & LV_SCORE_WIDE) if (!u.slopes) return 0.f;
+    return -1.4426950408889634f * u.slopes[head];
+}
+// log2(e) cap tanh(x ln(2) / 2) of a wide cap; rc = 1 / (2^x + 1), c = scale log2(e)
+__device__ __forceinline__ float lv_score_wide(float s, float c, float x, float rc, const ScoreRule& u) {
+    const float z = x * x, near = s * c;
+    float a = __builtin_fmaf(z, 3.5919336e-06f, -9.193529e-05f);
+    a = __builtin_fmaf(z, a, 0.001922566f);
+    a = __builtin_fmaf(z, a, -0.040037528f);
+    return __builtin_fabsf(x) < 1.4426950f ? __builtin_fmaf(near, z * a, near) : __builtin_fmaf(-2.f * u.cap_out, rc, u.cap_out);
+}
 // raw product s -> t; `dist` = signed distance of the two positions
 template <int MOD>
 __device__ __forceinline__ float lv_score(float s, float c, const ScoreRule& u, float nslope2, float dist) {
     float t;
-    if constexpr (MOD & LV_SCORE_CAP) t = __builtin_fmaf(-2.f * u.cap_out, __builtin_amdgcn_rcpf(fast_exp2(s * u.cap_in) + 1.f), u.cap_out);
+    if constexpr (MOD & LV_SCORE_WIDE) {
+        const float x = s * u.cap_in;
+        t = lv_score_wide(s, c, x, __builtin_amdgcn_rcpf(fast_exp2(x) + 1.f), u);
+    } else if constexpr (MOD & LV_SCORE_CAP) t = __builtin_fmaf(-2.f * u.cap_out, __builtin_amdgcn_rcpf(fast_exp2(s * u.cap_in) + 1.f), u.cap_out);
     else t = s * c;
     if constexpr (MOD & LV_SCORE_BIAS) t = __builtin_fmaf(nslope2, __builtin_fabsf(dist), t);
     return t;
 }
-// t + (plus - lv_score_plus0): with a cap the caller's constant holds cap_out, so that no instruction per score adds it.
+// t + (plus - lv_score_plus0): with a cap (not a wide one, beside which the constant's other terms would be lost) the caller's
+// constant holds cap_out, so that no instruction per score adds it.
 // quarter: a fourth of the tanh's derivative, 1 - tanh^2 = 1 - (1 - 2 rc)^2 = 4 (rc - rc^2); the 4 goes into the caller's last
 // factor.  (Packed segments, 40 / 8 heads, cap 50: dQ 584 -> 577 us, dK / dV 700 -> 678 us.)
 template <int MOD>
-__device__ __forceinline__ float lv_score_plus0(const ScoreRule& u) { return (MOD & LV_SCORE_CAP) ? u.cap_out : 0.f; }
+__device__ __forceinline__ float lv_score_plus0(const ScoreRule& u) { return (MOD & LV_SCORE_CAP) ? u.plus0 : 0.f; }
 template <int MOD>
 __device__ __forceinline__ float lv_score_plus(float s, float c, const ScoreRule& u, float nslope2, float dist, float plus, float* quarter = nullptr) {
     float t;
     if constexpr (MOD & LV_SCORE_CAP) {
-        const float rc = __builtin_amdgcn_rcpf(fast_exp2(s * u.cap_in) + 1.f);
-        t = __builtin_fmaf(-2.f * u.cap_out, rc, plus);
+        const float x = s * u.cap_in, rc = __builtin_amdgcn_rcpf(fast_exp2(x) + 1.f);
+        if constexpr (MOD & LV_SCORE_WIDE) t = lv_score_wide(s, c, x, rc, u) + plus;
+        else t = __builtin_fmaf(-2.f * u.cap_out, rc, plus);
         if (quarter) *quarter = __builtin_fmaf(-rc, rc, rc);
     } else {
         t = __builtin_fmaf(s, c, plus);
