@@ -167,8 +167,10 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
 #pragma unroll
         for (int b = 0; b < RT; ++b) {
             const int row = p.row0 + 32 * b + r, rowc = min(row, n_rows - 1), token = rowc / p.group;
-            const bool on = row < n_rows && (!p.row_weight || p.row_weight[(int64_t)s * p.n + token] > 0.f) && !(p.parents && par[token] == LV_TREE_UNUSED);
-            const __bf16* qp = p.q + (int64_t)s * p.q_bs + (int64_t)token * p.q_ns + (int64_t)(kvh * p.group + rowc % p.group) * p.q_hs + 8 * h;
+            const int head = kvh * p.group + rowc % p.group;
+            const bool on = row < n_rows && (!p.row_weight || p.row_weight[(int64_t)s * p.n + token] > 0.f) && !(p.parents && par[token] == LV_TREE_UNUSED) &&
+                            p.lse[((int64_t)s * p.n + token) * p.hq + head] > -INFINITY;
+            const __bf16* qp = p.q + (int64_t)s * p.q_bs + (int64_t)token * p.q_ns + (int64_t)head * p.q_hs + 8 * h;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 qf[b][ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
@@ -283,14 +285,13 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
 #define LV_WEIGHT_KEYS 128                    // keys per workgroup
 #define LV_WEIGHT_ROWS 64                     // query rows per step
 
-// constants of the rows of (sequence, KV head): [3][rows padded to 64] = exponent offset, position, -log2(e) slope
+// constants of the rows of (sequence, KV head): [3][rows padded to 64] = exponent offset, position, -log2(e) slope; and, per 256
+// rows, whether one of them counts for nothing
 __global__ __launch_bounds__(256) void lv_weight_rows_kernel(WeightParams p) {
     __shared__ int par[LV_TREE_MAX_TOKENS], depth[LV_TREE_MAX_TOKENS];
     const int bh = blockIdx.y, s = bh / p.hkv, kvh = bh % p.hkv;
     if (p.parents) list_tree(p.parents + (int64_t)s * p.parents_bs, p.n, 0, false, par, depth, nullptr, threadIdx.x, 256);
     const int row = blockIdx.x * 256 + threadIdx.x;
-    if (row >= p.rows_pad) return;
-    float* out = p.row_const + (int64_t)bh * 3 * p.rows_pad + row;
     float cst = -INFINITY, pos = 0.f, slope = 0.f;
     if (row < p.n * p.group) {
         const int token = row / p.group, head = kvh * p.group + row % p.group;
@@ -298,12 +299,20 @@ __global__ __launch_bounds__(256) void lv_weight_rows_kernel(WeightParams p) {
         pos = (float)(list_len(p.cache_lens, s, p.rows, p.n) + (p.parents ? depth[token] : token));
         if (p.score.slopes) slope = -1.4426950408889634f * p.score.slopes[head];
     }
+    const int dead = __syncthreads_or(row < p.n * p.group && !(cst > -INFINITY));
+    if (threadIdx.x == 0) p.dead[(int64_t)bh * gridDim.x + blockIdx.x] = dead ? 1u : 0u;
+    if (row >= p.rows_pad) return;
+    float* out = p.row_const + (int64_t)bh * 3 * p.rows_pad + row;
     out[0] = cst;
     out[p.rows_pad] = pos;
     out[2 * (int64_t)p.rows_pad] = slope;
 }
 
 // three workgroups fit a compute unit (without a tree; with one, or with the positions and slopes of a bias in registers, two)
+// GUARD: rows that count for nothing (unused slots, a weight of 0, an lse of -inf) may hold anything, NaN included, so their terms are
+// guarded.  Where only an lse can make such a row (no parents, no row weights), the plain kernel leaves the pieces that have any
+// to a guarded launch behind it (p.rest), whose other workgroups end at once.  A prompt of 8,191 tokens, 40 / 8 heads: 392 us
+// without any such care, 395 so, 411 with a test for such rows inside the loop, 450 with every term guarded.
 template <int D, int MOD, bool GUARD>
 __global__ __launch_bounds__(256, (MOD & LV_SCORE_BIAS) || GUARD ? 2 : 3) void lv_weight_block_kernel(WeightParams p) {
     constexpr int KS = D / 16;
@@ -338,12 +347,24 @@ __global__ __launch_bounds__(256, (MOD & LV_SCORE_BIAS) || GUARD ? 2 : 3) void l
     const float* const wi = p.w_in + (int64_t)s * p.wi_bs + (int64_t)kvh * p.wi_hs;
     float* const wo = p.w_out + (int64_t)s * p.wo_bs + (int64_t)kvh * p.wo_hs;
     if (k0 >= keys) {                     // behind the last key: the weights stay as they are
-        if (piece == 0 && p.w_in != p.w_out)
+        if (piece == 0 && p.w_in != p.w_out && !p.rest)
             for (int j = k0 + tid; j < min(k0 + LV_WEIGHT_KEYS, p.rows); j += 256) wo[j] = wi[j];
         return;
     }
     const int n_rows = p.n * p.group;
     const int words = (p.n + 31) >> 5;
+
+    // the rows that see any key of the block, this piece's share of them
+    int row_lo = 0;
+    if (!p.parents && k0 > len) row_lo = (k0 - len) * p.group / TR * TR;     // a chain: drafted key j is seen from token j on
+    const int steps = (n_rows - row_lo + TR - 1) / TR;
+    const int st0 = (int)((int64_t)steps * piece / p.pieces), st1 = (int)((int64_t)steps * (piece + 1) / p.pieces);
+    if (!GUARD || p.rest) {               // (rows past the last repeat it, in its own step)
+        const uint32_t* flag = p.dead + (int64_t)bh * ((p.rows_pad + 255) >> 8);
+        uint32_t any = 0;
+        for (int i = ((row_lo + st0 * TR) >> 8) + lane; i <= (min(row_lo + st1 * TR, n_rows) - 1) >> 8; i += 64) any |= flag[i];
+        if (__any(st0 < st1 && any != 0) != GUARD) return;        // (the same in all four waves)
+    }
     if (p.parents && k0 + LV_WEIGHT_KEYS > len) list_tree(p.parents + (int64_t)s * p.parents_bs, p.n, words, true, par, depth, anc, tid, 256);
 
     // ---- this wave's keys: two groups of 32, fragments for the whole kernel
@@ -369,11 +390,6 @@ __global__ __launch_bounds__(256, (MOD & LV_SCORE_BIAS) || GUARD ? 2 : 3) void l
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(kf[g][ks]));
 
-    // ---- the rows that see any key of the block, this piece's share of them
-    int row_lo = 0;
-    if (!p.parents && k0 > len) row_lo = (k0 - len) * p.group / TR * TR;     // a chain: drafted key j is seen from token j on
-    const int steps = (n_rows - row_lo + TR - 1) / TR;
-    const int st0 = (int)((int64_t)steps * piece / p.pieces), st1 = (int)((int64_t)steps * (piece + 1) / p.pieces);
 
     // ---- requests: wave w brings rows 16 w .. 16 w + 15 of a step and one of the constants' arrays.  A lane's rows move on by TR
     // per step, so their offsets from the step's first token are carried along instead of divided and multiplied for.
@@ -569,7 +585,7 @@ __global__ __launch_bounds__(256) void lv_weight_join_kernel(WeightParams p) {
 }
 
 // ---------------------------------------------------------------------------
-struct WeightPlan { bool stream; int shares, pieces, key_blocks, rows_pad; int64_t part_floats, const_floats; };
+struct WeightPlan { bool stream; int shares, pieces, key_blocks, rows_pad; int64_t part_floats, const_floats, flags; int64_t bytes() const { return 4 * (part_floats + const_floats + flags); } };
 static WeightPlan weight_plan(int batch, int n, int rows, int hq, int hkv) {
     WeightPlan t{};
     const int n_rows = n * (hq / hkv);
@@ -592,6 +608,7 @@ static WeightPlan weight_plan(int batch, int n, int rows, int hq, int hkv) {
     t.pieces = (int)(g < 1 ? 1 : g);
     t.part_floats = t.pieces > 1 ? (int64_t)t.pieces * batch * hkv * rows : 0;
     t.const_floats = (int64_t)batch * hkv * 3 * t.rows_pad;
+    t.flags = (int64_t)batch * hkv * ((t.rows_pad + 255) / 256);
     return t;
 }
 
@@ -633,8 +650,7 @@ static void launch_block(const WeightParams& p, int mod, bool guard, unsigned bl
 
 extern "C" int64_t lv_key_weights_workspace_bytes(int batch, int n, int rows, int hq, int hkv) {
     if (batch <= 0 || n <= 0 || rows < n || hq <= 0 || hkv <= 0 || hq % hkv || (int64_t)n * (hq / hkv) > 0x7ffff000LL) return 0;
-    const WeightPlan t = weight_plan(batch, n, rows, hq, hkv);
-    return (t.part_floats + t.const_floats) * (int64_t)sizeof(float);
+    return weight_plan(batch, n, rows, hq, hkv).bytes();
 }
 
 extern "C" int lv_key_weights(const void* q, const void* k, const float* lse, const float* row_weight, const float* w_in, float* w_out,
@@ -655,14 +671,14 @@ extern "C" int lv_key_weights(const void* q, const void* k, const float* lse, co
     if (!(softcap >= 0.f) || softcap > 1e30f) return lv_fail(LV_EINVAL, "lv_key_weights: softcap %g must be a finite number above 0 (0: no cap)", (double)softcap);
     if (!(softmax_scale > -1e30f && softmax_scale < 1e30f)) return lv_fail(LV_EINVAL, "lv_key_weights: softmax_scale is not finite");
     const WeightPlan t = weight_plan(batch, n, rows, hq, hkv);
-    const int64_t need = (t.part_floats + t.const_floats) * (int64_t)sizeof(float);
+    const int64_t need = t.bytes();
     if (need && (!workspace || ((uintptr_t)workspace & 15))) return lv_fail(LV_EINVAL, "lv_key_weights: workspace must be there and 16-byte aligned");
     if (workspace_bytes < need) return lv_fail(LV_ESIZE, "lv_key_weights: %lld bytes of workspace needed, room for %lld", (long long)need, (long long)workspace_bytes);
     if ((int64_t)batch * hkv > 65535 || (int64_t)batch * (rows / LV_WEIGHT_TILE + 16) > 0x7fffffffLL) return lv_fail(LV_EINVAL, "lv_key_weights: grid too large");
     WeightParams p{};
     p.q = (const __bf16*)q; p.k = (const __bf16*)k; p.lse = lse; p.row_weight = row_weight; p.w_in = w_in; p.w_out = w_out;
     p.cache_lens = cache_lens; p.parents = parents; p.parents_bs = parents_bs;
-    p.row_const = (float*)workspace; p.part = p.row_const + t.const_floats;
+    p.row_const = (float*)workspace; p.part = p.row_const + t.const_floats; p.dead = (uint32_t*)(p.part + t.part_floats);
     p.batch = batch; p.n = n; p.rows = rows; p.hq = hq; p.hkv = hkv; p.group = hq / hkv; p.pieces = t.pieces; p.shares = t.shares; p.rows_pad = t.rows_pad;
     p.q_bs = q_bs; p.q_ns = q_ns; p.q_hs = q_hs; p.k_bs = k_bs; p.k_rs = k_rs; p.k_hs = k_hs;
     p.wi_bs = wi_bs; p.wi_hs = wi_hs; p.wo_bs = wo_bs; p.wo_hs = wo_hs;
@@ -685,8 +701,10 @@ extern "C" int lv_key_weights(const void* q, const void* k, const float* lse, co
         if (blocks > 0x7fffffffLL) return lv_fail(LV_EINVAL, "lv_key_weights: grid too large");
         hipLaunchKernelGGL(lv_weight_rows_kernel, dim3((unsigned)((t.rows_pad + 255) / 256), (unsigned)(batch * hkv)), dim3(256), 0, st, p);
         const bool guard = parents || row_weight;
-        if (d == 128) launch_block<128>(p, mod, guard, (unsigned)blocks, st);
-        else launch_block<64>(p, mod, guard, (unsigned)blocks, st);
+        for (p.rest = 0; p.rest < (guard ? 1 : 2); ++p.rest) {
+            if (d == 128) launch_block<128>(p, mod, guard || p.rest, (unsigned)blocks, st);
+            else launch_block<64>(p, mod, guard || p.rest, (unsigned)blocks, st);
+        }
         if (t.pieces > 1)
             hipLaunchKernelGGL(lv_weight_join_kernel, dim3((unsigned)((rows + 255) / 256), (unsigned)(batch * hkv)), dim3(256), 0, st, p);
     }

@@ -204,7 +204,8 @@ struct WeightParams {
     int64_t parents_bs;
     float* row_const;            // [batch * hkv][3][rows_pad]
     float* part;                 // [pieces][batch * hkv][rows]
-    int batch, n, rows, hq, hkv, group, pieces, shares, rows_pad, row0;
+    uint32_t* dead;              // [batch * hkv][rows_pad / 256]: a row of these 256 counts for nothing
+    int batch, n, rows, hq, hkv, group, pieces, shares, rows_pad, row0, rest;
     int64_t q_bs, q_ns, q_hs, k_bs, k_rs, k_hs, wi_bs, wi_hs, wo_bs, wo_hs;
     float scale_log2e;
     ScoreRule score;
