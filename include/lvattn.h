@@ -59,6 +59,13 @@ int lvattn_abi_version(void);
  * lockstep kernel with LVATTN_FWD_KERNEL=lockstep LVATTN_FWD_WAVES=4: then 128). */
 int lvattn_fwd_block_m(void);
 const char* lvattn_last_error(void);
+/* For callers that keep memory which a captured launch reads at every replay.  lv_capture_id: 1 and *id = the number of the
+ * capture that `stream` is in, or 0 (not capturing).  lv_capture_watch: from now on the end of that capture's graph is noted (the
+ * graph and every executable graph made from it destroyed); once per capture.  lv_capture_ended: takes up to `max` numbers of
+ * captures whose graphs have ended off the list, returns how many.  Host only, any thread. */
+int lv_capture_id(void* stream, unsigned long long* id);
+int lv_capture_watch(void* stream);
+int lv_capture_ended(unsigned long long* ids, int max);
 
 /* Diagnostic, no counterpart in the reference: the shader clock the chip holds under a dense bf16 MFMA loop (the 2.5
  * PFLOP/s peak assumes 2.4 GHz).  n_workgroups x 4 waves run `iters` x 4 v_mfma_f32_32x32x16_bf16 on the 1024 bf16

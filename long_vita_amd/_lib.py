@@ -24,6 +24,9 @@ _f = C.c_float
 _SIGNATURES = {
     "lvattn_abi_version": (C.c_int, []),
     "lvattn_last_error": (C.c_char_p, []),
+    "lv_capture_id": (_int, [_vp, C.POINTER(C.c_ulonglong)]),
+    "lv_capture_watch": (_int, [_vp]),
+    "lv_capture_ended": (_int, [C.POINTER(C.c_ulonglong), _int]),
     "lvattn_fwd_block_m": (C.c_int, []),
     "lv_build_fwd_blocks": (_int, [_i32p, _int, _int, _i32p, _int]),
     "lv_build_bwd_blocks": (_int, [_i32p, _int, _int, _i32p, _int]),

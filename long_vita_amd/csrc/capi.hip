@@ -5,11 +5,13 @@
 #include "internal.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <vector>
 
 static thread_local char g_err[512] = "";
@@ -31,6 +33,69 @@ int lv_fail(int code, const char* fmt, ...) {   // fail() for the other translat
 }
 
 extern "C" int lvattn_abi_version(void) { return 1; }
+
+// ---------------------------------------------------------------------------
+// The life of captured graphs.  A graph owns a user object whose release, when the graph and the executables made from it are gone,
+// puts the capture's number on a list.  The release runs inside a HIP call on some thread: it allocates nothing and calls nothing.
+// ---------------------------------------------------------------------------
+namespace {
+struct Watch { unsigned long long id; Watch* next; };
+std::atomic<Watch*> g_ended{nullptr};
+void watch_ended(void* p) {
+    Watch* w = (Watch*)p;
+    w->next = g_ended.load();
+    while (!g_ended.compare_exchange_weak(w->next, w)) {}
+}
+int capture_of(void* stream, unsigned long long* id, hipGraph_t* graph) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    if (hipError_t e = hipStreamGetCaptureInfo_v2((hipStream_t)stream, &status, id, graph, nullptr, nullptr))
+        return fail(LV_ELAUNCH, "hipStreamGetCaptureInfo_v2: %s", hipGetErrorString(e));
+    return status == hipStreamCaptureStatusActive ? 1 : 0;
+}
+}  // namespace
+
+extern "C" int lv_capture_id(void* stream, unsigned long long* id) {
+    if (!id) return fail(LV_EINVAL, "lv_capture_id: null id pointer");
+    hipGraph_t graph = nullptr;
+    return capture_of(stream, id, &graph);
+}
+
+extern "C" int lv_capture_watch(void* stream) {
+    unsigned long long id = 0;
+    hipGraph_t graph = nullptr;
+    const int on = capture_of(stream, &id, &graph);
+    if (on < 0) return on;
+    if (!on) return fail(LV_EINVAL, "lv_capture_watch: the stream is not being captured");
+    Watch* w = new (std::nothrow) Watch{id, nullptr};
+    hipUserObject_t object = nullptr;
+    if (!w) return fail(LV_ESIZE, "lv_capture_watch: out of memory");
+    if (hipError_t e = hipUserObjectCreate(&object, w, watch_ended, 1, hipUserObjectNoDestructorSync)) {
+        delete w;
+        return fail(LV_ELAUNCH, "hipUserObjectCreate: %s", hipGetErrorString(e));
+    }
+    if (hipError_t e = hipGraphRetainUserObject(graph, object, 1, hipGraphUserObjectMove)) {
+        (void)hipUserObjectRelease(object, 1);       // (the capture then counts as ended: nothing it would have kept is kept)
+        return fail(LV_ELAUNCH, "hipGraphRetainUserObject: %s", hipGetErrorString(e));
+    }
+    return LV_OK;
+}
+
+extern "C" int lv_capture_ended(unsigned long long* ids, int max) {
+    if (!ids || max < 0) return fail(LV_EINVAL, "lv_capture_ended: null ids pointer or max < 0");
+    Watch* w = g_ended.exchange(nullptr);
+    int n = 0;
+    while (w) {
+        Watch* next = w->next;
+        if (n < max) {
+            ids[n++] = w->id;
+            delete w;
+        } else {
+            watch_ended(w);                          // for the next call
+        }
+        w = next;
+    }
+    return n;
+}
 
 // Forward kernel choice.  Default: the one-wave-per-SIMD kernel ("a4") for head dim 128 when a work item sweeps at least
 // 32,768 keys on average (shorter sweeps take "pp", see fwd_a4 below) and the lockstep kernel for head dim 64; the ping-pong

@@ -853,7 +853,48 @@ def varlen_attention(q, k, v, cu_seqlens: Sequence[int], scale: float | None = N
 # ---------------------------------------------------------------------------
 # autograd: packed attention whose scores follow a rule (tanh cap, distance bias, prefix)
 # ---------------------------------------------------------------------------
+# (capture, table key) -> table: a graph reads its tables at every replay, so they outlive their turn in the cache, and another
+# graph's table of the same packing.  Those whose graph is gone wait in _ended_tables for the next table that is built: a last
+# replay may still be running, and a capture cannot wait for it
 _captured_tables: dict = {}
+_ended_tables: dict = {}
+_watched_captures: set = set()
+
+
+def _capture_number() -> int:
+    n = C.c_ulonglong(0)
+    check(_lib.lib().lv_capture_id(_stream(), C.byref(n)), "lv_capture_id")
+    return n.value
+
+
+def _watch_capture(number: int) -> None:
+    if number not in _watched_captures:
+        check(_lib.lib().lv_capture_watch(_stream()), "lv_capture_watch")
+        _watched_captures.add(number)
+
+
+def _drop_ended_captures(wait: bool) -> None:
+    """Takes the tables whose graphs are gone out of _captured_tables and, with ``wait``, lets them go."""
+    ids = (C.c_ulonglong * 64)()
+    while _watched_captures:
+        n = check(_lib.lib().lv_capture_ended(ids, 64), "lv_capture_ended")
+        ended = set(ids[:n])
+        _watched_captures.difference_update(ended)
+        for key in [k for k in _captured_tables if k[0] in ended]:
+            table = _captured_tables.pop(key)
+            _ended_tables[id(table)] = table
+        if n < 64:
+            break
+    if wait and _ended_tables:
+        torch.cuda.synchronize()
+        _ended_tables.clear()
+
+
+def _keep_for_capture(key, table) -> None:
+    number = _capture_number()
+    _drop_ended_captures(wait=False)
+    _watch_capture(number)
+    _captured_tables[number, key] = table
 
 
 class _ScoreRule:
@@ -884,6 +925,7 @@ class _ScoreRule:
     def tables(self, backward, piece, device) -> SplitTables:
         """Work items on the device; ``comb`` is None and ``ws_rows`` 0 when the sweeps stay whole (``piece`` 0)."""
         def build():
+            _drop_ended_captures(wait=True)
             cu, _pre, pre_p, band = self._host()
             n_comb, ws_rows = C.c_int(0), C.c_int(0)
 
@@ -904,7 +946,7 @@ class _ScoreRule:
                               "stream capture does not allow: call it once, forward and backward, before the capture")
         t = _blocks.get(key, build)
         if capturing:
-            _captured_tables[key] = t       # a graph reads the table at every replay: it outlives its turn in the cache
+            _keep_for_capture(key, t)
         return t
 
 
