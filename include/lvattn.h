@@ -290,7 +290,8 @@ int lvattn_decode_noalloc(const void* q, const void* k, const void* v, void* out
  * counts as -1.  softmax_scale > 0.
  * parents == NULL: a chain (token i sees drafted tokens 0 .. i); n == 1 is the ordinary decode step.  The score rule is
  * lvattn_fwd_score's, with token i at position cache_lens[b] + its depth and cached key j at position j.
- * n <= 256, batch <= 512.  workspace: lvattn_tree_workspace_bytes(...) bytes, contents undefined afterwards, not shared by calls
+ * n <= 256, batch <= 512.  out, lse and workspace must not overlap the inputs or each other.  workspace: lvattn_tree_workspace_bytes(...)
+ * bytes, contents undefined afterwards, not shared by calls
  * that may overlap.  Results do not depend on what lies behind row cache_lens[b] + n. */
 int64_t lvattn_tree_workspace_bytes(int batch, int n, int rows, int hq, int hkv, int d);
 int lvattn_tree(const void* q, const void* k, const void* v, void* out, float* lse, const int32_t* cache_lens, const int32_t* parents,

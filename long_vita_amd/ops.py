@@ -336,14 +336,16 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_lens
     ``cache_lens[s]`` + its depth and cached row j at position j (of an evicted cache that is no longer so).  The rows of tokens
     that are there must be finite (unused slots and rows behind the tokens may hold anything).
 
-    At most 256 tokens per sequence and 512 sequences.  ``out`` must not overlap q, k or v.  ``workspace`` (uint8, at least ``tree_workspace_bytes(...)``) lets a
-    program keep its own; calls that may overlap need one each.  No gradient."""
+    At most 256 tokens per sequence and 512 sequences.  ``out``, ``lse`` and ``workspace`` must not overlap q, k, v or each other (views
+    that lie interleaved in one buffer do not).  ``workspace`` (uint8, at least ``tree_workspace_bytes(...)``) lets a program keep its
+    own; calls that may overlap need one each.  No gradient."""
     who = "tree_attention"
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         raise LvAttnError(f"{who} has no gradient: call it under torch.no_grad() or on tensors that do not require one")
     b, n, rows, hq, hkv, d = _check_cache(q, k, v, cache_lens, who)
     if n > TREE_MAX_TOKENS or b > TREE_MAX_BATCH:
         raise LvAttnError(f"{who}: {b} sequences of {n} tokens (at most {TREE_MAX_BATCH} of {TREE_MAX_TOKENS})")
+    given = (q, k, v)
     k, v = _cache_rows(k, "k", who), _cache_rows(v, "v", who)
     s0, s1, s2, s3 = q.stride()
     if s3 != 1 or q.data_ptr() % 16 or min(s0, s1, s2) < 0 or (s0 | s1 | s2) % 8:
@@ -360,17 +362,21 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_lens
         raise LvAttnError(f"{who}: out must be bf16 [b, n, hq, d] on q's device with a contiguous last dimension")
     elif 0 in out.stride() and any(s == 0 and m > 1 for s, m in zip(out.stride(), out.shape)):
         raise LvAttnError(f"{who}: an expanded tensor cannot be written")
-    elif out.data_ptr() in (q.data_ptr(), k.data_ptr(), v.data_ptr()):
+    elif any(_overlap(out, t) for t in given):
         raise LvAttnError(f"{who}: out must not overlap q, k or v")
     if lse is None:
         lse = torch.empty((b, n, hq), dtype=torch.float32, device=q.device) if return_lse else None
     elif lse.shape != (b, n, hq) or lse.dtype != torch.float32 or lse.device != q.device or not lse.is_contiguous():
         raise LvAttnError(f"{who}: lse must be contiguous fp32 [b, n, hq] on q's device")
+    elif any(_overlap(lse, t) for t in (*given, out)):
+        raise LvAttnError(f"{who}: lse must not overlap q, k, v or out")
     need = tree_workspace_bytes(b, n, rows, hq, hkv, d)
     if workspace is None:
         workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
     elif workspace.dtype != torch.uint8 or workspace.device != q.device or not workspace.is_contiguous() or workspace.numel() < need:
         raise LvAttnError(f"{who}: workspace must be contiguous uint8 of at least {need} bytes on q's device")
+    elif any(_overlap(workspace, t) for t in (*given, cache_lens, out, *(t for t in (lse, parents, slopes) if t is not None))):
+        raise LvAttnError(f"{who}: workspace must not overlap the inputs or results")
     check(_lib.lib().lvattn_tree(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(lse), _ptr(cache_lens), _ptr(parents), p_bs, _ptr(workspace),
                                  workspace.numel(), b, n, rows, hq, hkv, d, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
                                  *out.stride()[:3], scale, cap, _ptr(slopes), _stream()), "lvattn_tree")
@@ -469,13 +475,43 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: tor
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether the address ranges of two tensors meet."""
-    def span(t):
-        return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    if a.numel() == 0 or b.numel() == 0:
+    """Whether two tensors share a byte.  Views that lie interleaved in one buffer (K and V of [b, rows, 2, hkv, d]) do not, and
+    tensors of different storages never do (under 1 us to see; ranges of one storage that do not meet 5, interleaved views 30 to 90)."""
+    if not torch._C._is_alias_of(a, b) or a.numel() == 0 or b.numel() == 0:
         return False
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    a0, b0, size_a, size_b = a.data_ptr(), b.data_ptr(), a.element_size(), b.element_size()
+    if (a0 + size_a * (1 + sum((n - 1) * s for n, s in zip(a.shape, a.stride()))) <= b0 or
+            b0 + size_b * (1 + sum((n - 1) * s for n, s in zip(b.shape, b.stride()))) <= a0):
+        return False
+    unit = math.gcd(size_a, size_b, abs(a0 - b0))
+    # addresses in units: a's are a0 + x, b's b0 + y, x and y sums of multiples of the strides; they meet iff x - y = b0 - a0
+    terms: dict = {}           # stride -> (lowest, highest) multiple in x - y
+    for t, sign, scale in ((a, 1, size_a // unit), (b, -1, size_b // unit)):
+        for n, s in (*((n, s * scale) for n, s in zip(t.shape, t.stride())), (scale, 1)):
+            if n > 1 and s:
+                lo, hi = terms.get(s, (0, 0))
+                terms[s] = (lo, hi + n - 1) if sign > 0 else (lo - n + 1, hi)
+    steps = sorted(terms.items(), reverse=True)
+    below = [(0, 0)]           # the range that the strides from here on can make up, smallest first
+    for s, (lo, hi) in reversed(steps):
+        below.append((below[-1][0] + s * lo, below[-1][1] + s * hi))
+    below.reverse()
+    budget = 4096              # nested strides leave one or two multiples to try at each; anything wilder counts as meeting
+
+    def meet(i: int, rest: int) -> bool:
+        nonlocal budget
+        if not below[i][0] <= rest <= below[i][1]:
+            return False
+        if i == len(steps):
+            return True        # (the range is [0, 0])
+        s, (lo, hi) = steps[i]
+        first, last = max(lo, -((below[i + 1][1] - rest) // s)), min(hi, (rest - below[i + 1][0]) // s)
+        for m in range(first, last + 1):
+            budget -= 1
+            if budget < 0 or meet(i + 1, rest - m * s):
+                return True
+        return False
+    return meet(0, (b0 - a0) // unit)
 
 
 def evict_cache(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, cache_lens: torch.Tensor, keep: int, sink: int = 0, recent: int = 0,
