@@ -557,7 +557,7 @@ def evict_cache(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, cache_le
             raise LvAttnError(f"{who}: out weight must be fp32 [{b}, {hkv}, {keep} or more] with contiguous rows")
         if any(s == 0 and m > 1 for t in out for s, m in zip(t.stride(), t.shape)):
             raise LvAttnError(f"{who}: an expanded tensor cannot be written")
-        if any(_overlap(o, i) for o in out for i in (k, v, weight)) or k_out.data_ptr() == v_out.data_ptr():
+        if any(_overlap(o, i) for o in out for i in (k, v, weight, cache_lens)) or _overlap(k_out, v_out) or _overlap(k_out, w_out) or _overlap(v_out, w_out):
             raise LvAttnError(f"{who}: the out buffers must not overlap each other or the caches they are filled from")
     index = torch.empty((b, hkv, keep), dtype=torch.int32, device=dev)
     lens = torch.empty((b,), dtype=torch.int32, device=dev)
