@@ -413,8 +413,8 @@ def tree_accept(k: torch.Tensor, v: torch.Tensor, cache_lens: torch.Tensor, path
     if weight is not None and (weight.dtype != torch.float32 or weight.shape != (b, hkv, rows) or weight.stride(2) != 1):
         raise LvAttnError(f"{who}: weight must be fp32 [{b}, {hkv}, {rows}] with contiguous rows")
     _cache_rows(k, "k", who), _cache_rows(v, "v", who)
-    if any(s == 0 and m > 1 for t in (k, v) for s, m in zip(t.stride(), t.shape)):
-        raise LvAttnError(f"{who}: an expanded cache cannot be written in place")
+    if any(s == 0 and m > 1 for t in ((k, v) if weight is None else (k, v, weight)) for s, m in zip(t.stride(), t.shape)):
+        raise LvAttnError(f"{who}: an expanded cache or weight cannot be written in place")
     if b and hkv:
         w_s = (0, 0) if weight is None else weight.stride()[:2]
         check(_lib.lib().lv_tree_accept(_ptr(k), _ptr(v), _ptr(weight), _ptr(cache_lens), _ptr(path), _ptr(n_accept), b, path.shape[1], rows, hkv, d,
