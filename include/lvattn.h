@@ -301,11 +301,15 @@ int lvattn_tree(const void* q, const void* k, const void* v, void* out, float* l
                 int64_t o_token_stride, int64_t o_head_stride, float softmax_scale, float softcap, const float* slopes, void* stream);
 /* The accepted path of a tree becomes the cache's next rows, in place: row cache_lens[b] + path[b][i] -> row cache_lens[b] + i
  * for i < n_accept[b] (path [batch, n] int32, ascending token numbers, as a path from the root down is), K and V and, when
- * given, the accumulated weights [batch, hkv, rows] fp32 (batch / head strides).  Rows from cache_lens[b] + n_accept[b] on keep
- * what they hold or held before their row moved. */
+ * given, the accumulated weights [batch, hkv, rows] fp32 (batch / head strides).  Lengths are clamped to [0, rows - n], n_accept to
+ * [0, n].  Rows from cache_lens[b] + n_accept[b] on keep what they hold or held before their row moved.  lv_tree_accept_lens:
+ * new_lens [batch] int32 (or NULL) receives the new lengths, the sum of the two. */
 int lv_tree_accept(void* k, void* v, float* weight, const int32_t* cache_lens, const int32_t* path, const int32_t* n_accept, int batch, int n,
                    int rows, int hkv, int d, int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride, int64_t v_batch_stride,
                    int64_t v_row_stride, int64_t v_head_stride, int64_t w_batch_stride, int64_t w_head_stride, void* stream);
+int lv_tree_accept_lens(void* k, void* v, float* weight, const int32_t* cache_lens, const int32_t* path, const int32_t* n_accept, int32_t* new_lens,
+                        int batch, int n, int rows, int hkv, int d, int64_t k_batch_stride, int64_t k_row_stride, int64_t k_head_stride,
+                        int64_t v_batch_stride, int64_t v_row_stride, int64_t v_head_stride, int64_t w_batch_stride, int64_t w_head_stride, void* stream);
 
 /* ---- eviction by accumulated attention weight -----------------------------------
  * No counterpart in the reference, whose cache only grows.

@@ -80,6 +80,7 @@ _SIGNATURES = {
     "lv_evict_index": (_int, [_vp] * 5 + [_i64] + [_int] * 6 + [_i64, _i64, _vp]),
     "lv_evict_take": (_int, [_vp] * 7 + [_int] * 5 + [_i64] * 16 + [_vp]),
     "lv_tree_accept": (_int, [_vp] * 6 + [_int] * 5 + [_i64] * 8 + [_vp]),
+    "lv_tree_accept_lens": (_int, [_vp] * 7 + [_int] * 5 + [_i64] * 8 + [_vp]),
     "lvattn_decode_noalloc_max_bytes": (_i64, []),
     "lvattn_decode_noalloc": (_int, [_vp, _vp, _vp, _vp, _vp, _int, _int, _int, _int, _int,
                                      _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _f, _int, _vp]),

@@ -705,6 +705,7 @@ __global__ __launch_bounds__(512) void lv_tree_accept_kernel(AcceptParams p) {
     const int s = blockIdx.x / p.hkv, kvh = blockIdx.x % p.hkv;
     const int len = min(max(p.cache_lens[s], 0), p.rows - p.n);
     const int m = min(max(p.n_accept[s], 0), p.n);
+    if (p.new_lens && kvh == 0 && threadIdx.x == 0) p.new_lens[s] = len + m;
     const int cpr = p.d / 8;
     const int* path = p.path + (int64_t)s * p.n;
     const int step = blockDim.x / cpr;
@@ -733,9 +734,9 @@ __global__ __launch_bounds__(512) void lv_tree_accept_kernel(AcceptParams p) {
     }
 }
 
-extern "C" int lv_tree_accept(void* k, void* v, float* weight, const int32_t* cache_lens, const int32_t* path, const int32_t* n_accept, int batch,
-                              int n, int rows, int hkv, int d, int64_t k_bs, int64_t k_rs, int64_t k_hs, int64_t v_bs, int64_t v_rs, int64_t v_hs,
-                              int64_t w_bs, int64_t w_hs, void* stream) {
+extern "C" int lv_tree_accept_lens(void* k, void* v, float* weight, const int32_t* cache_lens, const int32_t* path, const int32_t* n_accept,
+                                   int32_t* new_lens, int batch, int n, int rows, int hkv, int d, int64_t k_bs, int64_t k_rs, int64_t k_hs,
+                                   int64_t v_bs, int64_t v_rs, int64_t v_hs, int64_t w_bs, int64_t w_hs, void* stream) {
     if (!k || !v || !cache_lens || !path || !n_accept) return lv_fail(LV_EINVAL, "lv_tree_accept: null pointer");
     if (d != 64 && d != 128) return lv_fail(LV_EINVAL, "lv_tree_accept: head dim %d (64 or 128)", d);
     if (batch <= 0 || hkv <= 0 || n <= 0 || rows < n) return lv_fail(LV_EINVAL, "lv_tree_accept: bad sizes");
@@ -743,9 +744,15 @@ extern "C" int lv_tree_accept(void* k, void* v, float* weight, const int32_t* ca
         return lv_fail(LV_EINVAL, "lv_tree_accept: k / v must be 16-byte aligned with strides %% 8 == 0");
     if ((int64_t)batch * hkv > 0x7fffffffLL) return lv_fail(LV_EINVAL, "lv_tree_accept: grid too large");
     AcceptParams p{};
-    p.k = (__bf16*)k; p.v = (__bf16*)v; p.weight = weight; p.cache_lens = cache_lens; p.path = path; p.n_accept = n_accept;
+    p.k = (__bf16*)k; p.v = (__bf16*)v; p.weight = weight; p.cache_lens = cache_lens; p.path = path; p.n_accept = n_accept; p.new_lens = new_lens;
     p.n = n; p.rows = rows; p.hkv = hkv; p.d = d;
     p.k_bs = k_bs; p.k_rs = k_rs; p.k_hs = k_hs; p.v_bs = v_bs; p.v_rs = v_rs; p.v_hs = v_hs; p.w_bs = w_bs; p.w_hs = w_hs;
     hipLaunchKernelGGL(lv_tree_accept_kernel, dim3((unsigned)(batch * hkv)), dim3(512), 0, (hipStream_t)stream, p);
     return hipGetLastError() == hipSuccess ? LV_OK : lv_fail(LV_ELAUNCH, "lv_tree_accept: launch failed");
+}
+
+extern "C" int lv_tree_accept(void* k, void* v, float* weight, const int32_t* cache_lens, const int32_t* path, const int32_t* n_accept, int batch,
+                              int n, int rows, int hkv, int d, int64_t k_bs, int64_t k_rs, int64_t k_hs, int64_t v_bs, int64_t v_rs, int64_t v_hs,
+                              int64_t w_bs, int64_t w_hs, void* stream) {
+    return lv_tree_accept_lens(k, v, weight, cache_lens, path, n_accept, nullptr, batch, n, rows, hkv, d, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, w_bs, w_hs, stream);
 }

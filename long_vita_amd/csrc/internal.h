@@ -188,6 +188,7 @@ struct AcceptParams {
     const int32_t* cache_lens;
     const int32_t* path;         // [batch, n] ascending token numbers
     const int32_t* n_accept;     // [batch]
+    int32_t* new_lens;           // [batch] or null
     int n, rows, hkv, d;
     int64_t k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, w_bs, w_hs;
 };

@@ -398,8 +398,8 @@ def tree_accept(k: torch.Tensor, v: torch.Tensor, cache_lens: torch.Tensor, path
     """The accepted path of a draft tree becomes the caches' next rows, in place: row ``cache_lens[s] + path[s, i]`` moves to row
     ``cache_lens[s] + i`` for i < ``n_accept[s]``, in k, v [b, rows, hkv, d] and ``weight`` [b, hkv, rows] when given.  ``path``
     int32 [b, n] holds ascending token numbers (a parent stands before its child); entries past n_accept are not looked at.
-    ``cache_lens`` is at most rows - n and ``n_accept`` 0 to n, as they were for the attention (rows outside are never touched).
-    Returns the new lengths, cache_lens + n_accept."""
+    Lengths are clamped to [0, rows - n], as the attention clamps them, and ``n_accept`` to [0, n].  Returns the new lengths, the sum of
+    the two."""
     who = "tree_accept"
     _require_gpu(k, v, cache_lens, path, n_accept, weight)
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.dim() != 4 or k.shape != v.shape or k.shape[3] not in (64, 128):
@@ -415,11 +415,13 @@ def tree_accept(k: torch.Tensor, v: torch.Tensor, cache_lens: torch.Tensor, path
     _cache_rows(k, "k", who), _cache_rows(v, "v", who)
     if any(s == 0 and m > 1 for t in ((k, v) if weight is None else (k, v, weight)) for s, m in zip(t.stride(), t.shape)):
         raise LvAttnError(f"{who}: an expanded cache or weight cannot be written in place")
-    if b and hkv:
-        w_s = (0, 0) if weight is None else weight.stride()[:2]
-        check(_lib.lib().lv_tree_accept(_ptr(k), _ptr(v), _ptr(weight), _ptr(cache_lens), _ptr(path), _ptr(n_accept), b, path.shape[1], rows, hkv, d,
-                                        *k.stride()[:3], *v.stride()[:3], *w_s, _stream()), "lv_tree_accept")
-    return cache_lens + n_accept
+    if not (b and hkv):
+        return cache_lens.clamp(0, rows - path.shape[1]) + n_accept.clamp(0, path.shape[1])
+    new_lens = torch.empty((b,), dtype=torch.int32, device=k.device)
+    w_s = (0, 0) if weight is None else weight.stride()[:2]
+    check(_lib.lib().lv_tree_accept_lens(_ptr(k), _ptr(v), _ptr(weight), _ptr(cache_lens), _ptr(path), _ptr(n_accept), _ptr(new_lens), b, path.shape[1],
+                                         rows, hkv, d, *k.stride()[:3], *v.stride()[:3], *w_s, _stream()), "lv_tree_accept_lens")
+    return new_lens
 
 
 def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: torch.Tensor, cache_lens: torch.Tensor, scale: float | None = None,
