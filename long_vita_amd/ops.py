@@ -543,6 +543,7 @@ def evict_cache(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, cache_le
     if cache_lens.dtype != torch.int32 or cache_lens.shape != (b,):
         raise LvAttnError(f"{who}: cache_lens must be int32 [{b}]")
     k, v = _cache_rows(k, "k", who), _cache_rows(v, "v", who)
+    cache_lens = cache_lens.contiguous()       # (a copy has to live until the launch)
     dev = k.device
     fresh = out is None
     if fresh:
@@ -565,7 +566,7 @@ def evict_cache(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, cache_le
     lens = torch.empty((b,), dtype=torch.int32, device=dev)
     need = _workspace_bytes("lv_evict_workspace_bytes", b, rows, hkv)
     ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need else None
-    check(_lib.lib().lv_evict_index(_ptr(weight), _ptr(cache_lens.contiguous()), _ptr(index), _ptr(lens), _ptr(ws), need, b, rows, hkv, keep, sink, recent,
+    check(_lib.lib().lv_evict_index(_ptr(weight), _ptr(cache_lens), _ptr(index), _ptr(lens), _ptr(ws), need, b, rows, hkv, keep, sink, recent,
                                     *weight.stride()[:2], _stream()), "lv_evict_index")
     check(_lib.lib().lv_evict_take(_ptr(k), _ptr(v), _ptr(weight), _ptr(index), _ptr(k_out), _ptr(v_out), _ptr(w_out), b, hkv, d, keep, int(fresh),
                                    *k.stride()[:3], *v.stride()[:3], *weight.stride()[:2], *k_out.stride()[:3], *v_out.stride()[:3],
