@@ -15,6 +15,7 @@ from typing import Sequence
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import LV_BWD_BLOCK_N, LV_DESC_INTS, LvAttnError, check
@@ -274,6 +275,18 @@ def decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
     return (out, lse) if return_lse else out
 
 
+def _no_gradient(who: str, *tensors) -> None:
+    """Refuses what an operator without a gradient would drop silently: tensors that require one, tangents of forward mode."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise LvAttnError(f"{who} has no gradient: call it under torch.no_grad() or on tensors that do not require one")
+    _no_tangents(who, *tensors)
+
+
+def _no_tangents(who: str, *tensors) -> None:
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise LvAttnError(f"{who} has no forward-mode derivative: its tensors carry tangents")
+
+
 TREE_MAX_TOKENS = 256       # drafted tokens per sequence of tree_attention
 TREE_MAX_BATCH = 512
 TREE_UNUSED = -2            # parents[] entry of a slot that holds no token
@@ -340,8 +353,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache_lens
     that lie interleaved in one buffer do not).  ``workspace`` (uint8, at least ``tree_workspace_bytes(...)``) lets a program keep its
     own; calls that may overlap need one each.  No gradient."""
     who = "tree_attention"
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        raise LvAttnError(f"{who} has no gradient: call it under torch.no_grad() or on tensors that do not require one")
+    _no_gradient(who, q, k, v)
     b, n, rows, hq, hkv, d = _check_cache(q, k, v, cache_lens, who)
     if n > TREE_MAX_TOKENS or b > TREE_MAX_BATCH:
         raise LvAttnError(f"{who}: {b} sequences of {n} tokens (at most {TREE_MAX_BATCH} of {TREE_MAX_TOKENS})")
@@ -401,6 +413,7 @@ def tree_accept(k: torch.Tensor, v: torch.Tensor, cache_lens: torch.Tensor, path
     Lengths are clamped to [0, rows - n], as the attention clamps them, and ``n_accept`` to [0, n].  Returns the new lengths, the sum of
     the two."""
     who = "tree_accept"
+    _no_gradient(who, k, v, weight)
     _require_gpu(k, v, cache_lens, path, n_accept, weight)
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.dim() != 4 or k.shape != v.shape or k.shape[3] not in (64, 128):
         raise LvAttnError(f"{who}: expects bfloat16 caches [b, rows, hkv, 64 or 128]")
@@ -436,8 +449,7 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: tor
     turned down) or whose lse is -inf counts for nothing, whatever its row of q holds.  Returns a new tensor, or ``out`` (fp32
     [b, hkv, rows]; ``weight`` itself for an update in place).  Weights of rows that hold no key are carried over.  No gradient."""
     who = "key_weights"
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad):
-        raise LvAttnError(f"{who} has no gradient: call it under torch.no_grad() or on tensors that do not require one")
+    _no_gradient(who, q, k, lse, weight, row_weight)
     b, n, rows, hq, hkv, d = _check_cache(q, k, None, cache_lens, who)
     _require_gpu(lse, weight, row_weight, out)
     k = _cache_rows(k, "k", who)
@@ -529,9 +541,8 @@ def evict_cache(k: torch.Tensor, v: torch.Tensor, weight: torch.Tensor, cache_le
     ``out`` = (k, v, weight) buffers with ``keep`` rows or more that must not overlap the old ones: their first rows are written,
     all others are left as they are."""
     who = "evict_cache"
+    _no_gradient(who, k, v, weight)
     _require_gpu(k, v, weight, cache_lens)
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad or weight.requires_grad):
-        raise LvAttnError(f"{who} has no gradient: call it under torch.no_grad() or on tensors that do not require one")
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or k.dim() != 4 or k.shape != v.shape or k.shape[3] not in (64, 128) or 0 in k.shape:
         raise LvAttnError(f"{who}: expects bfloat16 caches [b, rows, hkv, 64 or 128]")
     b, rows, hkv, d = k.shape
@@ -1095,6 +1106,7 @@ def _check_rule_args(hq, hkv, softcap, slopes, device, who):
             raise LvAttnError(f"{who}: alibi_slopes must be an fp32 tensor [{hq}] (one slope per query head)")
         if slopes.requires_grad:
             raise LvAttnError(f"{who}: alibi_slopes get no gradient; pass a tensor that does not require one")
+        _no_tangents(who, slopes)
         if slopes.device != device:
             raise LvAttnError(f"{who}: alibi_slopes live on {slopes.device}, the queries on {device}")
         if hkv and hq // hkv > 64:
@@ -1117,6 +1129,7 @@ def score_attention(q, k, v, cu_seqlens: Sequence[int], scale: float | None = No
     for t in (q, k, v):
         if not isinstance(t, torch.Tensor):
             raise LvAttnError("score_attention: q, k, v must be tensors")
+    _no_tangents("score_attention", q, k, v)
     _check_qkv(q, k, v)
     if q.shape[0] != k.shape[0]:
         raise LvAttnError(f"score_attention: {q.shape[0]} query rows and {k.shape[0]} key rows (packed self attention has as many of both)")
