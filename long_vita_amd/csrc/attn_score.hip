@@ -116,7 +116,8 @@ int check_rule(int d, int hq, int hkv, float softmax_scale, float softcap, const
 
 ScoreRule lv_score_rule(float scale, float softcap, const float* slopes) {
     ScoreRule r;
-    r.cap_in = softcap > 0.f ? (float)(2.0 * 1.4426950408889634 * (double)scale / (double)softcap) : 0.f;
+    // (finite whatever the two are: a raw product of 0 stays 0)
+    r.cap_in = softcap > 0.f ? (float)std::clamp(2.0 * 1.4426950408889634 * (double)scale / (double)softcap, -3e38, 3e38) : 0.f;
     r.cap_out = softcap * 1.4426950408889634f;
     r.plus0 = softcap > LV_SCORE_WIDE_CAP ? 0.f : r.cap_out;
     r.slopes = slopes;

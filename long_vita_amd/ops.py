@@ -1099,8 +1099,10 @@ class _ScoreAttention(torch.autograd.Function):
 def _check_rule_args(hq, hkv, softcap, slopes, device, who):
     """softcap as a float (0 = none) and the slopes as contiguous fp32 on the device."""
     cap = 0.0 if softcap is None else float(softcap)
-    if softcap is not None and not (0.0 < cap < 1e30):
-        raise LvAttnError(f"{who}: softcap must be a finite number above 0 (None for no cap), not {softcap!r}")
+    if softcap is not None:
+        if not 0.0 < cap < 1e30:
+            raise LvAttnError(f"{who}: softcap must be a number above 0 and below 1e30 (None for no cap), not {softcap!r}")
+        cap = max(cap, 2.0 ** -126)       # below fp32's numbers a cap would read as none; either way every score is 0 beside 1
     if slopes is not None:
         if not isinstance(slopes, torch.Tensor) or slopes.dtype != torch.float32 or slopes.shape != (hq,):
             raise LvAttnError(f"{who}: alibi_slopes must be an fp32 tensor [{hq}] (one slope per query head)")
