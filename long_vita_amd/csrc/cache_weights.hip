@@ -158,7 +158,7 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
             const int tc = min(p.row0 + tid, n_rows - 1), token = tc / p.group, head = kvh * p.group + tc % p.group;
             rc[tid] = (p.row0 + tid < n_rows && !(p.parents && par[token] == LV_TREE_UNUSED)) ? row_constant(p, s, token, head) : -INFINITY;
             if constexpr ((MOD & LV_SCORE_BIAS) != 0) {
-                rc[SR + tid] = (float)(len + (p.parents ? depth[token] : token));
+                rc[SR + tid] = (float)(p.parents ? depth[token] : token);
                 rc[2 * SR + tid] = lv_slope2<MOD>(p.score, head);
             }
             rtok[tid] = token;
@@ -213,9 +213,10 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
                 const float old = *(LDS_PTR(float, kb + 32 * ROWB + 4 * r));
                 const bool masked = kb0 + 32 > len;
                 const int jt = key - len;
-                float kpos = (float)key;
+                // positions count from the sequence's length: exact where it matters, also in caches of more than 2^24 keys
+                float kpos = (float)jt;
                 if constexpr ((MOD & LV_SCORE_BIAS) != 0)
-                    if (p.parents && jt >= 0 && jt < p.n) kpos = (float)(len + depth[jt]);
+                    if (p.parents && jt >= 0 && jt < p.n) kpos = (float)depth[jt];
                 float sum = 0.f;
                 int row_of = 4 * h;       // (with four row tiles the constants are read from LDS every time: the registers are full)
                 if constexpr (RT > 2) asm volatile("" : "+v"(row_of));
@@ -285,7 +286,7 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
 #define LV_WEIGHT_KEYS 128                    // keys per workgroup
 #define LV_WEIGHT_ROWS 64                     // query rows per step
 
-// constants of the rows of (sequence, KV head): [3][rows padded to 64] = exponent offset, position, -log2(e) slope; and, per 256
+// constants of the rows of (sequence, KV head): [3][rows padded to 64] = exponent offset, position behind the cache, -log2(e) slope; and, per 256
 // rows, whether one of them counts for nothing
 __global__ __launch_bounds__(256) void lv_weight_rows_kernel(WeightParams p) {
     __shared__ int par[LV_TREE_MAX_TOKENS], depth[LV_TREE_MAX_TOKENS];
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(256) void lv_weight_rows_kernel(WeightParams p) {
     if (row < p.n * p.group) {
         const int token = row / p.group, head = kvh * p.group + row % p.group;
         if (!(p.parents && par[token] == LV_TREE_UNUSED)) cst = row_constant(p, s, token, head);
-        pos = (float)(list_len(p.cache_lens, s, p.rows, p.n) + (p.parents ? depth[token] : token));
+        pos = (float)(p.parents ? depth[token] : token);
         if (p.score.slopes) slope = -1.4426950408889634f * p.score.slopes[head];
     }
     const int dead = __syncthreads_or(row < p.n * p.group && !(cst > -INFINITY));
@@ -381,9 +382,9 @@ __global__ __launch_bounds__(256, (MOD & LV_SCORE_BIAS) || GUARD ? 2 : 3) void l
         const int off = (int)(r * p.k_rs * 2) + 16 * h;
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) kf[g][ks] = __builtin_bit_cast(bf16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, off + 32 * ks, 0, 0));
-        kpos[g] = (float)key[g];
+        kpos[g] = (float)(key[g] - len);
         if constexpr ((MOD & LV_SCORE_BIAS) != 0)
-            if (p.parents && key[g] >= len && key[g] < keys) kpos[g] = (float)(len + depth[key[g] - len]);
+            if (p.parents && key[g] >= len && key[g] < keys) kpos[g] = (float)depth[key[g] - len];
     }
 #pragma unroll
     for (int g = 0; g < 2; ++g)
