@@ -447,7 +447,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: tor
 
     ``row_weight`` (fp32 [b, n]) weighs the tokens' contributions; a token whose weight is not above 0 (a drafted token that was
     turned down) or whose lse is -inf counts for nothing, whatever its row of q holds.  Returns a new tensor, or ``out`` (fp32
-    [b, hkv, rows]; ``weight`` itself for an update in place).  Weights of rows that hold no key are carried over.  No gradient."""
+    [b, hkv, rows]; ``weight`` itself for an update in place; it must not overlap the other inputs).  Weights of rows that hold no key
+    are carried over.  No gradient."""
     who = "key_weights"
     _no_gradient(who, q, k, lse, weight, row_weight)
     b, n, rows, hq, hkv, d = _check_cache(q, k, None, cache_lens, who)
@@ -462,11 +463,14 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: tor
     for name, t in (("weight", weight), ("out", out)):
         if t is not None and (t.dtype != torch.float32 or t.shape != (b, hkv, rows) or t.stride(2) != 1 or min(t.stride()) < 0):
             raise LvAttnError(f"{who}: {name} must be fp32 [{b}, {hkv}, {rows}] with contiguous rows")
+    given_out = out is not None
     if out is None:
         out = torch.empty((b, hkv, rows), dtype=torch.float32, device=q.device)
     elif out.data_ptr() != weight.data_ptr() or out.stride() != weight.stride():
         if _overlap(out, weight):
             raise LvAttnError(f"{who}: out must be weight itself or not overlap it")
+    if given_out and any(_overlap(out, t) for t in (q, k, lse, cache_lens, parents, row_weight, alibi_slopes) if t is not None):
+        raise LvAttnError(f"{who}: out must not overlap the other inputs")
     if 0 in out.stride() and any(x == 0 and m > 1 for x, m in zip(out.stride(), out.shape)):
         raise LvAttnError(f"{who}: an expanded tensor cannot be written")
     s0, s1, s2, s3 = q.stride()
