@@ -463,14 +463,12 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: tor
     for name, t in (("weight", weight), ("out", out)):
         if t is not None and (t.dtype != torch.float32 or t.shape != (b, hkv, rows) or t.stride(2) != 1 or min(t.stride()) < 0):
             raise LvAttnError(f"{who}: {name} must be fp32 [{b}, {hkv}, {rows}] with contiguous rows")
-    given_out = out is not None
+    given = None if out is None else (q, k, lse, cache_lens, parents, row_weight, alibi_slopes)      # (before any of them is copied)
     if out is None:
         out = torch.empty((b, hkv, rows), dtype=torch.float32, device=q.device)
     elif out.data_ptr() != weight.data_ptr() or out.stride() != weight.stride():
         if _overlap(out, weight):
             raise LvAttnError(f"{who}: out must be weight itself or not overlap it")
-    if given_out and any(_overlap(out, t) for t in (q, k, lse, cache_lens, parents, row_weight, alibi_slopes) if t is not None):
-        raise LvAttnError(f"{who}: out must not overlap the other inputs")
     if 0 in out.stride() and any(x == 0 and m > 1 for x, m in zip(out.stride(), out.shape)):
         raise LvAttnError(f"{who}: an expanded tensor cannot be written")
     s0, s1, s2, s3 = q.stride()
@@ -484,6 +482,8 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: tor
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not math.isfinite(scale):
         raise LvAttnError(f"{who}: scale {scale} is not finite")
+    if given and any(_overlap(out, t) for t in given if t is not None):
+        raise LvAttnError(f"{who}: out must not overlap the other inputs")
     need = _workspace_bytes("lv_key_weights_workspace_bytes", b, n, rows, hq, hkv)
     ws = torch.empty((need,), dtype=torch.uint8, device=q.device) if need else None
     check(_lib.lib().lv_key_weights(_ptr(q), _ptr(k), _ptr(lse), _ptr(row_weight), _ptr(weight), _ptr(out), _ptr(cache_lens), _ptr(parents), p_bs,

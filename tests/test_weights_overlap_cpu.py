@@ -54,3 +54,11 @@ def test_out_holds_an_input(launches, name, in_place):
     with pytest.raises(_lib.LvAttnError, match="overlap"):
         ops.key_weights(**a, out=out)
     assert not launches
+
+
+@pytest.mark.parametrize("name,bad", [("parents", [-1, 0, 1]), ("alibi_slopes", [0.0] * HQ)])
+def test_types_are_looked_at_first(launches, name, bad):
+    a = inputs()
+    a[name] = bad
+    with pytest.raises(_lib.LvAttnError, match=name):
+        ops.key_weights(**a, out=torch.zeros(B, HKV, ROWS))
