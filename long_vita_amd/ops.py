@@ -277,9 +277,12 @@ def decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: f
 
 def _no_gradient(who: str, *tensors) -> None:
     """Refuses what an operator without a gradient would drop silently: tensors that require one, tangents of forward mode."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise LvAttnError(f"{who} has no gradient: call it under torch.no_grad() or on tensors that do not require one")
-    _no_tangents(who, *tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise LvAttnError(f"{who} has no gradient: call it under torch.no_grad() or on tensors that do not require one")
+    if _forward_ad._current_level >= 0:
+        _no_tangents(who, *tensors)
 
 
 def _no_tangents(who: str, *tensors) -> None:
