@@ -317,8 +317,10 @@ int lv_tree_accept_lens(void* k, void* v, float* weight, const int32_t* cache_le
  *   row_weight[b, i] * exp(t_ij - lse[b, i, h]): what the attention of lvattn_tree (same tokens, keys, tree and score rule; lse is
  *   its output) gave to key j.  n tokens per sequence: one decode step, a tree (n <= 256 with parents), or a whole prompt
  *   (parents == NULL, cache_lens 0).  row_weight [batch, n] fp32 or NULL (1); a token whose weight is not above 0 counts for nothing,
- *   whatever its row holds.  w_in / w_out [batch, hkv, rows] fp32 with batch / head strides, w_out may be w_in; weights of rows
- *   that are no keys are carried over.  Sums are compensated fp32 in a fixed order.  workspace may be NULL when
+ *   and neither does a (token, head) whose lse is -inf or NaN, whatever their rows of q hold.  w_in / w_out [batch, hkv, rows] fp32 with batch / head strides, w_out may be w_in; weights of rows
+ *   that are no keys are carried over.  Sums are fp32 in a fixed order: compensated for more than 256 query rows per KV head or 512
+ *   sequences, their pieces then added one after the other (at most one per 512 rows, 2^-24 of the sum each); up to 256 rows pairwise (at most 11
+ *   additions on a term's way, 2^-24 each).  workspace may be NULL when
  *   lv_key_weights_workspace_bytes is 0.
  * lv_evict_index: index[b][kvh][0 .. min(len, keep)) = the rows to keep, ascending: all when cache_lens[b] <= keep, else rows
  *   [0, sink), the last `recent`, and the heaviest of those between (ties: the lower row; NaN is heaviest), keep in all.  -1 behind

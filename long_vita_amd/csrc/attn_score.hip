@@ -9,8 +9,10 @@
 // The products are those of plain attention, so the kernels are the ping-pong forward, the ping-pong dQ and the role-split
 // dK/dV kernels instantiated with the rule applied to every raw product in their vector phase (lv_score in internal.h).  What
 // the rule needs is not the matrix pipe: a cap adds an exponential and a reciprocal to the one exponential of the softmax.
-// Measured, 40 / 8 heads of 128, forward / dQ / dK and dV: 8,192 packed rows with a cap 420 / 560 / 650 us, 12,288 rows with
-// slopes 1,570 / 2,020 / 3,360 us (without a rule 1,710 / 2,360 / 3,430 us on these kernels' plain forms).
+// Measured, 40 / 8 heads of 128, forward / dQ / dK and dV within a training step: 8,192 packed rows with a cap 420 / 524 / 658 us,
+// 12,288 rows with slopes 1,705 / 2,077 / 3,441 us.  With the cap the matrix pipe is busy 27 / 33 / 32 % of the cycles and vector
+// instructions issue in 43 / 38 / 43 % of them: neither is full, the chain exponential - reciprocal - exponential of a tile is waited
+// for.  With slopes 43 / 57 / 42 % and 39 / 48 / 41 %.
 // This file holds the host side: work-item tables that know the prefix and the band (whole sweeps or sweeps cut into
 // pieces), the choice of the piece length, and the entry points.
 #include "internal.h"

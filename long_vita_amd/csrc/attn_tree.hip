@@ -17,7 +17,11 @@
 // goes to partial slot g + s (the pairs (g, s) along the list only ever step forward, so the sum is unique) and a second kernel
 // joins a sequence's slots in order.
 //
-// Measured: 64 tokens over 131,000 keys, 40 / 8 heads, 224 us (768 TFLOP/s); 8 tokens over 1,040,000 keys, 5 / 1 heads, 105 us
+// With 128 rows per workgroup and heads of 128 the registers do not hold everything: 9 to 28 vector registers spill, outside the
+// tile loop.
+//
+// Measured: 64 tokens over 131,000 keys, 40 / 8 heads, 225 us (763 TFLOP/s; three blocks of 128 rows for 320 rows and 10 shares each
+// leave 16 of the 256 compute units without work); 8 tokens over 1,040,000 keys, 5 / 1 heads, 105 us
 // (5.1 TB/s); one token over 1,048,576 keys, 40 / 8 heads, 718 us (6.0 TB/s); 25 tokens over 8 caches of 0 to 16,001 keys 63 us.
 #include "cache_list.h"
 #include "../../include/lvattn.h"
@@ -531,7 +535,7 @@ __global__ __launch_bounds__(TreeShape<WR>::THREADS, 2) void lv_tree_kernel(Tree
 }
 
 // out / lse of a row = the log-sum-exp merge of its sequence's slots; every sum has a fixed order.  D / 4 threads take a slot's
-// columns; the 1024 / D groups of them share one row's slots (JR = 1: many shares per sequence) or take a row each (few).
+// columns; the 1024 / D groups of them share one row's slots (ONE_ROW: few rows) or take a row each (many).
 template <int D, int WR, bool ONE_ROW>
 __global__ __launch_bounds__(256) void lv_tree_join_kernel(TreeParams p) {
     constexpr int rows_pb = 32 * WR;

@@ -18,8 +18,13 @@
 //   multiply-adds and adds per 32 x 32 scores, so the vector work bounds it; few rows pay for every 128 keys' loads (125 rows
 //   of the 16 ragged caches below: 192 us, streamed 68 us).
 //
-// Measured, 40 / 8 heads of 128: one token over 4 caches of 7,777 to 65,536 keys 65 us (47 us streaming, 5.8 TB/s; 6 us copying
-// the unused rows); a prompt of 8,191 tokens 386 us (890 TFLOP/s).
+// Registers: the streaming kernel with four row tiles of 128 spills 16 to 45 vector registers (73 with a wide cap); with a cap and
+// slopes some are reloaded inside the tile loop, and such a wait is also one for the requests on their way.  The other kernel's spills
+// (5 to 7, heads of 128 without slopes) lie outside its loop.
+//
+// Measured, 40 / 8 heads of 128: one token over 4 caches of 7,777 to 65,536 keys 65 us (48 us streaming, 5.7 TB/s; 5 us copying
+// the unused rows); a prompt of 8,191 tokens 398 us (864 TFLOP/s); trees of 25 / 32 / 51 / 64 / 128 tokens over 16 ragged caches of
+// 107K keys, in place, 70 / 126 / 135 / 207 / 338 us.
 #include "cache_list.h"
 #include "../../include/lvattn.h"
 

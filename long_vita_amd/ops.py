@@ -449,7 +449,7 @@ def key_weights(q: torch.Tensor, k: torch.Tensor, lse: torch.Tensor, weight: tor
     tree (at most 256 with ``parents``) or a whole prompt (``cache_lens`` 0, no parents).
 
     ``row_weight`` (fp32 [b, n]) weighs the tokens' contributions; a token whose weight is not above 0 (a drafted token that was
-    turned down) or whose lse is -inf counts for nothing, whatever its row of q holds.  Returns a new tensor, or ``out`` (fp32
+    turned down) or whose lse is -inf or NaN counts for nothing, whatever its row of q holds.  Returns a new tensor, or ``out`` (fp32
     [b, hkv, rows]; ``weight`` itself for an update in place; it must not overlap the other inputs).  Weights of rows that hold no key
     are carried over.  No gradient."""
     who = "key_weights"
@@ -1134,7 +1134,9 @@ def score_attention(q, k, v, cu_seqlens: Sequence[int], scale: float | None = No
     visible to all of its rows, as the tokens of an image that opens a sample are; a length past the segment means the whole
     segment.  ``band`` (causal only, not with prefix_lens): a query sees itself and the ``band`` keys before it.
     Rows outside every segment come back as zeros with lse -inf.  ``alibi_slopes`` (fp32 [Hq] on q's device) are constants.  As in
-    ``varlen_attention`` a segment's k and v must be finite: a key that a row does not see has weight 0, and 0 * NaN is NaN."""
+    ``varlen_attention`` a segment's k and v must be finite: a key that a row does not see has weight 0, and 0 * NaN is NaN.
+    ``softcap`` is above 0 and below 1e30; beyond 64 the scores are formed by a longer formula that keeps small scores beside a large
+    cap (half again the time).  No forward-mode derivative."""
     for t in (q, k, v):
         if not isinstance(t, torch.Tensor):
             raise LvAttnError("score_attention: q, k, v must be tensors")
