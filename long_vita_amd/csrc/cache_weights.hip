@@ -18,13 +18,13 @@
 //   multiply-adds and adds per 32 x 32 scores, so the vector work bounds it; few rows pay for every 128 keys' loads (125 rows
 //   of the 16 ragged caches below: 192 us, streamed 68 us).
 //
-// Registers: the streaming kernel with four row tiles of 128 spills 16 to 45 vector registers (73 with a wide cap); with a cap and
+// Registers: the streaming kernel with four row tiles of 128 spills 16 to 57 vector registers (97 with a wide cap); with a cap and
 // slopes some are reloaded inside the tile loop, and such a wait is also one for the requests on their way.  The other kernel's spills
 // (5 to 7, heads of 128 without slopes) lie outside its loop.
 //
 // Measured, 40 / 8 heads of 128: one token over 4 caches of 7,777 to 65,536 keys 65 us (48 us streaming, 5.7 TB/s; 5 us copying
 // the unused rows); a prompt of 8,191 tokens 398 us (864 TFLOP/s); trees of 25 / 32 / 51 / 64 / 128 tokens over 16 ragged caches of
-// 107K keys, in place, 70 / 126 / 135 / 207 / 338 us.
+// 107K keys, in place, 67 / 126 / 135 / 207 / 338 us.
 #include "cache_list.h"
 #include "../../include/lvattn.h"
 
@@ -172,15 +172,9 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
 #pragma unroll
         for (int b = 0; b < RT; ++b) {
             const int row = p.row0 + 32 * b + r, rowc = min(row, n_rows - 1), token = rowc / p.group;
-            const int head = kvh * p.group + rowc % p.group;
-            const bool on = row < n_rows && (!p.row_weight || p.row_weight[(int64_t)s * p.n + token] > 0.f) && !(p.parents && par[token] == LV_TREE_UNUSED) &&
-                            p.lse[((int64_t)s * p.n + token) * p.hq + head] > -INFINITY;
-            const __bf16* qp = p.q + (int64_t)s * p.q_bs + (int64_t)token * p.q_ns + (int64_t)head * p.q_hs + 8 * h;
+            const __bf16* qp = p.q + (int64_t)s * p.q_bs + (int64_t)token * p.q_ns + (int64_t)(kvh * p.group + rowc % p.group) * p.q_hs + 8 * h;
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                qf[b][ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
-                if (!on) qf[b][ks] = bf16x8{};      // a row that counts for nothing may hold anything
-            }
+            for (int ks = 0; ks < KS; ++ks) qf[b][ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
         }
         // every ordinary load and store retires here: from now on the counter holds requests and the loop's stores
 #pragma unroll
@@ -189,6 +183,11 @@ __global__ __launch_bounds__(512, 2) void lv_weight_stream_kernel(WeightParams p
             for (int ks = 0; ks < KS; ++ks) asm volatile("" : "+v"(qf[b][ks]));
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
+#pragma unroll
+        for (int b = 0; b < RT; ++b)                // a row that counts for nothing may hold anything
+            if (!(rc[32 * b + r] > -INFINITY))
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) qf[b][ks] = bf16x8{};
 
         int sl = 0;
         for (int t = t0; t < t1; ++t) {
