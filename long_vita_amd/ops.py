@@ -943,7 +943,8 @@ def _drop_ended_captures(wait: bool) -> None:
         if n < 64:
             break
     if wait and _ended_tables:
-        torch.cuda.synchronize()
+        for device in {t.desc.device for t in _ended_tables.values()}:
+            torch.cuda.synchronize(device)
         _ended_tables.clear()
 
 

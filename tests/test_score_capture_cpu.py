@@ -38,7 +38,7 @@ def played(monkeypatch):
     monkeypatch.setattr(ops, "_watched_captures", set(), raising=False)
     monkeypatch.setattr(ops, "_blocks", ops._BlockCache(4))
     monkeypatch.setattr(ops, "_ended_tables", {}, raising=False)
-    monkeypatch.setattr(torch.cuda, "synchronize", lambda: state.__setitem__("waits", state.get("waits", 0) + (state["capture"] == 0)))
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device: state.__setitem__("waits", state.get("waits", 0) + (state["capture"] == 0)))
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capture"] != 0)
     return state
 
